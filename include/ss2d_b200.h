@@ -496,6 +496,64 @@ typedef struct ss2d_relayout_params {
 int ss2d_pixels_norm_to_planes(const ss2d_relayout_params *p, void *cuda_stream);
 int ss2d_planes_to_pixels(const ss2d_relayout_params *p, void *cuda_stream);
 
+/* ------------------------------------------------------------------------------------
+ * Linear attention with a decay for each head (the scan of the m0 family of SS2D, classification/models/vmamba.py:717-911, in attention's terms:
+ * C, B and x dt are q, k and v, dt A is log_decay).  For every sequence b and head h, with group h / (heads / n_groups) of q and k:
+ *   S_t = exp(log_decay_t) S_{t-1} + k_t v_t^T          S (dk, dv) fp32, S_0 = initial_state or zero
+ *   out_t = scale S_t^T q_t
+ * q, k: (batch, seqlen, n_groups, dk), v: (batch, seqlen, heads, dv), of `dtype`, last dimension contiguous, the others strided (elements,
+ * >= 0: heads that share rows have a stride of 0); log_decay: (batch, seqlen, heads) fp32, strided.  -inf resets the state; values are meant
+ * to be <= 0.  out: (batch, seqlen, heads, dv) of `dtype`, dense; initial_state, final_state: (batch, heads, dk, dv) fp32, dense, NULL where
+ * there is none.  chunk_states: NULL, or fp32 (batch, heads, ceil(seqlen / 64), dk, dv), the state in front of every 64th token, which the backward
+ * call needs.  dk and dv up to 128 (else SS2D_ENOTSUP).  A value that is not finite may reach every output of its 64 tokens, also those in front
+ * of it.  workspace: ss2d_linear_attention_workspace_bytes() bytes, 16-byte aligned (0: none).  dense tensors are aligned to two elements (fp32 ones to 8 bytes).
+ * No atomics: repeated calls give bit-identical results.
+ * -------------------------------------------------------------------------------- */
+typedef struct ss2d_linear_attention_params {
+    const void *q, *k, *v, *log_decay;
+    const void *initial_state;
+    void *out, *final_state, *chunk_states, *workspace;
+    int64_t workspace_bytes;
+    int64_t batch, seqlen, n_groups, heads, dk, dv;
+    int64_t q_batch_stride, q_token_stride, q_head_stride;
+    int64_t k_batch_stride, k_token_stride, k_head_stride;
+    int64_t v_batch_stride, v_token_stride, v_head_stride;
+    int64_t decay_batch_stride, decay_token_stride, decay_head_stride;
+    int32_t dtype;
+    float scale;
+} ss2d_linear_attention_params;
+
+int ss2d_linear_attention_fwd(const ss2d_linear_attention_params *p, void *cuda_stream);
+int64_t ss2d_linear_attention_workspace_bytes(const ss2d_linear_attention_params *p);    /* < 0: invalid arguments */
+
+/* Its backward call: `fwd` as in the forward call, with the chunk_states that it wrote (out, final_state and initial_state are not read); dout of
+ * `dtype`, (batch, seqlen, heads, dv), strided; dfinal_state fp32, NULL: zero.  Results, dense: dq, dk (batch, seqlen, n_groups, dk), summed over the heads of
+ * a group, dv (batch, seqlen, heads, dv) of `dtype`; dlog_decay (batch, seqlen, heads) fp32; dinitial_state fp32 or NULL. */
+typedef struct ss2d_linear_attention_bwd_params {
+    ss2d_linear_attention_params fwd;
+    const void *dout, *dfinal_state;
+    void *dq, *dk, *dv, *dlog_decay, *dinitial_state, *workspace;
+    int64_t workspace_bytes;
+    int64_t dout_batch_stride, dout_token_stride, dout_head_stride;
+} ss2d_linear_attention_bwd_params;
+
+int ss2d_linear_attention_bwd(const ss2d_linear_attention_bwd_params *p, void *cuda_stream);
+int64_t ss2d_linear_attention_bwd_workspace_bytes(const ss2d_linear_attention_bwd_params *p);
+
+/* One token of every sequence: q, k (batch, n_groups, dk), v (batch, heads, dv), log_decay (batch, heads), strided as above; state and state_out fp32
+ * (batch, heads, dk, dv), dense but for the batch stride, the same memory or memory that does not overlap; out (batch, heads, dv), dense. */
+typedef struct ss2d_linear_attention_step_params {
+    const void *q, *k, *v, *log_decay, *state;
+    void *state_out, *out;
+    int64_t batch, n_groups, heads, dk, dv;
+    int64_t q_batch_stride, q_head_stride, k_batch_stride, k_head_stride, v_batch_stride, v_head_stride;
+    int64_t decay_batch_stride, decay_head_stride, state_batch_stride, state_out_batch_stride;
+    int32_t dtype;
+    float scale;
+} ss2d_linear_attention_step_params;
+
+int ss2d_linear_attention_step(const ss2d_linear_attention_step_params *p, void *cuda_stream);
+
 int ss2d_version(void);
 const char *ss2d_strerror(int status);
 /* number of kernel launches issued by this library in this process so far (all entry points) */

@@ -122,6 +122,27 @@ class RowProductsParams(ctypes.Structure):
                                     "b_outer_stride", "b_group_stride", "b_row_stride")] + [("dtype", _i32), ("turned", _i32)]
 
 
+class LinearAttentionParams(ctypes.Structure):
+    _fields_ = [(n, _vp) for n in ("q", "k", "v", "log_decay", "initial_state", "out", "final_state", "chunk_states", "workspace")] + \
+               [(n, _i64) for n in ("workspace_bytes", "batch", "seqlen", "n_groups", "heads", "dk", "dv",
+                                    "q_batch_stride", "q_token_stride", "q_head_stride", "k_batch_stride", "k_token_stride", "k_head_stride",
+                                    "v_batch_stride", "v_token_stride", "v_head_stride",
+                                    "decay_batch_stride", "decay_token_stride", "decay_head_stride")] + [("dtype", _i32), ("scale", _f32)]
+
+
+class LinearAttentionBwdParams(ctypes.Structure):
+    _fields_ = [("fwd", LinearAttentionParams)] + \
+               [(n, _vp) for n in ("dout", "dfinal_state", "dq", "dk", "dv", "dlog_decay", "dinitial_state", "workspace")] + \
+               [(n, _i64) for n in ("workspace_bytes", "dout_batch_stride", "dout_token_stride", "dout_head_stride")]
+
+
+class LinearAttentionStepParams(ctypes.Structure):
+    _fields_ = [(n, _vp) for n in ("q", "k", "v", "log_decay", "state", "state_out", "out")] + \
+               [(n, _i64) for n in ("batch", "n_groups", "heads", "dk", "dv", "q_batch_stride", "q_head_stride", "k_batch_stride", "k_head_stride",
+                                    "v_batch_stride", "v_head_stride", "decay_batch_stride", "decay_head_stride",
+                                    "state_batch_stride", "state_out_batch_stride")] + [("dtype", _i32), ("scale", _f32)]
+
+
 EXPORTS = {
     # name: (restype, argtypes)
     "ss2d_selective_scan_fwd": (ctypes.c_int, [ctypes.POINTER(ScanParams), _vp]),
@@ -157,6 +178,11 @@ EXPORTS = {
     "ss2d_mlp_fwd": (ctypes.c_int, [ctypes.POINTER(MlpParams), _vp]),
     "ss2d_linear_supported": (ctypes.c_int, [ctypes.POINTER(LinearParams)]),
     "ss2d_linear_fwd": (ctypes.c_int, [ctypes.POINTER(LinearParams), _vp]),
+    "ss2d_linear_attention_fwd": (ctypes.c_int, [ctypes.POINTER(LinearAttentionParams), _vp]),
+    "ss2d_linear_attention_workspace_bytes": (_i64, [ctypes.POINTER(LinearAttentionParams)]),
+    "ss2d_linear_attention_bwd": (ctypes.c_int, [ctypes.POINTER(LinearAttentionBwdParams), _vp]),
+    "ss2d_linear_attention_bwd_workspace_bytes": (_i64, [ctypes.POINTER(LinearAttentionBwdParams)]),
+    "ss2d_linear_attention_step": (ctypes.c_int, [ctypes.POINTER(LinearAttentionStepParams), _vp]),
     "ss2d_set_debug_checks": (ctypes.c_int, [ctypes.c_int]),
     "ss2d_version": (ctypes.c_int, []),
     "ss2d_strerror": (ctypes.c_char_p, [ctypes.c_int]),

@@ -44,6 +44,11 @@ int pixels_norm_to_planes(const ss2d_relayout_params* p, cudaStream_t st);
 int planes_to_pixels(const ss2d_relayout_params* p, cudaStream_t st);
 int bias_act(const ss2d_pointwise_params* p, cudaStream_t st);
 int dwconv3x3_act(const ss2d_pointwise_params* p, cudaStream_t st);
+int linear_attention_fwd(const ss2d_linear_attention_params* p, cudaStream_t st);
+long long linear_attention_workspace_bytes(const ss2d_linear_attention_params* p);
+int linear_attention_bwd(const ss2d_linear_attention_bwd_params* p, cudaStream_t st);
+long long linear_attention_bwd_workspace_bytes(const ss2d_linear_attention_bwd_params* p);
+int linear_attention_step(const ss2d_linear_attention_step_params* p, cudaStream_t st);
 
 static std::atomic<long long> g_launches{0};
 static std::atomic<int> g_debug_checks{[] { const char* v = std::getenv("SS2D_DEBUG_CHECKS"); return (v && v[0] == '1') ? 1 : 0; }()};
@@ -206,6 +211,24 @@ int ss2d_linear_fwd(const ss2d_linear_params* p, void* stream) {
     return ss2d::linear_fwd(p, (cudaStream_t)stream);
 }
 
+int ss2d_linear_attention_fwd(const ss2d_linear_attention_params* p, void* stream) {
+    ss2d::Range nvtx_("ss2d_linear_attention_fwd");
+    if (p) SS2D_CHECK_PTRS(p->q, p->k, p->v, p->log_decay, p->initial_state, p->out, p->final_state, p->chunk_states, p->workspace);
+    return ss2d::linear_attention_fwd(p, (cudaStream_t)stream);
+}
+int64_t ss2d_linear_attention_workspace_bytes(const ss2d_linear_attention_params* p) { return ss2d::linear_attention_workspace_bytes(p); }
+int ss2d_linear_attention_bwd(const ss2d_linear_attention_bwd_params* p, void* stream) {
+    ss2d::Range nvtx_("ss2d_linear_attention_bwd");
+    if (p) SS2D_CHECK_PTRS(p->fwd.q, p->fwd.k, p->fwd.v, p->fwd.log_decay, p->fwd.chunk_states, p->dout, p->dfinal_state, p->dq, p->dk, p->dv,
+                           p->dlog_decay, p->dinitial_state, p->workspace);
+    return ss2d::linear_attention_bwd(p, (cudaStream_t)stream);
+}
+int64_t ss2d_linear_attention_bwd_workspace_bytes(const ss2d_linear_attention_bwd_params* p) { return ss2d::linear_attention_bwd_workspace_bytes(p); }
+int ss2d_linear_attention_step(const ss2d_linear_attention_step_params* p, void* stream) {
+    ss2d::Range nvtx_("ss2d_linear_attention_step");
+    if (p) SS2D_CHECK_PTRS(p->q, p->k, p->v, p->log_decay, p->state, p->state_out, p->out);
+    return ss2d::linear_attention_step(p, (cudaStream_t)stream);
+}
 int ss2d_version(void) { return SS2D_ABI_VERSION; }
 int64_t ss2d_launch_count(void) { return ss2d::g_launches.load(std::memory_order_relaxed); }
 

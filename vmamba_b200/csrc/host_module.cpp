@@ -5,6 +5,7 @@ namespace host {
 void bind_ops(pybind11::module_& m);
 void bind_core(pybind11::module_& m);
 void bind_backbone(pybind11::module_& m);
+void bind_attention(pybind11::module_& m);
 }  // namespace host
 
 PYBIND11_MODULE(_host, m) {
@@ -21,4 +22,5 @@ PYBIND11_MODULE(_host, m) {
     host::bind_ops(m);
     host::bind_core(m);
     host::bind_backbone(m);
+    host::bind_attention(m);
 }

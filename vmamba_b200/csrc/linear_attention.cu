@@ -1,0 +1,859 @@
+// Linear attention with a decay for each head:
+//   S_t = exp(g_t) S_{t-1} + k_t v_t^T        (S: dk x dv, fp32)
+//   o_t = scale S_t^T q_t
+// walked in chunks of 64 tokens.  With G the cumulative sum of g inside a chunk (base 2 from here on), e_i = 2^G_i, w_j = 2^(G_C - G_j):
+//   o_i  = scale (e_i S_in^T q_i + sum_{j <= i} 2^(G_i - G_j) (q_i . k_j) v_j)
+//   S_out = 2^G_C S_in + sum_j w_j k_j v_j^T
+// and for the gradients, with dS the gradient of the state behind the chunk,
+//   dS_in = 2^G_C dS + scale sum_i e_i q_i do_i^T
+//   dq_i  = scale (e_i S_in do_i + sum_{j <= i} D_ij (do_i . v_j) k_j),   D_ij = 2^(G_i - G_j)
+//   dk_j  = w_j dS v_j + scale sum_{i >= j} D_ij (do_i . v_j) q_i
+//   dv_j  = w_j dS^T k_j + scale sum_{i >= j} D_ij (q_i . k_j) do_i
+//   dg_t  = what crosses the boundary in front of token t: 2^G_C <S_in, dS> + sum_{s >= t} scale e_s q_s^T S_in do_s
+//           + sum_{r < t} w_r k_r^T dS v_r + sum_{r < t <= s} scale D_sr (q_s . k_r)(do_s . v_r)
+// (the telescoped form q . dq - k . dk summed from the end needs no states, but its terms cancel over the whole sequence: with products of
+// 16-bit operands the noise of thousands of tokens stays in every dg).
+//
+// Decays are differences of two numbers, an integer and a fraction, so that a chunk whose decays run to thousands loses nothing of the small
+// ones behind; log decays below 2^-200 a token count as a reset (exp is 0 in fp32 long before), so -inf is one.
+//
+// Kernels.  la_walk: one CTA per (sequence, head, 64 columns of v, segment of chunks) walks its chunks with the state in registers and writes
+// outputs and, where asked, the state in front of every chunk; the same kernel without outputs gathers the states of a segment, or the state gradients
+// backwards.  la_join: states in front of the segments from those that the segments gather.  la_grad: everything else of the backward pass, one CTA per
+// (sequence, group of heads, chunk), no order between them.  la_step: one token, the state read and written once.
+#include "mma_tiles.cuh"
+
+namespace ss2d {
+
+namespace {
+
+using namespace mt;
+
+constexpr int kChunk = 64;
+constexpr int kSlice = 64;          // columns of v of a walking CTA
+constexpr int kSlab = 32;           // rows of the states that the gradient kernel holds at a time
+constexpr float kFloor = -200.f;    // 2^-200 is 0 in fp32
+
+struct Rows {                       // (batch, token, head) rows of contiguous elements
+    const void* p;
+    long long b, l, h;
+    bool vec;
+};
+
+// ---- decays of a chunk -------------------------------------------------------------------------------------------------
+struct Cum { float n, f; };         // n + f, n whole, 0 <= f < 1: exact in n, 2^-25 in f
+__device__ __forceinline__ Cum cum_of(float log_decay) {
+    float x = log_decay * kLog2e;
+    x = x < kFloor ? kFloor : x;    // (NaN stays)
+    const float n = floorf(x);
+    return {n, x - n};
+}
+__device__ __forceinline__ Cum cum_add(Cum a, Cum b) {
+    const float f = a.f + b.f, c = f >= 1.f ? 1.f : 0.f;
+    return {a.n + b.n + c, f - c};
+}
+__device__ __forceinline__ float exp_diff(Cum a, Cum b) { return ex2_approx((a.n - b.n) + (a.f - b.f)); }
+
+struct Decays {
+    float n[kChunk], f[kChunk];     // cumulative sums
+    float e[kChunk], w[kChunk];     // 2^G_i, 2^(G_C - G_i)
+    float total_n, total_f, total;  // G_C, 2^G_C
+    __device__ __forceinline__ Cum at(int i) const { return {n[i], f[i]}; }
+};
+// one warp: from the log decays of tokens 2 lane and 2 lane + 1
+__device__ __forceinline__ void fill_decays(Decays& d, float g0, float g1, int lane) {
+    const Cum a = cum_of(g0);
+    Cum s = cum_add(a, cum_of(g1));
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const Cum o = {__shfl_up_sync(0xffffffffu, s.n, off), __shfl_up_sync(0xffffffffu, s.f, off)};
+        if (lane >= off) s = cum_add(o, s);
+    }
+    Cum before = {__shfl_up_sync(0xffffffffu, s.n, 1), __shfl_up_sync(0xffffffffu, s.f, 1)};
+    if (lane == 0) before = {0.f, 0.f};
+    const Cum first = cum_add(before, a);
+    const Cum all = {__shfl_sync(0xffffffffu, s.n, 31), __shfl_sync(0xffffffffu, s.f, 31)};
+    d.n[2 * lane] = first.n; d.f[2 * lane] = first.f;
+    d.n[2 * lane + 1] = s.n; d.f[2 * lane + 1] = s.f;
+    d.e[2 * lane] = ex2_approx(first.n + first.f);
+    d.e[2 * lane + 1] = ex2_approx(s.n + s.f);
+    d.w[2 * lane] = exp_diff(all, first);
+    d.w[2 * lane + 1] = exp_diff(all, s);
+    if (lane == 0) { d.total_n = all.n; d.total_f = all.f; d.total = ex2_approx(all.n + all.f); }
+}
+// a token past the end decays nothing
+__device__ __forceinline__ void load_decays(float& g0, float& g1, const float* g, long long stride, int first, int L, int lane) {
+    const int t = first + 2 * lane;
+    g0 = t < L ? g[t * stride] : 0.f;
+    g1 = t + 1 < L ? g[(t + 1) * stride] : 0.f;
+}
+
+// ---- walking a sequence ------------------------------------------------------------------------------------------------
+struct WalkArgs {
+    Rows q, k, v;                   // kOut: q, k, v.  Otherwise the rows of the state's update: k (forwards) or q (backwards), and v or do
+    const float* g;
+    long long g_b, g_l, g_h;
+    const float* start;             // (B, H, segments, dk, dv) or NULL: zeros
+    float* end;                     // the same, or NULL
+    float* end_decay;               // (B, H, segments): log2 of the decay over the segment, or NULL
+    float* states;                  // (B, H, chunks, dk, dv): the state in front of every chunk (walking backwards: behind it), or NULL
+    void* o;                        // (B, L, H, dv)
+    int H, rep, L, dk, dv, chunks, per_segment, segments, pairs;
+    float scale;
+};
+
+template <typename T, int DK> struct WalkSmem {
+    using P = typename Plane<T>::type;
+    static constexpr int kLdK = DK + 8, kLdV = kSlice + 8;
+    static constexpr int kQ = kChunk * kLdK, kV = kChunk * kLdV;       // elements
+    static constexpr size_t stage(bool out) { return ((out ? 2 : 1) * kQ + kV) * sizeof(T); }
+    static constexpr size_t plane(bool out) { return out ? DK * kLdV * sizeof(P) : 0; }
+    static constexpr size_t bytes(bool out) { return 2 * stage(out) + plane(out) + 2 * sizeof(Decays); }
+};
+
+// Four warps.  Outputs: a warp has 16 tokens.  State: a warp has DK / 4 of its rows, in accumulators, DK / 64 blocks of 16 (one for two warps at DK = 32).
+template <typename T, int DK, bool kOut, bool kBack>
+__global__ void __launch_bounds__(128) la_walk_kernel(const WalkArgs a) {
+    follow_previous();
+    using M = WalkSmem<T, DK>;
+    using P = typename M::P;
+    extern __shared__ __align__(16) unsigned char smem[];
+    constexpr int kBlocks = (DK + 63) / 64;
+    T* const stage0 = reinterpret_cast<T*>(smem);
+    P* const plane = reinterpret_cast<P*>(smem + 2 * M::stage(kOut));
+    Decays* const decays = reinterpret_cast<Decays*>(smem + 2 * M::stage(kOut) + M::plane(kOut));
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, t = lane & 3;
+    const int slices = (a.dv + kSlice - 1) / kSlice, slice = blockIdx.x % slices, bh = blockIdx.x / slices, seg = blockIdx.y;
+    const int v0 = slice * kSlice, dv = min(kSlice, a.dv - v0), b = bh / a.H, h = bh % a.H;
+    const int c0 = seg * a.per_segment, c1 = min(a.chunks, c0 + a.per_segment);
+    const T* const q = (const T*)a.q.p + b * a.q.b + (h / a.rep) * a.q.h;
+    const T* const k = (const T*)a.k.p + b * a.k.b + (h / a.rep) * a.k.h;
+    const T* const v = (const T*)a.v.p + b * a.v.b + h * a.v.h + v0;
+    const float* const g = a.g + b * a.g_b + h * a.g_h;
+    const long long state_size = (long long)a.dk * a.dv;
+
+    float S[kBlocks][8][4];
+    const int m_first = warp * 16;                         // first row of the warp's block 0; the next one is 64 rows on
+    const bool holds = DK >= 64 || warp < DK / 16;
+    auto for_state = [&](auto&& f) {                       // f(row, column, first of two accumulators)
+#pragma unroll
+        for (int m = 0; m < kBlocks; ++m)
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) f(m_first + 64 * m + gq + 8 * r, 8 * n + 2 * t, S[m][n] + 2 * r);
+    };
+    {
+        const float* s0 = a.start ? a.start + ((long long)bh * a.segments + seg) * state_size + v0 : nullptr;
+        for_state([&](int row, int col, float* s) {
+            const bool in = s0 && holds && row < a.dk;
+            s[0] = in && col < dv ? s0[(long long)row * a.dv + col] : 0.f;
+            s[1] = in && col + 1 < dv ? s0[(long long)row * a.dv + col + 1] : 0.f;
+        });
+    }
+    auto put_plane = [&] {
+        if constexpr (kOut)
+            if (holds) for_state([&](int row, int col, float* s) { put2<T, 1>(plane + row * M::kLdV + col, 0, s[0], s[1]); });
+    };
+    auto write_state = [&](float* to) {
+        if (holds)
+            for_state([&](int row, int col, float* s) {
+                if (row >= a.dk) return;
+                float* p = to + (long long)row * a.dv + v0 + col;
+                if (a.pairs && col + 1 < dv) *reinterpret_cast<float2*>(p) = make_float2(s[0], s[1]);
+                else {
+                    if (col < dv) p[0] = s[0];
+                    if (col + 1 < dv) p[1] = s[1];
+                }
+            });
+    };
+    auto fetch = [&](int c, int buf) {
+        T* s = stage0 + buf * ((kOut ? 2 : 1) * M::kQ + M::kV);
+        const int first = c * kChunk, rows = min(kChunk, a.L - first);
+        fetch_rows<T, kChunk, DK>(s, M::kLdK, k + (long long)first * a.k.l, a.k.l, rows, a.dk, a.k.vec, tid, 128);
+        fetch_rows<T, kChunk, kSlice>(s + M::kQ, M::kLdV, v + (long long)first * a.v.l, a.v.l, rows, dv, a.v.vec, tid, 128);
+        if constexpr (kOut) fetch_rows<T, kChunk, DK>(s + M::kQ + M::kV, M::kLdK, q + (long long)first * a.q.l, a.q.l, rows, a.dk, a.q.vec, tid, 128);
+        commit_copies();
+    };
+
+    const int n = c1 - c0;
+    auto chunk_at = [&](int i) { return kBack ? c1 - 1 - i : c0 + i; };
+    float g0 = 0.f, g1 = 0.f;
+    fetch(chunk_at(0), 0);
+    load_decays(g0, g1, g, a.g_l, chunk_at(0) * kChunk, a.L, lane);
+    put_plane();
+    Cum over = {0.f, 0.f};
+    for (int i = 0; i < n; ++i) {
+        const int c = chunk_at(i), buf = i & 1;
+        Decays& d = decays[buf];
+        if (warp == 0) fill_decays(d, g0, g1, lane);
+        wait_copies();
+        __syncthreads();
+        if (i + 1 < n) {
+            fetch(chunk_at(i + 1), buf ^ 1);
+            load_decays(g0, g1, g, a.g_l, chunk_at(i + 1) * kChunk, a.L, lane);
+        }
+        if (a.states) write_state(a.states + ((long long)bh * a.chunks + c) * state_size);
+        const T* sk = stage0 + buf * ((kOut ? 2 : 1) * M::kQ + M::kV);
+        const T* sv = sk + M::kQ;
+        if constexpr (kOut) {
+            const T* sq = sv + M::kV;
+            const int r0 = warp * 16;
+            float p[8][4] = {}, o[8][4] = {};
+#pragma unroll
+            for (int k0 = 0; k0 < DK; k0 += 16) {
+                const OpA<T> qa = load_a<false>(sq, M::kLdK, r0, k0, lane);
+#pragma unroll
+                for (int j = 0; j < 8; j += 2)
+                    if (j <= 2 * warp) {                   // keys up to the warp's last token
+                        OpB<T> b0, b1;
+                        load_b2<false>(b0, b1, sk, M::kLdK, 8 * j, k0, lane);
+                        mma_exact(p[j], qa, b0);
+                        mma_exact(p[j + 1], qa, b1);
+                    }
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) mma_plane2<T, 1, true>(o[j], o[j + 1], qa, plane, 0, M::kLdV, 8 * j, k0, lane);
+            }
+            const Cum lo = d.at(r0 + gq), hi = d.at(r0 + gq + 8);
+            const float el = d.e[r0 + gq], eh = d.e[r0 + gq + 8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                o[j][0] *= el; o[j][1] *= el; o[j][2] *= eh; o[j][3] *= eh;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j += 2)
+                if (j <= 2 * warp) {
+                    float x[8];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int s = 0; s < 2; ++s) {
+                            const int col = 8 * (j + u) + 2 * t + s;
+                            const Cum at = d.at(col);
+                            x[4 * u + s] = col <= r0 + gq ? p[j + u][s] * exp_diff(lo, at) : 0.f;
+                            x[4 * u + 2 + s] = col <= r0 + gq + 8 ? p[j + u][2 + s] * exp_diff(hi, at) : 0.f;
+                        }
+                    const Derived<T, 1> pd = derive<T, 1>(x);
+#pragma unroll
+                    for (int u = 0; u < 8; u += 2) {
+                        OpB<T> b0, b1;
+                        load_b2<true>(b0, b1, sv, M::kLdV, 8 * u, 8 * j, lane);
+                        mma_derived<T, 1>(o[u], pd, b0);
+                        mma_derived<T, 1>(o[u + 1], pd, b1);
+                    }
+                }
+            T* const out = (T*)a.o + ((long long)b * a.L + c * kChunk) * a.H * a.dv + (long long)h * a.dv + v0;
+            const int rows = min(kChunk, a.L - c * kChunk);
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int row = r0 + gq + 8 * r;
+                if (row < rows) {
+                    T* to = out + (long long)row * a.H * a.dv;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const int col = 8 * j + 2 * t;
+                        const float y[2] = {a.scale * o[j][2 * r], a.scale * o[j][2 * r + 1]};
+                        if (a.pairs && col + 1 < dv) Vec<T, 2>::store(to + col, y);
+                        else {
+                            if (col < dv) to[col] = from_f<T>(y[0]);
+                            if (col + 1 < dv) to[col + 1] = from_f<T>(y[1]);
+                        }
+                    }
+                }
+            }
+            __syncthreads();                               // the plane has been read
+        }
+        // state: rows of k^T weighted by what is left of them at the end of the chunk (backwards: of q^T by what reaches them)
+        const float keep = d.total;
+        if (holds) {
+#pragma unroll
+            for (int m = 0; m < kBlocks; ++m)
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+#pragma unroll
+                    for (int s = 0; s < 4; ++s) S[m][j][s] *= keep;
+#pragma unroll
+            for (int k0 = 0; k0 < kChunk; k0 += 16) {
+                const float* w = kBack ? d.e : d.w;
+                float ws[4] = {w[k0 + 2 * t], w[k0 + 2 * t + 1], w[k0 + 8 + 2 * t], w[k0 + 9 + 2 * t]};
+                if constexpr (kBack) {
+#pragma unroll
+                    for (int s = 0; s < 4; ++s) ws[s] *= a.scale;
+                }
+                OpB<T> vb[8];
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) load_b2<true>(vb[j], vb[j + 1], sv, M::kLdV, 8 * j, k0, lane);
+#pragma unroll
+                for (int m = 0; m < kBlocks; ++m) {
+                    float x[8];
+                    values(load_a<true>(sk, M::kLdK, m_first + 64 * m, k0, lane), x);
+#pragma unroll
+                    for (int s = 0; s < 8; ++s) x[s] *= ws[(s & 1) + 2 * (s >> 2)];
+                    const Derived<T, 2> kd = derive<T, 2>(x);       // two pieces: the state is an fp32 result
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) mma_derived<T, 2>(S[m][j], kd, vb[j]);
+                }
+            }
+        }
+        put_plane();
+        over = cum_add(over, {d.total_n, d.total_f});
+    }
+    if (a.end) write_state(a.end + ((long long)bh * a.segments + seg) * state_size);
+    if (a.end_decay && slice == 0 && tid == 0) a.end_decay[(long long)bh * a.segments + seg] = over.n + over.f;
+}
+
+// ---- states in front of the segments -----------------------------------------------------------------------------------
+struct JoinArgs {
+    const float* first;             // (B, H, dk, dv) or NULL
+    float* part;                    // (B, H, segments, dk, dv): what the segments gather; becomes the state that each starts from
+    const float* decay;             // (B, H, segments)
+    float* last;                    // (B, H, dk, dv) or NULL
+    long long size;                 // dk dv
+    int segments;
+    bool back;
+};
+__global__ void __launch_bounds__(256) la_join_kernel(const JoinArgs a) {
+    follow_previous();
+    const long long blocks = (a.size + 255) / 256, bh = blockIdx.x / blocks, e = blockIdx.x % blocks * 256 + threadIdx.x;
+    if (e >= a.size) return;
+    float s = a.first ? a.first[bh * a.size + e] : 0.f;
+    for (int i = 0; i < a.segments; ++i) {
+        const long long at = bh * a.segments + (a.back ? a.segments - 1 - i : i);
+        const float x = a.part[at * a.size + e];
+        a.part[at * a.size + e] = s;
+        s = fmaf(ex2_approx(a.decay[at]), s, x);
+    }
+    if (a.last) a.last[bh * a.size + e] = s;
+}
+
+// ---- gradients of a chunk ----------------------------------------------------------------------------------------------
+struct GradArgs {
+    Rows q, k, v, dy;
+    const float* g;
+    long long g_b, g_l, g_h;
+    const float *states, *dstates;  // (B, H, chunks, dk, dv): in front of the chunk; gradient of the state behind it
+    void *dq, *dk_, *dv_;           // dense
+    float* dg;                      // (B, L, H)
+    float *sum_q, *sum_k;           // (B, L, G, dk) where heads share their keys
+    int G, rep, L, dk, dv, chunks, pairs_k, pairs_v;
+    float scale;
+};
+
+template <typename T, int DK, int DV> struct GradSmem {
+    using P = typename Plane<T>::type;
+    static constexpr int kParts = 2, kPlanes = Plane<T>::kSplit ? kParts : 1;
+    static constexpr int kLdK = DK + 8, kLdV = DV + 8;
+    static constexpr int kK = kChunk * kLdK, kV = kChunk * kLdV, kPlane = kSlab * kLdV;
+    static constexpr size_t kRowBytes = (2 * kK + 2 * kV) * sizeof(T), kStateBytes = 2 * kPlanes * kPlane * sizeof(P);
+    static constexpr size_t bytes() { return kRowBytes + kStateBytes + sizeof(Decays) + (4 * kChunk + 8) * sizeof(float); }
+};
+
+// Eight warps: four have 16 queries each, the other four 16 keys each and the transposed products.  The states pass in slabs of 32 rows.
+template <typename T, int DK, int DV>
+__global__ void __launch_bounds__(256) la_grad_kernel(const GradArgs a) {
+    follow_previous();
+    using M = GradSmem<T, DK, DV>;
+    using P = typename M::P;
+    constexpr int kLdK = M::kLdK, kLdV = M::kLdV, kParts = M::kParts;
+    extern __shared__ __align__(16) unsigned char smem[];
+    T *const sq = reinterpret_cast<T*>(smem), *const sk = sq + M::kK, *const sv = sk + M::kK, *const sy = sv + M::kV;
+    P *const s_in = reinterpret_cast<P*>(smem + M::kRowBytes), *const s_out = s_in + M::kPlanes * M::kPlane;
+    Decays& d = *reinterpret_cast<Decays*>(smem + M::kRowBytes + M::kStateBytes);
+    float *const row_sum = reinterpret_cast<float*>(&d + 1), *const col_sum = row_sum + kChunk, *const into = col_sum + kChunk,
+                *const from = into + kChunk, *const cross = from + kChunk;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, t = lane & 3;
+    const bool keys = warp >= 4;
+    const int w4 = warp & 3, r0 = 16 * w4;
+    const int c = blockIdx.x % a.chunks, bg = blockIdx.x / a.chunks, b = bg / a.G, grp = bg % a.G, H = a.G * a.rep;
+    const int first = c * kChunk, rows = min(kChunk, a.L - first);
+    auto src = [&](const Rows& r, int head) { return (const T*)r.p + b * r.b + (long long)first * r.l + head * r.h; };
+    fetch_rows<T, kChunk, DK>(sq, kLdK, src(a.q, grp), a.q.l, rows, a.dk, a.q.vec, tid, 256);
+    fetch_rows<T, kChunk, DK>(sk, kLdK, src(a.k, grp), a.k.l, rows, a.dk, a.k.vec, tid, 256);
+    for (int hh = 0; hh < a.rep; ++hh) {
+        const int h = grp * a.rep + hh;
+        if (hh) __syncthreads();
+        fetch_rows<T, kChunk, DV>(sv, kLdV, src(a.v, h), a.v.l, rows, a.dv, a.v.vec, tid, 256);
+        fetch_rows<T, kChunk, DV>(sy, kLdV, src(a.dy, h), a.dy.l, rows, a.dv, a.dy.vec, tid, 256);
+        commit_copies();
+        if (warp == 0) {
+            float g0, g1;
+            load_decays(g0, g1, a.g + b * a.g_b + h * a.g_h, a.g_l, first, a.L, lane);
+            fill_decays(d, g0, g1, lane);
+        }
+        wait_copies();
+        __syncthreads();
+        // rows of the warp: queries (columns: keys) or keys (columns: queries)
+        float qk[8][4] = {}, yv[8][4] = {};
+        {
+            const T *const A = keys ? sk : sq, *const B = keys ? sq : sk, *const Ay = keys ? sv : sy, *const By = keys ? sy : sv;
+            auto live = [&](int j) { return keys ? j >= 2 * w4 : j <= 2 * w4; };      // pairs of column blocks
+#pragma unroll
+            for (int k0 = 0; k0 < DK; k0 += 16) {
+                const OpA<T> x = load_a<false>(A, kLdK, r0, k0, lane);
+#pragma unroll
+                for (int j = 0; j < 8; j += 2)
+                    if (live(j)) {
+                        OpB<T> b0, b1;
+                        load_b2<false>(b0, b1, B, kLdK, 8 * j, k0, lane);
+                        mma_exact(qk[j], x, b0);
+                        mma_exact(qk[j + 1], x, b1);
+                    }
+            }
+#pragma unroll
+            for (int k0 = 0; k0 < DV; k0 += 16) {
+                const OpA<T> x = load_a<false>(Ay, kLdV, r0, k0, lane);
+#pragma unroll
+                for (int j = 0; j < 8; j += 2)
+                    if (live(j)) {
+                        OpB<T> b0, b1;
+                        load_b2<false>(b0, b1, By, kLdV, 8 * j, k0, lane);
+                        mma_exact(yv[j], x, b0);
+                        mma_exact(yv[j + 1], x, b1);
+                    }
+            }
+            // pairs: decays, and the sums of what crosses (the pair of a token with itself crosses nothing)
+            float sum[2] = {0.f, 0.f};
+            const Cum own[2] = {d.at(r0 + gq), d.at(r0 + gq + 8)};
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+                        const int row = r0 + gq + 8 * r, col = 8 * j + 2 * t + s;
+                        const bool in = keys ? col >= row : col <= row;
+                        const Cum at = d.at(col);
+                        const float D = in ? a.scale * (keys ? exp_diff(at, own[r]) : exp_diff(own[r], at)) : 0.f;
+                        float &x = qk[j][2 * r + s], &y = yv[j][2 * r + s];
+                        if (in && col != row) sum[r] = fmaf(D * x, y, sum[r]);
+                        x *= D;
+                        y *= D;
+                    }
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
+                sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
+                if (t == 0) (keys ? col_sum : row_sum)[r0 + gq + 8 * r] = sum[r];
+            }
+        }
+        const long long at = ((long long)(b * H + h) * a.chunks + c) * a.dk * a.dv;
+        const float wl = (keys ? d.w : d.e)[r0 + gq] * (keys ? 1.f : a.scale), wh = (keys ? d.w : d.e)[r0 + gq + 8] * (keys ? 1.f : a.scale);
+        float dv[DV / 8][4] = {};
+        float through[2] = {0.f, 0.f}, both = 0.f;
+        const T *const X = keys ? sv : sy, *const Own = keys ? sk : sq, *const Other = keys ? sq : sk;
+        for (int m0 = 0; m0 < a.dk; m0 += kSlab) {
+            __syncthreads();
+            for (int i = tid; i < kSlab * DV / 2; i += 256) {
+                const int m = i / (DV / 2), n = (i % (DV / 2)) * 2;
+                float x[2] = {0.f, 0.f}, y[2] = {0.f, 0.f};
+                if (m0 + m < a.dk && n < a.dv) {
+                    const long long p = at + (long long)(m0 + m) * a.dv + n;
+                    if (a.pairs_v) { Vec<float, 2>::load(a.states + p, x); Vec<float, 2>::load(a.dstates + p, y); }
+                    else {
+                        x[0] = a.states[p]; y[0] = a.dstates[p];
+                        if (n + 1 < a.dv) { x[1] = a.states[p + 1]; y[1] = a.dstates[p + 1]; }
+                    }
+                }
+                both = fmaf(x[0], y[0], fmaf(x[1], y[1], both));
+                put2<T, kParts>(s_in + m * kLdV + n, M::kPlane, x[0], x[1]);
+                put2<T, kParts>(s_out + m * kLdV + n, M::kPlane, y[0], y[1]);
+            }
+            __syncthreads();
+            const P* const S = keys ? s_out : s_in;
+            float acc[4][4] = {};
+#pragma unroll
+            for (int k0 = 0; k0 < DV; k0 += 16) {
+                const OpA<T> x = load_a<false>(X, kLdV, r0, k0, lane);
+#pragma unroll
+                for (int j = 0; j < 4; j += 2) mma_plane2<T, kParts, false>(acc[j], acc[j + 1], x, S, M::kPlane, kLdV, 8 * j, k0, lane);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const T* p = Own + (r0 + gq + 8 * r) * kLdK + m0 + 8 * j + 2 * t;
+                    through[r] = fmaf(to_f<T>(p[0]), acc[j][2 * r], fmaf(to_f<T>(p[1]), acc[j][2 * r + 1], through[r]));
+                    acc[j][2 * r] *= r ? wh : wl;
+                    acc[j][2 * r + 1] *= r ? wh : wl;
+                }
+#pragma unroll
+            for (int j = 0; j < 8; j += 2)
+                if (keys ? j >= 2 * w4 : j <= 2 * w4) {
+                    const float x[8] = {yv[j][0], yv[j][1], yv[j][2], yv[j][3], yv[j + 1][0], yv[j + 1][1], yv[j + 1][2], yv[j + 1][3]};
+                    const Derived<T, 1> xd = derive<T, 1>(x);
+#pragma unroll
+                    for (int u = 0; u < 4; u += 2) {
+                        OpB<T> b0, b1;
+                        load_b2<true>(b0, b1, Other, kLdK, m0 + 8 * u, 8 * j, lane);
+                        mma_derived<T, 1>(acc[u], xd, b0);
+                        mma_derived<T, 1>(acc[u + 1], xd, b1);
+                    }
+                }
+            if (keys) {
+#pragma unroll
+                for (int k0 = 0; k0 < kSlab; k0 += 16) {
+                    const OpA<T> x = load_a<false>(sk, kLdK, r0, m0 + k0, lane);
+#pragma unroll
+                    for (int j = 0; j < DV / 8; j += 2) mma_plane2<T, 1, true>(dv[j], dv[j + 1], x, s_out, M::kPlane, kLdV, 8 * j, k0, lane);
+                }
+            }
+            T* const to = (T*)(keys ? a.dk_ : a.dq);
+            float* const part = keys ? a.sum_k : a.sum_q;
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int row = r0 + gq + 8 * r;
+                if (row >= rows) continue;
+                const long long p = (((long long)b * a.L + first + row) * a.G + grp) * a.dk + m0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int col = 8 * j + 2 * t;
+                    float y[2] = {acc[j][2 * r], acc[j][2 * r + 1]};
+                    if (a.pairs_k && m0 + col + 1 < a.dk) {
+                        if (hh) { float z[2]; Vec<float, 2>::load(part + p + col, z); y[0] += z[0]; y[1] += z[1]; }
+                        if (hh + 1 < a.rep) Vec<float, 2>::store(part + p + col, y);
+                        else Vec<T, 2>::store(to + p + col, y);
+                    } else {
+#pragma unroll
+                        for (int s = 0; s < 2; ++s)
+                            if (m0 + col + s < a.dk) {
+                                if (hh) y[s] += part[p + col + s];
+                                if (hh + 1 < a.rep) part[p + col + s] = y[s];
+                                else to[p + col + s] = from_f<T>(y[s]);
+                            }
+                    }
+                }
+            }
+        }
+        if (keys) {
+#pragma unroll
+            for (int j = 0; j < DV / 8; ++j) {
+                dv[j][0] *= wl; dv[j][1] *= wl; dv[j][2] *= wh; dv[j][3] *= wh;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j += 2)
+                if (j >= 2 * w4) {
+                    const float x[8] = {qk[j][0], qk[j][1], qk[j][2], qk[j][3], qk[j + 1][0], qk[j + 1][1], qk[j + 1][2], qk[j + 1][3]};
+                    const Derived<T, 1> xd = derive<T, 1>(x);
+#pragma unroll
+                    for (int u = 0; u < DV / 8; u += 2) {
+                        OpB<T> b0, b1;
+                        load_b2<true>(b0, b1, sy, kLdV, 8 * u, 8 * j, lane);
+                        mma_derived<T, 1>(dv[u], xd, b0);
+                        mma_derived<T, 1>(dv[u + 1], xd, b1);
+                    }
+                }
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int row = r0 + gq + 8 * r;
+                if (row >= rows) continue;
+                T* to = (T*)a.dv_ + (((long long)b * a.L + first + row) * H + h) * a.dv;
+#pragma unroll
+                for (int j = 0; j < DV / 8; ++j) {
+                    const int col = 8 * j + 2 * t;
+                    const float y[2] = {dv[j][2 * r], dv[j][2 * r + 1]};
+                    if (a.pairs_v && col + 1 < a.dv) Vec<T, 2>::store(to + col, y);
+                    else {
+                        if (col < a.dv) to[col] = from_f<T>(y[0]);
+                        if (col + 1 < a.dv) to[col + 1] = from_f<T>(y[1]);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            through[r] *= r ? wh : wl;
+            through[r] += __shfl_xor_sync(0xffffffffu, through[r], 1);
+            through[r] += __shfl_xor_sync(0xffffffffu, through[r], 2);
+            if (t == 0) (keys ? from : into)[r0 + gq + 8 * r] = through[r];
+        }
+#pragma unroll
+        for (int off = 16; off; off >>= 1) both += __shfl_xor_sync(0xffffffffu, both, off);
+        if (lane == 0) cross[warp] = both;
+        __syncthreads();
+        if (tid < rows) {
+            float x = 0.f;
+            for (int i = 0; i < 8; ++i) x += cross[i];
+            x *= d.total;
+            for (int s = tid; s < kChunk; ++s) x += into[s] + (row_sum[s] - col_sum[s]);
+            for (int r = 0; r < tid; ++r) x += from[r];
+            // nothing crosses a reset; the pairs in front of it and behind it have cancelled to rounding only
+            const bool reset = d.n[tid] - (tid ? d.n[tid - 1] : 0.f) <= kFloor;
+            a.dg[((long long)b * a.L + first + tid) * H + h] = reset ? 0.f : x;
+        }
+    }
+}
+
+// ---- one token ---------------------------------------------------------------------------------------------------------
+struct StepArgs {
+    const void *q, *k, *v;
+    const float* g;
+    const float* state;
+    float* state_out;
+    void* o;                        // (B, H, dv)
+    long long q_b, q_h, k_b, k_h, v_b, v_h, g_b, g_h, s_b, so_b;
+    int H, rep, dk, dv;
+    float scale;
+};
+constexpr int kStepThreads = 256, kMostRow = 128;
+
+// A CTA has one head's state.  Threads stand on kVec neighbouring columns each and take every n-th row.
+template <typename T, int kVec>
+__global__ void __launch_bounds__(kStepThreads) la_step_kernel(const StepArgs a) {
+    follow_previous();
+    __shared__ float sq[kMostRow], sk[kMostRow];
+    __shared__ __align__(16) float part[kStepThreads * kVec];
+    const int tid = threadIdx.x, b = blockIdx.x / a.H, h = blockIdx.x % a.H;
+    const T* q = (const T*)a.q + b * a.q_b + (h / a.rep) * a.q_h;
+    const T* k = (const T*)a.k + b * a.k_b + (h / a.rep) * a.k_h;
+    for (int i = tid; i < a.dk; i += kStepThreads) { sq[i] = a.scale * to_f<T>(q[i]); sk[i] = to_f<T>(k[i]); }
+    const float keep = expf(a.g[b * a.g_b + h * a.g_h]);
+    const int across = (a.dv + kVec - 1) / kVec, down = kStepThreads / across, col = tid % across, row0 = tid / across;
+    const bool live = row0 < down;
+    float v[kVec], o[kVec] = {};
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) v[i] = to_f<T>(((const T*)a.v + b * a.v_b + h * a.v_h)[col * kVec + i]);
+    __syncthreads();
+    const long long first = (long long)h * a.dk * a.dv + col * kVec;
+    const float* s = a.state + b * a.s_b + first;
+    float* to = a.state_out + b * a.so_b + first;
+    if (live) {
+#pragma unroll 8
+        for (int r = row0; r < a.dk; r += down) {
+            float x[kVec];
+            Vec<float, kVec>::load(s + (long long)r * a.dv, x);
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) {
+                x[i] = fmaf(keep, x[i], sk[r] * v[i]);
+                o[i] = fmaf(sq[r], x[i], o[i]);
+            }
+            Vec<float, kVec>::store(to + (long long)r * a.dv, x);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) part[tid * kVec + i] = o[i];
+    __syncthreads();
+    T* out = (T*)a.o + (long long)blockIdx.x * a.dv;
+    for (int i = tid; i < a.dv; i += kStepThreads) {
+        float x = 0.f;
+        for (int r = 0; r < down; ++r) x += part[r * across * kVec + i];
+        out[i] = from_f<T>(x);
+    }
+}
+
+// ---- host --------------------------------------------------------------------------------------------------------------
+constexpr int kMostWidth = 128;
+
+int check_common(const ss2d_linear_attention_params& p) {
+    if (!p.q || !p.k || !p.v || !p.log_decay) return SS2D_EINVAL_NULL;
+    if (!dtype_ok(p.dtype)) return SS2D_EINVAL_DTYPE;
+    if (p.batch <= 0 || p.seqlen <= 0 || p.n_groups <= 0 || p.heads <= 0 || p.heads % p.n_groups || p.dk <= 0 || p.dv <= 0) return SS2D_EINVAL_SHAPE;
+    if (p.dk > kMostWidth || p.dv > kMostWidth) return SS2D_ENOTSUP;
+    // grids of (sequence, head, 256 elements of a state) and of (sequence, group, chunk)
+    if (p.seqlen > 0x7fffffc0LL || p.batch > 0x7fffffffLL / 64 / p.heads || p.batch * p.n_groups > 0x7fffffffLL / ((p.seqlen + kChunk - 1) / kChunk)) return SS2D_ENOTSUP;
+    for (int64_t s : {p.q_batch_stride, p.q_token_stride, p.q_head_stride, p.k_batch_stride, p.k_token_stride, p.k_head_stride, p.v_batch_stride,
+                      p.v_token_stride, p.v_head_stride, p.decay_batch_stride, p.decay_token_stride, p.decay_head_stride})
+        if (s < 0) return SS2D_EINVAL_STRIDE;
+    const size_t e = dtype_size(p.dtype);
+    if (!aligned_to(p.q, e) || !aligned_to(p.k, e) || !aligned_to(p.v, e) || !aligned_to(p.log_decay, 4)) return SS2D_EINVAL_ALIGN;
+    return SS2D_OK;
+}
+
+Rows rows_of(const void* p, int64_t b, int64_t l, int64_t h, int dtype) {
+    const int64_t per = 16 / (int64_t)dtype_size(dtype);
+    return {p, b, l, h, aligned_to(p, 16) && b % per == 0 && l % per == 0 && h % per == 0};
+}
+long long chunks_of(const ss2d_linear_attention_params& p) { return (p.seqlen + kChunk - 1) / kChunk; }
+
+// Segments of a sequence: where sequences, heads and slices leave SMs without a CTA, sequences are cut, and each segment's own state is gathered by a
+// walk of its own first.
+int segments_of(const ss2d_linear_attention_params& p) {
+    const long long ctas = p.batch * p.heads * ((p.dv + kSlice - 1) / kSlice), chunks = chunks_of(p);
+    const long long want = (2 * 148 + ctas - 1) / ctas;
+    if (want < 3 || chunks < 8) return 1;
+    const long long seg = want < chunks / 2 ? want : chunks / 2, per = (chunks + seg - 1) / seg;
+    return (int)((chunks + per - 1) / per);
+}
+long long segment_bytes(const ss2d_linear_attention_params& p) {
+    const long long seg = segments_of(p);
+    return seg == 1 ? 0 : 4 * p.batch * p.heads * seg * (p.dk * p.dv + 4);
+}
+
+template <typename F> int for_type(int dtype, F&& f) {
+    switch (dtype) {
+        case SS2D_F32: return f((float)0);
+        case SS2D_F16: return f(__half());
+        default: return f(__nv_bfloat16());
+    }
+}
+template <typename F> int for_dk(int64_t dk, F&& f) {
+    if (dk <= 32) return f(std::integral_constant<int, 32>());
+    if (dk <= 64) return f(std::integral_constant<int, 64>());
+    return f(std::integral_constant<int, 128>());
+}
+
+template <typename T, int DK, bool kOut, bool kBack> int launch_walk(const WalkArgs& a, long long bh, cudaStream_t st) {
+    auto kern = la_walk_kernel<T, DK, kOut, kBack>;
+    const size_t smem = WalkSmem<T, DK>::bytes(kOut);
+    if (const int rc = allow_dynamic_smem(kern, smem)) return rc;
+    launch(kern, dim3((unsigned)(bh * ((a.dv + kSlice - 1) / kSlice)), a.segments), 128, smem, st, a);
+    count_launch();
+    return check_launch();
+}
+
+// One pass over the sequences: gathers the segments' states first where there are several.  `first` and `last`: states before and behind the whole walk
+template <typename T, int DK, bool kOut, bool kBack>
+int walk(WalkArgs a, const float* first, float* last, void* workspace, long long bh, cudaStream_t st) {
+    const int seg = a.segments;
+    if (seg == 1) {
+        a.per_segment = a.chunks;
+        a.start = first; a.end = last;
+        return launch_walk<T, DK, kOut, kBack>(a, bh, st);
+    }
+    float* part = (float*)workspace;
+    float* decay = part + bh * seg * a.dk * a.dv;
+    a.per_segment = (a.chunks + seg - 1) / seg;
+    WalkArgs g = a;
+    if constexpr (kOut) g.q = Rows{};
+    g.states = nullptr; g.start = nullptr; g.end = part; g.end_decay = decay;
+    if (const int rc = launch_walk<T, DK, false, kBack>(g, bh, st)) return rc;
+    JoinArgs j = {first, part, decay, last, (long long)a.dk * a.dv, seg, kBack};
+    launch(la_join_kernel, (unsigned)(bh * ((j.size + 255) / 256)), 256, 0, st, j);
+    count_launch();
+    if (const int rc = check_launch()) return rc;
+    if (!kOut && !a.states) return SS2D_OK;
+    a.start = part; a.end = nullptr;
+    return launch_walk<T, DK, kOut, kBack>(a, bh, st);
+}
+
+WalkArgs walk_args(const ss2d_linear_attention_params& p) {
+    WalkArgs a = {};
+    a.g = (const float*)p.log_decay;
+    a.g_b = p.decay_batch_stride; a.g_l = p.decay_token_stride; a.g_h = p.decay_head_stride;
+    a.H = (int)p.heads; a.rep = (int)(p.heads / p.n_groups); a.L = (int)p.seqlen; a.dk = (int)p.dk; a.dv = (int)p.dv;
+    a.chunks = (int)chunks_of(p); a.segments = segments_of(p); a.scale = p.scale;
+    a.pairs = p.dv % 2 == 0;
+    return a;
+}
+
+}  // namespace
+
+long long linear_attention_workspace_bytes(const ss2d_linear_attention_params* p) {
+    if (!p || check_common(*p) != SS2D_OK) return -1;
+    return segment_bytes(*p);
+}
+
+int linear_attention_fwd(const ss2d_linear_attention_params* p, cudaStream_t st) {
+    if (!p) return SS2D_EINVAL_NULL;
+    if (const int rc = check_common(*p)) return rc;
+    if (!p->out) return SS2D_EINVAL_NULL;
+    if (!aligned_to(p->out, 2 * dtype_size(p->dtype)) || !aligned_to(p->initial_state, 4) || !aligned_to(p->final_state, 8) || !aligned_to(p->chunk_states, 8))
+        return SS2D_EINVAL_ALIGN;
+    const long long need = segment_bytes(*p), bh = p->batch * p->heads;
+    if (need && (!p->workspace || p->workspace_bytes < need || !aligned_to(p->workspace, 16))) return SS2D_EWORKSPACE;
+    WalkArgs a = walk_args(*p);
+    a.q = rows_of(p->q, p->q_batch_stride, p->q_token_stride, p->q_head_stride, p->dtype);
+    a.k = rows_of(p->k, p->k_batch_stride, p->k_token_stride, p->k_head_stride, p->dtype);
+    a.v = rows_of(p->v, p->v_batch_stride, p->v_token_stride, p->v_head_stride, p->dtype);
+    a.o = p->out;
+    a.states = (float*)p->chunk_states;
+    return for_type(p->dtype, [&](auto z) {
+        return for_dk(p->dk, [&](auto n) {
+            return walk<decltype(z), decltype(n)::value, true, false>(a, (const float*)p->initial_state, (float*)p->final_state, p->workspace, bh, st);
+        });
+    });
+}
+
+namespace {
+struct BwdPlan { long long segments, dstates, sums, total; };
+BwdPlan bwd_plan(const ss2d_linear_attention_params& p) {
+    BwdPlan b = {};
+    b.segments = (segment_bytes(p) + 255) / 256 * 256;
+    b.dstates = (4 * p.batch * p.heads * chunks_of(p) * p.dk * p.dv + 255) / 256 * 256;
+    b.sums = p.heads == p.n_groups ? 0 : (4 * p.batch * p.seqlen * p.n_groups * p.dk + 255) / 256 * 256;
+    b.total = b.segments + b.dstates + 2 * b.sums;
+    return b;
+}
+template <typename T, int DK, int DV> int launch_grad(const GradArgs& a, long long groups, cudaStream_t st) {
+    auto kern = la_grad_kernel<T, DK, DV>;
+    const size_t smem = GradSmem<T, DK, DV>::bytes();
+    if (const int rc = allow_dynamic_smem(kern, smem)) return rc;
+    launch(kern, (unsigned)(groups * a.chunks), 256, smem, st, a);
+    count_launch();
+    return check_launch();
+}
+}  // namespace
+
+long long linear_attention_bwd_workspace_bytes(const ss2d_linear_attention_bwd_params* p) {
+    if (!p || check_common(p->fwd) != SS2D_OK) return -1;
+    return bwd_plan(p->fwd).total;
+}
+
+int linear_attention_bwd(const ss2d_linear_attention_bwd_params* p, cudaStream_t st) {
+    if (!p) return SS2D_EINVAL_NULL;
+    const ss2d_linear_attention_params& f = p->fwd;
+    if (const int rc = check_common(f)) return rc;
+    if (!f.chunk_states || !p->dout || !p->dq || !p->dk || !p->dv || !p->dlog_decay) return SS2D_EINVAL_NULL;
+    if (p->dout_batch_stride < 0 || p->dout_token_stride < 0 || p->dout_head_stride < 0) return SS2D_EINVAL_STRIDE;
+    const size_t e = dtype_size(f.dtype);
+    if (!aligned_to(p->dout, e) || !aligned_to(p->dq, 2 * e) || !aligned_to(p->dk, 2 * e) || !aligned_to(p->dv, 2 * e) || !aligned_to(p->dlog_decay, 4) ||
+        !aligned_to(f.chunk_states, 8) || !aligned_to(p->dfinal_state, 4) || !aligned_to(p->dinitial_state, 8))
+        return SS2D_EINVAL_ALIGN;
+    const BwdPlan plan = bwd_plan(f);
+    if (!p->workspace || p->workspace_bytes < plan.total || !aligned_to(p->workspace, 16)) return SS2D_EWORKSPACE;
+    const long long bh = f.batch * f.heads;
+    char* ws = (char*)p->workspace;
+    float* dstates = (float*)(ws + plan.segments);
+    WalkArgs w = walk_args(f);
+    w.k = rows_of(f.q, f.q_batch_stride, f.q_token_stride, f.q_head_stride, f.dtype);
+    w.v = rows_of(p->dout, p->dout_batch_stride, p->dout_token_stride, p->dout_head_stride, f.dtype);
+    w.states = dstates;
+    GradArgs a = {};
+    a.q = w.k; a.dy = w.v;
+    a.k = rows_of(f.k, f.k_batch_stride, f.k_token_stride, f.k_head_stride, f.dtype);
+    a.v = rows_of(f.v, f.v_batch_stride, f.v_token_stride, f.v_head_stride, f.dtype);
+    a.g = w.g; a.g_b = w.g_b; a.g_l = w.g_l; a.g_h = w.g_h;
+    a.states = (const float*)f.chunk_states; a.dstates = dstates;
+    a.dq = p->dq; a.dk_ = p->dk; a.dv_ = p->dv; a.dg = (float*)p->dlog_decay;
+    a.sum_q = (float*)(ws + plan.segments + plan.dstates); a.sum_k = (float*)(ws + plan.segments + plan.dstates + plan.sums);
+    a.G = (int)f.n_groups; a.rep = w.rep; a.L = w.L; a.dk = w.dk; a.dv = w.dv; a.chunks = w.chunks; a.scale = f.scale;
+    a.pairs_k = a.dk % 2 == 0; a.pairs_v = a.dv % 2 == 0;
+    return for_type(f.dtype, [&](auto z) {
+        using T = decltype(z);
+        return for_dk(f.dk, [&](auto n) {
+            constexpr int DK = decltype(n)::value;
+            if (const int rc = walk<T, DK, false, true>(w, (const float*)p->dfinal_state, (float*)p->dinitial_state, ws, bh, st)) return rc;
+            return f.dv <= 64 ? launch_grad<T, DK, 64>(a, f.batch * f.n_groups, st) : launch_grad<T, DK, 128>(a, f.batch * f.n_groups, st);
+        });
+    });
+}
+
+int linear_attention_step(const ss2d_linear_attention_step_params* p, cudaStream_t st) {
+    if (!p || !p->q || !p->k || !p->v || !p->log_decay || !p->state || !p->state_out || !p->out) return SS2D_EINVAL_NULL;
+    if (!dtype_ok(p->dtype)) return SS2D_EINVAL_DTYPE;
+    if (p->batch <= 0 || p->n_groups <= 0 || p->heads <= 0 || p->heads % p->n_groups || p->dk <= 0 || p->dv <= 0) return SS2D_EINVAL_SHAPE;
+    if (p->dk > kMostWidth || p->dv > kMostWidth || p->batch > 0x7fffffffLL / p->heads) return SS2D_ENOTSUP;
+    const int64_t size = p->heads * p->dk * p->dv;
+    for (int64_t s : {p->q_batch_stride, p->q_head_stride, p->k_batch_stride, p->k_head_stride, p->v_batch_stride, p->v_head_stride,
+                      p->decay_batch_stride, p->decay_head_stride})
+        if (s < 0) return SS2D_EINVAL_STRIDE;
+    if (p->state_batch_stride < size || p->state_out_batch_stride < size) return SS2D_EINVAL_STRIDE;
+    const size_t e = dtype_size(p->dtype);
+    if (!aligned_to(p->q, e) || !aligned_to(p->k, e) || !aligned_to(p->v, e) || !aligned_to(p->out, e) || !aligned_to(p->log_decay, 4) ||
+        !aligned_to(p->state, 4) || !aligned_to(p->state_out, 4))
+        return SS2D_EINVAL_ALIGN;
+    StepArgs a = {p->q, p->k, p->v, (const float*)p->log_decay, (const float*)p->state, (float*)p->state_out, p->out,
+                  p->q_batch_stride, p->q_head_stride, p->k_batch_stride, p->k_head_stride, p->v_batch_stride, p->v_head_stride,
+                  p->decay_batch_stride, p->decay_head_stride, p->state_batch_stride, p->state_out_batch_stride,
+                  (int)p->heads, (int)(p->heads / p->n_groups), (int)p->dk, (int)p->dv, p->scale};
+    const bool vec = p->dv % 4 == 0 && p->state_batch_stride % 4 == 0 && p->state_out_batch_stride % 4 == 0 && aligned_to(p->state, 16) && aligned_to(p->state_out, 16);
+    return for_type(p->dtype, [&](auto z) {
+        using T = decltype(z);
+        const unsigned grid = (unsigned)(p->batch * p->heads);
+        if (vec) launch(la_step_kernel<T, 4>, grid, kStepThreads, 0, st, a);
+        else launch(la_step_kernel<T, 1>, grid, kStepThreads, 0, st, a);
+        count_launch();
+        return check_launch();
+    });
+}
+
+}  // namespace ss2d

@@ -175,6 +175,38 @@ selective_scan_cuda_oflex = _ExtShim()
 
 
 # --------------------------------------------------------------------------------------------
+# linear attention with a decay for each head
+# --------------------------------------------------------------------------------------------
+def linear_attention_fn(q, k, v, log_decay, scale=None, initial_state=None, return_final_state=False):
+    """Linear attention whose state decays, one rate for each head and token:
+
+        S_t = exp(log_decay_t) S_{t-1} + k_t v_t^T,    o_t = scale S_t^T q_t
+
+    the scan of the reference's m0 family (classification/models/vmamba.py:717-911: C, B and x dt are q, k and v, dt A is log_decay) and what
+    `selective_scan_fn` computes where all channels of a head share one decay.
+
+    q, k: (batch, tokens, groups, dk), v: (batch, tokens, heads, dv), one dtype (float32, float16, bfloat16); heads is a multiple of groups, and heads
+    h * groups // heads share their queries and keys.  Any strides (rows whose last dimension is not contiguous are copied); dk and dv up to 128.
+    log_decay: (batch, tokens, heads), or (heads,) for rates that the tokens share; computed in float32.  It is meant to be <= 0; -inf resets the state
+    (what lies below -138 does).  scale: default dk ** -0.5.  initial_state: (batch, heads, dk, dv), default zeros.
+    Returns o (batch, tokens, heads, dv) of v's dtype; with `return_final_state` also the state behind the last token, float32.  Differentiable in
+    all tensors; the backward pass keeps the inputs and the state in front of every 64th token.  Repeated calls give bit-identical results.
+
+    Sequences of other lengths in one batch: k = 0 and log_decay = 0 on the padding leave the state as it is.  A value that is not finite may reach all
+    outputs of its 64 tokens, also those in front of it."""
+    o, state = _host.linear_attention_fn(q, k, v, log_decay, scale, initial_state, bool(return_final_state))
+    return (o, state) if return_final_state else o
+
+
+def linear_attention_step(q, k, v, log_decay, state, scale=None, state_out=None):
+    """One token of every sequence through `linear_attention_fn`: (o, new state).
+
+    q, k: (batch, groups, dk), v: (batch, heads, dv), log_decay: (batch, heads) or (heads,), state: float32 (batch, heads, dk, dv), dense but for its
+    batch stride (a slice of a larger cache will do).  The new state goes to `state_out` (default: a new tensor), which may be `state` itself.  Inference only."""
+    return _host.linear_attention_step(q, k, v, log_decay, state, scale, state_out)
+
+
+# --------------------------------------------------------------------------------------------
 # CrossScan / CrossMerge
 # --------------------------------------------------------------------------------------------
 def _check_flags(in_channel_first, out_channel_first, one_by_one, scans):
