@@ -1,0 +1,69 @@
+"""Gated feed-forward block: what its entry points refuse, before any launch.  No GPU needed."""
+import ctypes
+import os
+import subprocess
+
+import pytest
+import torch
+
+from vmamba_b200 import _lib
+
+
+def params():
+    buf = (ctypes.c_float * 64)()
+    a = (ctypes.addressof(buf) + 63) // 64 * 64
+    p = _lib.GatedMlpParams()
+    for f in ("x", "w1", "w2", "h", "y"):
+        setattr(p, f, a)
+    p.tokens, p.channels, p.hidden, p.outputs, p.x_row_stride, p.dtype, p.act = 10, 16, 32, 16, 16, _lib.SS2D_BF16, 1
+    p.keep = buf
+    return p, a
+
+
+def test_refusals_of_the_c_interface():
+    L = _lib.lib()
+    before = _lib.launch_count()
+    call = L.ss2d_gated_mlp_fwd
+    assert call(None, None) == -1
+    p, a = params()
+    for field, bad, code in (("x", None, -1), ("w2", None, -1), ("h", None, -1), ("y", None, -1), ("dtype", 9, -3), ("act", 0, -6), ("act", 3, -6),
+                             ("tokens", 0, -2), ("hidden", -1, -2), ("x_row_stride", 15, -5), ("w1", a + 1, -4), ("h", a + 8, -4), ("b1", a + 1, -4),
+                             ("y", a + 2, -4), ("tokens", 1 << 40, -6)):
+        p, a = params()
+        setattr(p, field, bad)
+        assert call(p, None) == code, field
+    b = _lib.GatedMlpBwdParams()
+    assert L.ss2d_gated_mlp_bwd(None, None) == -1 and L.ss2d_gated_mlp_bwd(b, None) == -1 and L.ss2d_gated_mlp_bwd_workspace_bytes(b) < 0
+    b.fwd, a = params()
+    assert L.ss2d_gated_mlp_bwd(b, None) == -1                    # no dy, no pre
+    b.dy = b.fwd.pre = a
+    assert L.ss2d_gated_mlp_bwd(b, None) == -5
+    b.dy_row_stride = 16
+    need = L.ss2d_gated_mlp_bwd_workspace_bytes(b)
+    assert need >= 2 * 10 * 64
+    assert L.ss2d_gated_mlp_bwd(b, None) == -8
+    b.workspace, b.workspace_bytes = a, need - 1
+    assert L.ss2d_gated_mlp_bwd(b, None) == -8
+    b.workspace_bytes, b.dx = need, a + 2
+    assert L.ss2d_gated_mlp_bwd(b, None) == -4
+    assert _lib.launch_count() == before
+
+
+def test_struct_layout(tmp_path):
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    prog = tmp_path / "sz.c"
+    prog.write_text('#include "ss2d_b200.h"\n#include <stdio.h>\n#include <stddef.h>\nint main(){printf("%zu %zu %zu %zu\\n",sizeof(ss2d_gated_mlp_params),'
+                    'offsetof(ss2d_gated_mlp_params,act),sizeof(ss2d_gated_mlp_bwd_params),offsetof(ss2d_gated_mlp_bwd_params,dy_row_stride));return 0;}\n')
+    exe = tmp_path / "sz"
+    subprocess.check_call(["gcc", "-I", os.path.join(root, "include"), str(prog), "-o", str(exe)])
+    A, B = _lib.GatedMlpParams, _lib.GatedMlpBwdParams
+    assert [int(t) for t in subprocess.check_output([str(exe)]).split()] == [ctypes.sizeof(A), A.act.offset, ctypes.sizeof(B), B.dy_row_stride.offset]
+
+
+def test_cpu_tensors_and_unknown_activations_are_refused():
+    import vmamba_b200 as vb
+    x, w1, w2 = torch.zeros(3, 8), torch.zeros(32, 8), torch.zeros(8, 16)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        vb.gated_mlp_fn(x, w1, w2)
+    with pytest.raises(ValueError, match="activation"):
+        vb.gated_mlp_fn(x, w1, w2, act="relu")

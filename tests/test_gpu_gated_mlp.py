@@ -1,0 +1,289 @@
+"""Gated feed-forward block against its formulas in 64 bits.
+
+Tolerances count, term by term: half a step of the type for every result and for what is rounded to it on the way (the hidden map, the gradients of value and
+gate); fp32 sums of n terms, n 2^-24 of the sum of magnitudes, and 2^-21 for products of pieces and the exponentials; and what an error of value or gate does behind the
+activation, whose derivative is at most 1.13 and whose second derivative at most 0.8 in magnitude.
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
+ORDER = ("x", "w1", "w2", "b1", "b2")
+
+
+@pytest.fixture(scope="module")
+def vb():
+    import vmamba_b200
+    return vmamba_b200
+
+
+def make(M, C, H, O, dtype, biases=True, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    rnd = lambda *s: torch.randn(s, generator=g)      # noqa: E731
+    t = {"x": rnd(M, C), "w1": rnd(2 * H, C) / C ** 0.5, "w2": rnd(O, H) / H ** 0.5}
+    if biases:
+        t["b1"], t["b2"] = 0.3 * rnd(2 * H), rnd(O)
+    return {n: v.to(dtype).cuda() for n, v in t.items()}, rnd(M, O).to(dtype).cuda()
+
+
+def bent(g, act):
+    """act, its derivative"""
+    if act == "silu":
+        s = torch.sigmoid(g)
+        return g * s, s * (1 + g * (1 - s))
+    phi = 0.5 * torch.erfc(-g / math.sqrt(2))
+    return g * phi, phi + g * torch.exp(-g * g / 2) / math.sqrt(2 * math.pi)
+
+
+def reference(t, dy, act, dtype):
+    """{name: (value, tolerance)}"""
+    u = HALF[dtype]
+    f = {n: v.detach().double() for n, v in t.items()}
+    x, w1, w2, dy = f["x"], f["w1"], f["w2"], dy.double()
+    (M, C), (O, H) = x.shape, w2.shape
+    b1 = f.get("b1", torch.zeros(2 * H, dtype=torch.float64, device="cuda"))
+    b2 = f.get("b2", torch.zeros(O, dtype=torch.float64, device="cuda"))
+    s = lambda n: (n + 2) * 2.0 ** -24 + 2.0 ** -21      # noqa: E731
+    v, g = (x @ w1.t() + b1).chunk(2, -1)
+    ev, eg = (s(C) * (x.abs() @ w1.abs().t() + b1.abs())).chunk(2, -1)
+    a, da = bent(g, act)
+    ea, eda = 1.13 * eg + 2.0 ** -21 * g.abs(), 0.8 * eg + 2.0 ** -20
+    h = v * a
+    eh = u * h.abs() + 1.01 * (ev * a.abs() + v.abs() * ea + ev * ea)
+    y = h @ w2.t() + b2
+    out = {"y": (y, eh @ w2.abs().t() + s(H) * (h.abs() @ w2.abs().t() + b2.abs()))}
+    dh = dy @ w2
+    edh = s(O) * (dy.abs() @ w2.abs())
+    dz = torch.cat((dh * a, dh * v * da), 1)
+    edz = torch.cat((edh * a.abs() + dh.abs() * ea + edh * ea,
+                     edh * (v * da).abs() + dh.abs() * (ev * da.abs() + v.abs() * eda + ev * eda) + edh * (ev * 1.13 + v.abs() * eda)), 1)
+    edz = 1.01 * edz + u * dz.abs()
+    out["x"] = (dz @ w1, edz @ w1.abs() + s(2 * H) * (dz.abs() @ w1.abs()))
+    out["w1"] = (dz.t() @ x, edz.t() @ x.abs() + s(M) * (dz.abs().t() @ x.abs()))
+    out["w2"] = (dy.t() @ h, dy.abs().t() @ eh + s(M) * (dy.abs().t() @ h.abs()))
+    out["b1"] = (dz.sum(0), edz.sum(0) + s(M) * dz.abs().sum(0))
+    out["b2"] = (dy.sum(0), s(M) * dy.abs().sum(0))
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 1e-38
+    return {n: (r, 1.01 * e + u * r.abs() + tiny * (1 + H)) for n, (r, e) in out.items()}
+
+
+def compare(got, ref, dtype):
+    for n, y in got.items():
+        r, tol = ref[n]
+        assert y.shape == r.shape and y.dtype == dtype, n
+        err = (y.double() - r).abs()
+        worst, rel = (err / tol).max().item(), (err.norm() / r.norm().clamp(min=1e-30)).item()
+        print(f"{n}: {worst:.3f} of the tolerance, relative error {rel:.2e}")
+        assert torch.isfinite(y).all() and worst <= 1, (n, worst)
+        # independent roundings: at most three on the way, each of a root mean square of half a step / sqrt(3)
+        assert y.numel() < 1000 or rel <= max(HALF[dtype], 2.0 ** -18), (n, rel)
+
+
+def run(vb, t, dy, act):
+    leaves = {n: v.detach().requires_grad_() for n, v in t.items()}
+    y = vb.gated_mlp_fn(**leaves, act=act)
+    return {"y": y.detach(), **dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), dy)))}
+
+
+SHAPES = [(1, 8, 8, 8), (1, 768, 1024, 768), (3, 64, 128, 64), (7, 200, 504, 96), (16, 96, 384, 96), (17, 128, 256, 128), (33, 72, 152, 40), (64, 64, 64, 64),
+          (65, 65, 33, 17), (100, 50, 30, 10), (130, 96, 256, 96), (250, 384, 1536, 384), (300, 1, 1, 1), (1000, 192, 512, 192), (2050, 128, 136, 264)]
+
+
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_against_the_formulas(vb, shape, dtype, act):
+    t, dy = make(*shape, dtype)
+    ref = reference(t, dy, act, dtype)
+    compare(run(vb, t, dy, act), ref, dtype)
+    with torch.no_grad():
+        compare({"y": vb.gated_mlp_fn(**t, act=act)}, ref, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_without_biases_and_with_one(vb, dtype):
+    t, dy = make(150, 64, 128, 64, dtype, biases=False)
+    compare(run(vb, t, dy, "silu"), reference(t, dy, "silu", dtype), dtype)
+    for name in ("b1", "b2"):
+        full, _ = make(150, 64, 128, 64, dtype)
+        one = {**t, name: full[name]}
+        compare(run(vb, one, dy, "gelu"), reference(one, dy, "gelu", dtype), dtype)
+
+
+@pytest.mark.parametrize("M", [5, 150, 600])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_strides_and_shapes(vb, dtype, M):
+    t, dy = make(M, 64, 128, 64, dtype)
+    want = run(vb, t, dy, "gelu")
+    wide = torch.zeros(M, 80, dtype=dtype, device="cuda")
+    for off in (0, 8, 3):                                          # rows apart, on any element
+        wide[:, off:off + 64] = t["x"]
+        got = run(vb, {**t, "x": wide[:, off:off + 64]}, dy, "gelu")
+        compare(got, reference(t, dy, "gelu", dtype), dtype)
+    got = run(vb, {**t, "w1": t["w1"].t().contiguous().t(), "x": t["x"].t().contiguous().t()}, dy.t().contiguous().t(), "gelu")
+    assert all(torch.equal(got[n], want[n]) for n in want)
+    y = vb.gated_mlp_fn(t["x"].view(1, M, 1, 64), t["w1"], t["w2"], t["b1"], t["b2"])
+    assert y.shape == (1, M, 1, 64) and torch.equal(y.view(M, 64), want["y"])
+    y = vb.gated_mlp_fn(t["x"][0], t["w1"], t["w2"], t["b1"], t["b2"])
+    assert y.shape == (64,)
+    same = t["x"][:1].expand(M, 64).detach().requires_grad_()      # one token for all rows
+    y = vb.gated_mlp_fn(same, t["w1"], t["w2"], t["b1"], t["b2"])
+    assert all(torch.equal(y[0], r) for r in y)
+    g, = torch.autograd.grad(y, same, dy[:1].expand(M, 64))
+    assert g.shape == same.shape
+
+
+def test_gradients_against_differences(vb):
+    """fp32, central differences along signs; the third derivative of the loss along a direction is bounded through that of the activation (3 in magnitude)."""
+    t, dy = make(20, 24, 40, 16, torch.float32)
+    got = run(vb, t, dy, "gelu")
+    loss = lambda q: (vb.gated_mlp_fn(**q).double() * dy.double()).sum()      # noqa: E731
+    gen = torch.Generator().manual_seed(3)
+    f = {n: v.double() for n, v in t.items()}
+    for n in t:
+        d = torch.randn(t[n].shape, generator=gen).sign().cuda()
+        e = 2.0 ** -9
+        diff = (loss({**t, n: t[n] + e * d}) - loss({**t, n: t[n] - e * d})) / (2 * e)
+        want = (got[n].double() * d.double()).sum()
+        up = {k: v.abs() + (e if k == n else 0) for k, v in f.items()}
+        z = up["x"] @ up["w1"].t() + up["b1"]
+        zd = {"x": torch.ones_like(up["x"]) @ up["w1"].t(), "w1": up["x"].sum(1, keepdim=True).expand_as(z), "b1": torch.ones_like(z)}.get(n, torch.zeros_like(z))
+        (v, g), (dv, dg) = z.chunk(2, -1), zd.chunk(2, -1)
+        back = dy.abs().double() @ up["w2"]
+        third = (back * (3 * v * dg ** 3 + 3 * 0.8 * dv * dg ** 2)).sum()
+        noise = 64 * 2.0 ** -24 * ((dy.abs() * (((v * g) @ up["w2"].t()) + up["b2"])).sum()) / e
+        print(n, diff.item(), want.item(), third.item() * e * e / 6, noise.item())
+        assert abs(diff - want) <= third * e * e / 6 + noise
+
+
+def test_large_and_small_gates(vb):
+    """Gates far out: the activation is the gate or zero, its derivative one or zero, and nothing overflows on the way."""
+    for dtype in (torch.float32, torch.bfloat16):
+        for act in ("gelu", "silu"):
+            x = torch.tensor([[1.0], [-1.0]], device="cuda").repeat(40, 8).to(dtype)
+            w1 = torch.cat((torch.ones(16, 8), 100.0 * torch.ones(16, 8))).cuda().to(dtype).requires_grad_()
+            w2 = torch.ones(8, 16, device="cuda", dtype=dtype)
+            y = vb.gated_mlp_fn(x, w1, w2, act=act)
+            assert (y[0::2] == 16 * 8 * 800).all() and (y[1::2] == 0).all()
+            g, = torch.autograd.grad(y, w1, torch.ones_like(y))
+            assert torch.isfinite(g).all()
+
+
+def test_no_tokens(vb):
+    t, _ = make(4, 16, 32, 8, torch.bfloat16)
+    leaves = {n: v.requires_grad_() for n, v in t.items()}
+    leaves["x"] = torch.zeros(2, 0, 16, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    y = vb.gated_mlp_fn(**leaves)
+    assert y.shape == (2, 0, 8) and y.dtype == torch.bfloat16
+    grads = torch.autograd.grad(y.sum(), list(leaves.values()))
+    assert all(g.shape == v.shape and (g == 0).all() for g, v in zip(grads, leaves.values()))
+
+
+@pytest.mark.parametrize("M", [4, 200])
+def test_only_some_gradients(vb, M):
+    t, dy = make(M, 64, 128, 64, torch.bfloat16)
+    want = run(vb, t, dy, "gelu")
+    for n in ORDER:
+        leaves = {k: v.detach() for k, v in t.items()}
+        leaves[n].requires_grad_()
+        y = vb.gated_mlp_fn(**leaves)
+        g, = torch.autograd.grad(y, leaves[n], dy)
+        assert torch.equal(g, want[n]), n
+        leaves = {k: v.detach() for k, v in t.items() if k != "b1" or n == "b1"}      # a missing bias in front of the one that is asked for
+        leaves[n].requires_grad_()
+        g, = torch.autograd.grad(vb.gated_mlp_fn(**leaves), leaves[n], dy)
+        assert g.shape == t[n].shape
+
+
+@pytest.mark.parametrize("M", [3, 300])
+def test_same_bits_streams_graphs_autocast(vb, M):
+    t, dy = make(M, 96, 256, 96, torch.bfloat16)
+    want = run(vb, t, dy, "gelu")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = run(vb, t, dy, "gelu")
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(want[n], again[n]) for n in want)
+    with torch.autocast("cuda", dtype=torch.float16):
+        again = run(vb, t, dy, "gelu")
+    assert all(torch.equal(want[n], again[n]) for n in want)
+    torch.cuda.synchronize()
+    graphs = []
+    for k in range(2):
+        x = t["x"] * (k + 1)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got = run(vb, {**t, "x": x}, dy, "gelu")
+        graphs.append((g, x, got))
+    for _ in range(2):
+        for g, _, _ in graphs:
+            g.replay()
+    torch.cuda.synchronize()
+    for _, x, got in graphs:
+        now = run(vb, {**t, "x": x}, dy, "gelu")
+        assert all(torch.equal(now[n], got[n]) for n in now)
+
+
+def test_refusals(vb):
+    t, _ = make(4, 16, 32, 8, torch.bfloat16)
+    f = vb.gated_mlp_fn
+    for bad in ({**t, "w1": t["w1"][:62]}, {**t, "w2": t["w2"][:, :30]}, {**t, "b1": t["b1"][:32]}, {**t, "b2": t["b2"][:4]}, {**t, "x": t["x"][:, :8]},
+                {**t, "w1": t["w1"].cpu()}, {**t, "w1": t["w1"][0]}):
+        with pytest.raises(RuntimeError):
+            f(**bad)
+    for bad in ({**t, "w1": t["w1"].float()}, {**t, "b2": t["b2"].float()}, {n: v.double() for n, v in t.items()}):
+        with pytest.raises(TypeError):
+            f(**bad)
+
+
+def test_block_of_attention_and_feed_forward(vb):
+    """The operators as a block runs them: queries, keys, values and decays from one projection, attention, residual, feed-forward, residual; a whole
+    sequence against a prompt and single tokens, and its training step against the formulas."""
+    B, L, H, d, C = 2, 100, 4, 16, 64
+    g = torch.Generator().manual_seed(0)
+    rnd = lambda *s: torch.randn(s, generator=g).cuda()      # noqa: E731
+    wi, w1, w2 = rnd(3 * C + H, C) / C ** 0.5, rnd(4 * C, C) / C ** 0.5, rnd(C, 2 * C) / C ** 0.5
+    x = rnd(B, L, C)
+
+    def split(z):
+        q, k, v, r = z.split((C, C, C, H), -1)
+        heads = lambda y: y.unflatten(-1, (H, d))      # noqa: E731
+        return heads(q), heads(k), heads(v), -torch.nn.functional.softplus(r)
+
+    def whole(x, wi, w1, w2, state=None):
+        o, S = vb.linear_attention_fn(*split(x @ wi.t()), initial_state=state, return_final_state=True)
+        x = x + o.flatten(-2)
+        return x + vb.gated_mlp_fn(x, w1, w2), S
+
+    def formulas(x, wi, w1, w2):
+        q, k, v, r = split(x @ wi.t())
+        S, o = torch.zeros(B, H, d, d, dtype=x.dtype, device="cuda"), []
+        for t in range(L):
+            S = torch.exp(r[:, t])[..., None, None] * S + k[:, t, :, :, None] * v[:, t, :, None, :]
+            o.append(d ** -0.5 * (q[:, t, :, :, None] * S).sum(-2))
+        x = x + torch.stack(o, 1).flatten(-2)
+        a, b = (x @ w1.t()).chunk(2, -1)
+        return x + (a * torch.nn.functional.gelu(b)) @ w2.t()
+
+    ref_in = [t.double().requires_grad_() for t in (x, wi, w1, w2)]
+    own_in = [t.clone().requires_grad_() for t in (x, wi, w1, w2)]
+    up = rnd(B, L, C)
+    want, (got, _) = formulas(*ref_in), whole(*own_in)
+    wanted, found = torch.autograd.grad(want, ref_in, up.double()), torch.autograd.grad(got, own_in, up)
+    # fp32 throughout: four products of up to 256 terms in a row, each of at most (256 + 2) 2^-24 of magnitudes that random signs leave some
+    # 16 times as large as the results, and as much again behind them
+    for a, b in zip((want, *wanted), (got, *found)):
+        assert (a - b).norm() <= 2.0 ** -13 * a.norm()
+    with torch.no_grad():
+        y, S = whole(x[:, :90], wi, w1, w2)
+        for t in range(90, L):
+            z = x[:, t]
+            o, S = vb.linear_attention_step(*split(z @ wi.t()), S, state_out=S)
+            z = z + o.flatten(-2)
+            z = z + vb.gated_mlp_fn(z, w1, w2)
+            assert (z - want[:, t]).norm() <= 2.0 ** -13 * want[:, t].norm()

@@ -388,3 +388,18 @@ def test_refusals(vb):
         step(*one, two[:s.numel()].view(s.shape), state_out=two[4:4 + s.numel()].view(s.shape))
     with pytest.raises(RuntimeError, match="no backward"):
         step(*one, s.clone().requires_grad_())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_long_memory(vb, dtype):
+    """No decay: the state is a sum over all tokens, here of positive terms.  Chunks are summed apart (64 terms of two pieces, cut off: 2^-16) and added in fp32
+    (512 roundings of 2^-24 at most, and as many products with a decay of one), so that the sum is as good after 32 768 tokens as after a few."""
+    B, L, H, d = 1, 32768, 2, 16
+    t, _ = make(B, L, H, H, d, d, dtype)
+    k, v = t["k"].abs(), t["v"].abs()
+    with torch.no_grad():
+        _, S = vb.linear_attention_fn(t["q"], k, v, torch.zeros(H, device="cuda"), return_final_state=True)
+    want = torch.einsum("blhk,blhv->bhkv", k.double(), v.double())
+    assert ((S - want).abs() / want).max() <= 2.0 ** -16 + 1024 * 2.0 ** -24 / 3
+    # the roundings of the additions are of random sign, those of the products fall off: a chunk's error is at most 24 steps of 2^-24 cut off
+    assert (S - want).norm() <= 2.0 ** -18 * want.norm()

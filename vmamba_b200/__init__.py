@@ -9,7 +9,7 @@ from . import _host  # noqa: E402,F401  the host extension of the same build
 
 from .ops import (CrossMerge, CrossMergeF, CrossMergeTritonF, CrossScan, CrossScanF, CrossScanTritonF,  # noqa: E402
                   SelectiveScanCuda, SelectiveScanOflex, cross_merge_fn, cross_merge_fwd, cross_scan_fn,
-                  cross_scan_fwd, flops_selective_scan_fn, layer_norm_cf, linear_attention_fn, linear_attention_step,
+                  cross_scan_fwd, flops_selective_scan_fn, gated_mlp_fn, layer_norm_cf, linear_attention_fn, linear_attention_step,
                   selective_scan_bwd, selective_scan_cuda_oflex,
                   selective_scan_flop_jit, selective_scan_fn, selective_scan_fwd)
 from .fused import CoreWeights, disable_fused, enable_fused, ss2d_core, ss2d_core_autograd  # noqa: E402
@@ -22,7 +22,7 @@ __all__ = [
     "selective_scan_cuda_oflex", "flops_selective_scan_fn", "selective_scan_flop_jit",
     "cross_scan_fn", "cross_merge_fn", "cross_scan_fwd", "cross_merge_fwd",
     "CrossScanF", "CrossMergeF", "CrossScanTritonF", "CrossMergeTritonF", "CrossScan", "CrossMerge",
-    "linear_attention_fn", "linear_attention_step",
+    "linear_attention_fn", "linear_attention_step", "gated_mlp_fn",
     "layer_norm_cf", "ss2d_core", "ss2d_core_autograd", "CoreWeights", "enable_fused", "disable_fused",
     "install", "uninstall", "preseed_sys_modules", "preseed_extension_module", "GraphedBackbone",
     "VSSMInfer", "AcceleratedVSSM", "accelerate",

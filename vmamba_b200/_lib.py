@@ -143,6 +143,16 @@ class LinearAttentionStepParams(ctypes.Structure):
                                     "state_batch_stride", "state_out_batch_stride")] + [("dtype", _i32), ("scale", _f32)]
 
 
+class GatedMlpParams(ctypes.Structure):
+    _fields_ = [(n, _vp) for n in ("x", "w1", "b1", "w2", "b2", "h", "pre", "y")] + \
+               [(n, _i64) for n in ("tokens", "channels", "hidden", "outputs", "x_row_stride")] + [("dtype", _i32), ("act", _i32)]
+
+
+class GatedMlpBwdParams(ctypes.Structure):
+    _fields_ = [("fwd", GatedMlpParams)] + [(n, _vp) for n in ("dy", "dx", "dw1", "db1", "dw2", "db2", "workspace")] + \
+               [("workspace_bytes", _i64), ("dy_row_stride", _i64)]
+
+
 EXPORTS = {
     # name: (restype, argtypes)
     "ss2d_selective_scan_fwd": (ctypes.c_int, [ctypes.POINTER(ScanParams), _vp]),
@@ -183,6 +193,9 @@ EXPORTS = {
     "ss2d_linear_attention_bwd": (ctypes.c_int, [ctypes.POINTER(LinearAttentionBwdParams), _vp]),
     "ss2d_linear_attention_bwd_workspace_bytes": (_i64, [ctypes.POINTER(LinearAttentionBwdParams)]),
     "ss2d_linear_attention_step": (ctypes.c_int, [ctypes.POINTER(LinearAttentionStepParams), _vp]),
+    "ss2d_gated_mlp_fwd": (ctypes.c_int, [ctypes.POINTER(GatedMlpParams), _vp]),
+    "ss2d_gated_mlp_bwd": (ctypes.c_int, [ctypes.POINTER(GatedMlpBwdParams), _vp]),
+    "ss2d_gated_mlp_bwd_workspace_bytes": (_i64, [ctypes.POINTER(GatedMlpBwdParams)]),
     "ss2d_set_debug_checks": (ctypes.c_int, [ctypes.c_int]),
     "ss2d_version": (ctypes.c_int, []),
     "ss2d_strerror": (ctypes.c_char_p, [ctypes.c_int]),

@@ -6,6 +6,7 @@ void bind_ops(pybind11::module_& m);
 void bind_core(pybind11::module_& m);
 void bind_backbone(pybind11::module_& m);
 void bind_attention(pybind11::module_& m);
+void bind_gated_mlp(pybind11::module_& m);
 }  // namespace host
 
 PYBIND11_MODULE(_host, m) {
@@ -23,4 +24,5 @@ PYBIND11_MODULE(_host, m) {
     host::bind_core(m);
     host::bind_backbone(m);
     host::bind_attention(m);
+    host::bind_gated_mlp(m);
 }

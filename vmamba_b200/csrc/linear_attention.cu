@@ -266,33 +266,35 @@ __global__ void __launch_bounds__(128) la_walk_kernel(const WalkArgs a) {
         // state: rows of k^T weighted by what is left of them at the end of the chunk (backwards: of q^T by what reaches them)
         const float keep = d.total;
         if (holds) {
+            // a chunk's products are summed on their own: tensor cores cut sums off towards zero, which a state of thousands of tokens would collect
 #pragma unroll
-            for (int m = 0; m < kBlocks; ++m)
+            for (int m = 0; m < kBlocks; ++m) {
+                float add[8][4] = {};
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
+                for (int k0 = 0; k0 < kChunk; k0 += 16) {
+                    const float* w = kBack ? d.e : d.w;
+                    float ws[4] = {w[k0 + 2 * t], w[k0 + 2 * t + 1], w[k0 + 8 + 2 * t], w[k0 + 9 + 2 * t]};
+                    if constexpr (kBack) {
 #pragma unroll
-                    for (int s = 0; s < 4; ++s) S[m][j][s] *= keep;
-#pragma unroll
-            for (int k0 = 0; k0 < kChunk; k0 += 16) {
-                const float* w = kBack ? d.e : d.w;
-                float ws[4] = {w[k0 + 2 * t], w[k0 + 2 * t + 1], w[k0 + 8 + 2 * t], w[k0 + 9 + 2 * t]};
-                if constexpr (kBack) {
-#pragma unroll
-                    for (int s = 0; s < 4; ++s) ws[s] *= a.scale;
-                }
-                OpB<T> vb[8];
-#pragma unroll
-                for (int j = 0; j < 8; j += 2) load_b2<true>(vb[j], vb[j + 1], sv, M::kLdV, 8 * j, k0, lane);
-#pragma unroll
-                for (int m = 0; m < kBlocks; ++m) {
+                        for (int s = 0; s < 4; ++s) ws[s] *= a.scale;
+                    }
                     float x[8];
                     values(load_a<true>(sk, M::kLdK, m_first + 64 * m, k0, lane), x);
 #pragma unroll
                     for (int s = 0; s < 8; ++s) x[s] *= ws[(s & 1) + 2 * (s >> 2)];
                     const Derived<T, 2> kd = derive<T, 2>(x);       // two pieces: the state is an fp32 result
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) mma_derived<T, 2>(S[m][j], kd, vb[j]);
+                    for (int j = 0; j < 8; j += 2) {
+                        OpB<T> b0, b1;
+                        load_b2<true>(b0, b1, sv, M::kLdV, 8 * j, k0, lane);
+                        mma_derived<T, 2>(add[j], kd, b0);
+                        mma_derived<T, 2>(add[j + 1], kd, b1);
+                    }
                 }
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+#pragma unroll
+                    for (int s = 0; s < 4; ++s) S[m][j][s] = fmaf(keep, S[m][j][s], add[j][s]);
             }
         }
         put_plane();

@@ -503,6 +503,20 @@ def mlp_fused(x: torch.Tensor, w1: torch.Tensor, b1: torch.Tensor, w2: torch.Ten
     return y
 
 
+def gated_mlp_fn(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, b1=None, b2=None, act="gelu") -> torch.Tensor:
+    """Gated feed-forward block, gMlp.forward (classification/models/vmamba.py:131-149) on tokens:
+
+        v, g = (x w1^T + b1).chunk(2, -1);    y = (v * act(g)) w2^T + b2
+
+    x: (..., channels), w1: (2 * hidden, channels), w2: (outputs, hidden), b1: (2 * hidden,) or None, b2: (outputs,) or None, all of one dtype (float32, float16,
+    bfloat16); act: "gelu" (erf) or "silu".  Returns (..., outputs).  Both projections, the activation and the product are one kernel; sums are fp32, the
+    hidden map is rounded to the inputs' type.  Differentiable in all tensors; the backward pass keeps x, the hidden map, and v and g in float32.
+    Repeated calls give bit-identical results."""
+    if act not in ("gelu", "silu"):
+        raise ValueError(f"unknown activation {act!r}: expected 'gelu' or 'silu'")
+    return _host.gated_mlp_fn(x, w1, w2, b1, b2, _ACTS[act])
+
+
 def linear_supported(M: int, K: int, n_pixels: int, dtype: torch.dtype) -> bool:
     """True when `linear_cf` takes a dense (K, n_pixels) map itself (the library's planner decides)."""
     if dtype not in (torch.bfloat16, torch.float16):
