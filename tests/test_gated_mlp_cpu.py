@@ -35,8 +35,8 @@ def test_refusals_of_the_c_interface():
     b = _lib.GatedMlpBwdParams()
     assert L.ss2d_gated_mlp_bwd(None, None) == -1 and L.ss2d_gated_mlp_bwd(b, None) == -1 and L.ss2d_gated_mlp_bwd_workspace_bytes(b) < 0
     b.fwd, a = params()
-    assert L.ss2d_gated_mlp_bwd(b, None) == -1                    # no dy, no pre
-    b.dy = b.fwd.pre = a
+    assert L.ss2d_gated_mlp_bwd(b, None) == -1                    # no dy
+    b.dy = a
     assert L.ss2d_gated_mlp_bwd(b, None) == -5
     b.dy_row_stride = 16
     need = L.ss2d_gated_mlp_bwd_workspace_bytes(b)

@@ -144,7 +144,7 @@ class LinearAttentionStepParams(ctypes.Structure):
 
 
 class GatedMlpParams(ctypes.Structure):
-    _fields_ = [(n, _vp) for n in ("x", "w1", "b1", "w2", "b2", "h", "pre", "y")] + \
+    _fields_ = [(n, _vp) for n in ("x", "w1", "b1", "w2", "b2", "h", "y")] + \
                [(n, _i64) for n in ("tokens", "channels", "hidden", "outputs", "x_row_stride")] + [("dtype", _i32), ("act", _i32)]
 
 

@@ -1,5 +1,7 @@
 // What follows the products of the gated feed-forward block, for accumulators of any kernel: value and gate to hidden, the gradients of both, biases.
 #pragma once
+#include <type_traits>
+
 #include "activations.cuh"
 
 namespace ss2d {
@@ -8,7 +10,7 @@ enum Epilogue { EPI_OUT = 0, EPI_GATE = 1, EPI_GRAD = 2, EPI_PART = 3 };
 
 struct EpiArgs {
     const void* bias;       // of the block's type or NULL: one for each output column (EPI_GATE: 2 hidden, values first)
-    void* out;              // EPI_OUT: (rows, cols); EPI_GATE: hidden (rows, hidden); EPI_GRAD: gradients of value and gate (rows, 2 hidden)
+    void* out;              // EPI_OUT: (rows, cols); EPI_GATE: hidden (rows, hidden) or NULL; EPI_GRAD: gradients of value and gate (rows, 2 hidden)
     float* pre;             // values and gates in front of the product, (rows, 2 hidden), fp32.  EPI_GATE: written unless NULL; EPI_GRAD: read
     float* part;            // EPI_PART: (splits, rows, cols)
     long long ld;           // elements between rows of `out`
@@ -30,6 +32,35 @@ template <int ACT> __device__ __forceinline__ void gate_act_grad(float g, float&
         const float s = __fdividef(1.0f, 1.0f + __expf(-g));
         a = g * s;
         da = s * fmaf(g, 1.0f - s, 1.0f);
+    }
+}
+
+// The same on pairs, for 16-bit types: gelu by a polynomial on the FMA pipe (error 3.5e-5), sigmoid through tanh.approx (2^-11 of tanh) where the
+// result is rounded to bf16, through an exponential and a division beside fp16.
+template <typename T> __device__ __forceinline__ float2 sigmoid_pair(float2 g) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const float2 h = __fmul2_rn(g, splat2(0.5f));
+        float2 t;
+        asm("tanh.approx.f32 %0, %1;" : "=f"(t.x) : "f"(h.x));
+        asm("tanh.approx.f32 %0, %1;" : "=f"(t.y) : "f"(h.y));
+        return __ffma2_rn(t, splat2(0.5f), splat2(0.5f));
+    } else
+        return make_float2(__fdividef(1.0f, 1.0f + __expf(-g.x)), __fdividef(1.0f, 1.0f + __expf(-g.y)));
+}
+template <typename T, int ACT> __device__ __forceinline__ float2 act_pair(float2 g) {
+    if constexpr (ACT == ACT_GELU) return __fmul2_rn(g, normal_cdf_pair(g));
+    else return __fmul2_rn(g, sigmoid_pair<T>(g));
+}
+template <typename T, int ACT> __device__ __forceinline__ void act_grad_pair(float2 g, float2& a, float2& da) {
+    if constexpr (ACT == ACT_GELU) {
+        const float2 phi = normal_cdf_pair(g);
+        const float2 e = __fmul2_rn(__fmul2_rn(g, g), splat2(-0.5f * kLog2e));
+        a = __fmul2_rn(g, phi);
+        da = __ffma2_rn(__fmul2_rn(g, splat2(0.3989422804014327f)), make_float2(ex2_approx(e.x), ex2_approx(e.y)), phi);
+    } else {
+        const float2 s = sigmoid_pair<T>(g);
+        a = __fmul2_rn(g, s);
+        da = __ffma2_rn(a, __ffma2_rn(s, splat2(-1.0f), splat2(1.0f)), s);
     }
 }
 
@@ -67,7 +98,7 @@ __device__ __forceinline__ void finish_pair(const EpiArgs& e, long long m, int n
             store_pair<float>(p, v[0], v[1], both, e.pairs);
             store_pair<float>(p + e.hidden, g[0], g[1], both, e.pairs);
         }
-        store_pair<T>((T*)e.out + m * e.ld + n, v[0] * gate_act<ACT>(g[0]), v[1] * gate_act<ACT>(g[1]), both, e.pairs);
+        if (e.out) store_pair<T>((T*)e.out + m * e.ld + n, v[0] * gate_act<ACT>(g[0]), v[1] * gate_act<ACT>(g[1]), both, e.pairs);
     } else {
         const float* p = e.pre + m * 2 * e.hidden + n;
         float v[2], g[2] = {0.f, 0.f}, a[2], da[2];

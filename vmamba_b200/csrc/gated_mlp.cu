@@ -1,10 +1,10 @@
 // Gated feed-forward block:  h = (x Wv^T + bv) * act(x Wg^T + bg),  y = h W2^T + b2, and its backward pass
 //   dh = dy W2;  dv = dh act(g);  dg = dh v act'(g);  dx = [dv dg] W1;  dW1 = [dv dg]^T x;  dW2 = dy^T h;  db1, db2 the column sums.
 // The two projections run as one product whose tile holds the same columns of value and gate, so that activation and product happen on its
-// accumulators; in the backward pass dh never leaves them either.  For training the forward call leaves v and g in fp32: rounded to 16 bits they would
-// put a second rounding into both gradients.
+// accumulators; in the backward pass dh never leaves them either.  Nothing but x and h is kept for it: v and g are computed again, in fp32.
 #include "gated_epilogue.cuh"
 #include "mma_tiles.cuh"
+#include "product_tc05.cuh"
 
 namespace ss2d {
 
@@ -206,50 +206,152 @@ int check_common(const ss2d_gated_mlp_params& p) {
     return SS2D_OK;
 }
 
-template <typename T, int ACT> int forward(const ss2d_gated_mlp_params& p, cudaStream_t st) {
+template <typename T, int ACT> int plain_forward(const ss2d_gated_mlp_params& p, cudaStream_t st) {
     ProductArgs a = product_args<T>(p.x, p.x_row_stride, p.w1, p.channels, p.tokens, p.hidden, p.channels);
     a.second = (int)p.hidden;
-    a.e.bias = p.b1; a.e.out = p.h; a.e.ld = p.hidden; a.e.hidden = (int)p.hidden; a.e.pre = (float*)p.pre; a.e.pairs = p.hidden % 2 == 0;
+    a.e.bias = p.b1; a.e.out = p.h; a.e.ld = p.hidden; a.e.hidden = (int)p.hidden; a.e.pairs = p.hidden % 2 == 0;
     if (const int rc = launch_product<T, false, false, EPI_GATE, ACT>(a, 1, st)) return rc;
     ProductArgs b = product_args<T>(p.h, p.hidden, p.w2, p.hidden, p.tokens, p.outputs, p.hidden);
     b.e.bias = p.b2; b.e.out = p.y; b.e.ld = p.outputs; b.e.pairs = p.outputs % 2 == 0;
     return launch_product<T, false, false, EPI_OUT, ACT_NONE>(b, 1, st);
 }
 
-struct BwdPlan { long long dz, part, total; };
+struct BwdPlan { long long dz, part, pre, total; };
+
+// 16-bit operands whose rows TMA can read: the tensor-core kernels.
+bool tc_fits(const ss2d_gated_mlp_params& p) {
+    if (p.dtype == SS2D_F32 || p.channels % 8 || p.hidden % 8 || p.outputs % 8 || p.x_row_stride % 8) return false;
+    for (const void* q : {p.x, p.w1, p.w2, p.b1, p.b2})
+        if (!aligned_to(q, 16)) return false;
+    return true;
+}
+
+// Time of a tensor-core product in cycles, for the choice among its tiles: rounds of tiles over the SMs, each as long as its MMAs (a step of 64 of the contraction
+// takes as many cycles as it has columns, and no fewer than 128 columns' worth) and a fixed part for filling the ring and the last tile's epilogue.
+double tc_cycles(long long tiles, long long steps, int columns) {
+    const long long rounds = (tiles + 147) / 148;
+    return (double)rounds * steps * (columns < 128 ? 128 : columns) + 1500.0;
+}
+long long tc_tiles(long long M, long long N, int out) { return ((M + ptc::kRows - 1) / ptc::kRows) * ((N + out - 1) / out); }
+
+template <typename T, int ACT> int tc_forward(const ss2d_gated_mlp_params& p, cudaStream_t st) {
+    ptc::Product a = {};
+    a.a = {p.x, p.x_row_stride}; a.b = {p.w1, p.channels};
+    a.M = p.tokens; a.N = p.hidden; a.K = p.channels; a.b_rows = 2 * p.hidden;
+    a.bias = p.b1; a.out = p.h; a.out_pitch = p.hidden;
+    const long long steps = (p.channels + ptc::kDepth - 1) / ptc::kDepth;
+    const bool wide = tc_cycles(tc_tiles(a.M, a.N, 128), steps, 256) <= tc_cycles(tc_tiles(a.M, a.N, 64), steps, 128);
+    if (const int rc = wide ? ptc::run_product<T, false, false, EPI_GATE, ACT, 256>(a, st) : ptc::run_product<T, false, false, EPI_GATE, ACT, 128>(a, st)) return rc;
+    ptc::Product b = {};
+    b.a = {p.h, p.hidden}; b.b = {p.w2, p.hidden};
+    b.M = p.tokens; b.N = p.outputs; b.K = p.hidden; b.b_rows = p.outputs;
+    b.bias = p.b2; b.out = p.y; b.out_pitch = p.outputs;
+    const long long steps2 = (p.hidden + ptc::kDepth - 1) / ptc::kDepth;
+    const bool wide2 = tc_cycles(tc_tiles(b.M, b.N, 256), steps2, 256) <= tc_cycles(tc_tiles(b.M, b.N, 128), steps2, 128);
+    return wide2 ? ptc::run_product<T, false, false, EPI_OUT, ACT_NONE, 256>(b, st) : ptc::run_product<T, false, false, EPI_OUT, ACT_NONE, 128>(b, st);
+}
+
+// Splits of a weight gradient's contraction over the tokens, and its tile: the fewest cycles, with the partial sums' way to memory and back (8 bytes an element
+// and split at about 3 300 bytes a cycle)
+struct WeightPlan { int splits, per_split; bool wide; };
+WeightPlan tc_weight_plan(long long M, long long N, long long K) {
+    const long long steps = (K + ptc::kDepth - 1) / ptc::kDepth;
+    WeightPlan best = {1, (int)steps, false};
+    double least = 1e30;
+    for (int wide = 0; wide < 2; ++wide)
+        for (long long s = 1; s <= 64 && s <= steps; ++s) {
+            const long long per = (steps + s - 1) / s, splits = (steps + per - 1) / per;
+            const double t = tc_cycles(tc_tiles(M, N, wide ? 256 : 128) * splits, per, wide ? 256 : 128) + (splits > 1 ? 3000.0 + 8.0 * splits * M * N / 3300.0 : 0.0);
+            if (t < least) { least = t; best = {(int)splits, (int)per, wide != 0}; }
+        }
+    return best;
+}
+template <typename T> int tc_weight_gradient(const void* a, long long lda, const void* b, long long ldb, long long M, long long N, long long K, void* out, float* part, cudaStream_t st) {
+    const WeightPlan w = tc_weight_plan(M, N, K);
+    ptc::Product p = {};
+    p.a = {a, lda}; p.b = {b, ldb};
+    p.M = M; p.N = N; p.K = K; p.b_rows = N; p.out_pitch = N;
+    if (w.splits == 1) {
+        p.out = out;
+        return w.wide ? ptc::run_product<T, true, true, EPI_OUT, ACT_NONE, 256>(p, st) : ptc::run_product<T, true, true, EPI_OUT, ACT_NONE, 128>(p, st);
+    }
+    p.out = part; p.splits = w.splits; p.per_split = w.per_split;
+    if (const int rc = w.wide ? ptc::run_product<T, true, true, EPI_PART, ACT_NONE, 256>(p, st) : ptc::run_product<T, true, true, EPI_PART, ACT_NONE, 128>(p, st)) return rc;
+    return add_parts<T>(part, out, M * N, w.splits, st);
+}
+
 BwdPlan bwd_plan(const ss2d_gated_mlp_params& p) {
     auto up = [](long long n) { return (n + 255) / 256 * 256; };
     BwdPlan b;
     b.dz = up(2 * p.tokens * p.hidden * (long long)dtype_size(p.dtype));
     const long long spans = (p.tokens + kSpan - 1) / kSpan;
     long long most = spans * (2 * p.hidden > p.outputs ? 2 * p.hidden : p.outputs);
-    for (long long n : {splits_of(2 * p.hidden, p.channels, p.tokens) * 2 * p.hidden * p.channels, splits_of(p.outputs, p.hidden, p.tokens) * p.outputs * p.hidden})
+    const long long M1 = 2 * p.hidden, N1 = p.channels, M2 = p.outputs, N2 = p.hidden;
+    for (long long n : {splits_of(M1, N1, p.tokens) * M1 * N1, splits_of(M2, N2, p.tokens) * M2 * N2, tc_weight_plan(M1, N1, p.tokens).splits * M1 * N1,
+                        tc_weight_plan(M2, N2, p.tokens).splits * M2 * N2})
         if (n > most) most = n;
     b.part = up(4 * most);
-    b.total = b.dz + b.part;
+    b.pre = up(8 * p.tokens * p.hidden);                      // of calls that the tensor-core kernels do not take, wherever their tensors start
+    b.total = b.dz + b.part + b.pre;
     return b;
 }
 
 template <typename T, int ACT> int backward(const ss2d_gated_mlp_bwd_params& p, cudaStream_t st) {
     const ss2d_gated_mlp_params& f = p.fwd;
     const BwdPlan plan = bwd_plan(f);
-    void* dz = p.workspace;
-    float* part = (float*)((char*)p.workspace + plan.dz);
-    const long long H2 = 2 * f.hidden;
+    char* const ws = (char*)p.workspace;
+    void* const dz = ws;
+    float *const part = (float*)(ws + plan.dz), *const pre = (float*)(ws + plan.dz + plan.part);
+    const long long H = f.hidden, H2 = 2 * H;
+    bool tc = false;
+    if constexpr (sizeof(T) == 2) {
+        tc = tc_fits(f) && p.dy_row_stride % 8 == 0;
+        for (const void* q : {p.dy, (const void*)p.dx, (const void*)p.dw1, (const void*)p.dw2}) tc = tc && aligned_to(q, 16);
+    }
     if (p.dx || p.dw1 || p.db1) {
-        ProductArgs a = product_args<T>(p.dy, p.dy_row_stride, f.w2, f.hidden, f.tokens, f.hidden, f.outputs);
-        a.e.out = dz; a.e.ld = H2; a.e.hidden = (int)f.hidden; a.e.pre = (float*)f.pre; a.e.pairs = f.hidden % 2 == 0;
-        if (const int rc = launch_product<T, false, true, EPI_GRAD, ACT>(a, 1, st)) return rc;
+        if constexpr (sizeof(T) == 2)
+            if (tc) {
+                ptc::Product a = {};
+                a.a = {f.x, f.x_row_stride}; a.b = {f.w1, f.channels}; a.a2 = {p.dy, p.dy_row_stride}; a.b2 = {f.w2, H};
+                a.M = f.tokens; a.N = H; a.K = f.channels; a.K2 = f.outputs; a.b_rows = H2; a.bias = f.b1;
+                a.out = dz; a.out2 = (T*)dz + H; a.out_pitch = H2;
+                if (const int rc = ptc::run_product<T, false, true, EPI_GRAD, ACT, 192>(a, st)) return rc;
+            }
+        if (!tc) {
+            ProductArgs g = product_args<T>(f.x, f.x_row_stride, f.w1, f.channels, f.tokens, H, f.channels);
+            g.second = (int)H;
+            g.e.bias = f.b1; g.e.hidden = (int)H; g.e.pre = pre; g.e.pairs = H % 2 == 0;
+            if (const int rc = launch_product<T, false, false, EPI_GATE, ACT>(g, 1, st)) return rc;
+            ProductArgs a = product_args<T>(p.dy, p.dy_row_stride, f.w2, H, f.tokens, H, f.outputs);
+            a.e.out = dz; a.e.ld = H2; a.e.hidden = (int)H; a.e.pre = pre; a.e.pairs = H % 2 == 0;
+            if (const int rc = launch_product<T, false, true, EPI_GRAD, ACT>(a, 1, st)) return rc;
+        }
     }
     if (p.dx) {
-        ProductArgs a = product_args<T>(dz, H2, f.w1, f.channels, f.tokens, f.channels, H2);
-        a.e.out = p.dx; a.e.ld = f.channels; a.e.pairs = f.channels % 2 == 0;
-        if (const int rc = launch_product<T, false, true, EPI_OUT, ACT_NONE>(a, 1, st)) return rc;
+        if constexpr (sizeof(T) == 2)
+            if (tc) {
+                ptc::Product a = {};
+                a.a = {dz, H2}; a.b = {f.w1, f.channels};
+                a.M = f.tokens; a.N = f.channels; a.K = H2; a.b_rows = f.channels; a.out = p.dx; a.out_pitch = f.channels;
+                const long long steps = (H2 + ptc::kDepth - 1) / ptc::kDepth;
+                const bool wide = tc_cycles(tc_tiles(a.M, a.N, 256), steps, 256) <= tc_cycles(tc_tiles(a.M, a.N, 128), steps, 128);
+                if (const int rc = wide ? ptc::run_product<T, false, true, EPI_OUT, ACT_NONE, 256>(a, st) : ptc::run_product<T, false, true, EPI_OUT, ACT_NONE, 128>(a, st)) return rc;
+            }
+        if (!tc) {
+            ProductArgs a = product_args<T>(dz, H2, f.w1, f.channels, f.tokens, f.channels, H2);
+            a.e.out = p.dx; a.e.ld = f.channels; a.e.pairs = f.channels % 2 == 0;
+            if (const int rc = launch_product<T, false, true, EPI_OUT, ACT_NONE>(a, 1, st)) return rc;
+        }
     }
+    auto weight = [&](const void* a, long long lda, const void* b, long long ldb, long long M, long long N, void* out) {
+        if constexpr (sizeof(T) == 2)
+            if (tc) return tc_weight_gradient<T>(a, lda, b, ldb, M, N, f.tokens, out, part, st);
+        return weight_gradient<T>(a, lda, b, ldb, M, N, f.tokens, out, part, st);
+    };
     if (p.dw1)
-        if (const int rc = weight_gradient<T>(dz, H2, f.x, f.x_row_stride, H2, f.channels, f.tokens, p.dw1, part, st)) return rc;
+        if (const int rc = weight(dz, H2, f.x, f.x_row_stride, H2, f.channels, p.dw1)) return rc;
     if (p.dw2)
-        if (const int rc = weight_gradient<T>(p.dy, p.dy_row_stride, f.h, f.hidden, f.outputs, f.hidden, f.tokens, p.dw2, part, st)) return rc;
+        if (const int rc = weight(p.dy, p.dy_row_stride, f.h, H, f.outputs, H, p.dw2)) return rc;
     if (p.db1)
         if (const int rc = column_sums<T>(dz, H2, f.tokens, (int)H2, p.db1, part, st)) return rc;
     if (p.db2)
@@ -274,8 +376,14 @@ int gated_mlp_fwd(const ss2d_gated_mlp_params* p, cudaStream_t st) {
     if (!p) return SS2D_EINVAL_NULL;
     if (const int rc = check_common(*p)) return rc;
     if (!p->h || !p->y) return SS2D_EINVAL_NULL;
-    if (!aligned_to(p->h, 16) || !aligned_to(p->y, 2 * dtype_size(p->dtype)) || !aligned_to(p->pre, 8)) return SS2D_EINVAL_ALIGN;
-    return for_type_act(p->dtype, p->act, [&](auto z, auto act) { return forward<decltype(z), decltype(act)::value>(*p, st); });
+    if (!aligned_to(p->h, 16) || !aligned_to(p->y, 2 * dtype_size(p->dtype))) return SS2D_EINVAL_ALIGN;
+    return for_type_act(p->dtype, p->act, [&](auto z, auto act) {
+        using T = decltype(z);
+        constexpr int A = decltype(act)::value;
+        if constexpr (sizeof(T) == 2)
+            if (tc_fits(*p) && aligned_to(p->y, 16)) return tc_forward<T, A>(*p, st);
+        return plain_forward<T, A>(*p, st);
+    });
 }
 
 long long gated_mlp_bwd_workspace_bytes(const ss2d_gated_mlp_bwd_params* p) {
@@ -287,10 +395,10 @@ int gated_mlp_bwd(const ss2d_gated_mlp_bwd_params* p, cudaStream_t st) {
     if (!p) return SS2D_EINVAL_NULL;
     const ss2d_gated_mlp_params& f = p->fwd;
     if (const int rc = check_common(f)) return rc;
-    if (!p->dy || !f.pre || !f.h) return SS2D_EINVAL_NULL;
+    if (!p->dy || !f.h) return SS2D_EINVAL_NULL;
     if (p->dy_row_stride < f.outputs) return SS2D_EINVAL_STRIDE;
     const size_t e = dtype_size(f.dtype);
-    if (!aligned_to(p->dy, e) || !aligned_to(f.h, 16) || !aligned_to(f.pre, 8)) return SS2D_EINVAL_ALIGN;
+    if (!aligned_to(p->dy, e) || !aligned_to(f.h, 16)) return SS2D_EINVAL_ALIGN;
     for (const void* q : {p->dx, p->dw1, p->dw2, p->db1, p->db2})
         if (!aligned_to(q, 2 * e)) return SS2D_EINVAL_ALIGN;
     if (!p->workspace || p->workspace_bytes < bwd_plan(f).total || !aligned_to(p->workspace, 16)) return SS2D_EWORKSPACE;

@@ -12,10 +12,15 @@ namespace host {
 using at::Tensor;
 using OptT = std::optional<Tensor>;
 
-// A status of the library, raised in Python as vmamba_b200._lib.Ss2dError(status, where).
-struct LibError {
+// A status of the library, raised in Python as vmamba_b200._lib.Ss2dError(status, where).  A std::exception: autograd's threads carry those alone to the
+// caller, and end the process for any other.
+struct LibError : std::exception {
     int status;
     const char* where;
+    std::string text;
+    LibError(int status, const char* where)
+        : status(status), where(where), text(std::string(where) + ": " + ss2d_strerror(status) + " (status " + std::to_string(status) + ")") {}
+    const char* what() const noexcept override { return text.c_str(); }
 };
 inline void check(int status, const char* where) {
     if (status != SS2D_OK) throw LibError{status, where};

@@ -17,23 +17,22 @@ static Tensor token_rows(const Tensor& x) {
     return t.stride(1) == 1 && (t.size(0) < 2 || t.stride(0) >= t.size(1)) ? t : t.contiguous();
 }
 
-struct Fed { Tensor y, h, pre; };
-static Fed mlp_fwd(const Tensor& x, const Tensor& w1, const Tensor& w2, const Tensor& b1, const Tensor& b2, int64_t act, bool train) {
+struct Fed { Tensor y, h; };
+static Fed mlp_fwd(const Tensor& x, const Tensor& w1, const Tensor& w2, const Tensor& b1, const Tensor& b2, int64_t act) {
     const CallGuard guard(x);
     ss2d_gated_mlp_params p = mlp_params(x, w1, w2, act);
     Fed r;
     r.y = at::empty({p.tokens, p.outputs}, x.options());
     r.h = at::empty({p.tokens, p.hidden}, x.options());
-    if (train) r.pre = at::empty({p.tokens, 2 * p.hidden}, x.options().dtype(at::kFloat));
-    p.b1 = ptr(b1); p.b2 = ptr(b2); p.h = r.h.data_ptr(); p.pre = ptr(r.pre); p.y = r.y.data_ptr();
+    p.b1 = ptr(b1); p.b2 = ptr(b2); p.h = r.h.data_ptr(); p.y = r.y.data_ptr();
     check(ss2d_gated_mlp_fwd(&p, stream_of(x)), "ss2d_gated_mlp_fwd");
     return r;
 }
 
 struct GatedMlpNode : public torch::autograd::Function<GatedMlpNode> {
     static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& w1, const Tensor& w2, const OptT& b1, const OptT& b2, int64_t act) {
-        const Fed r = mlp_fwd(x, w1, w2, opt(b1), opt(b2), act, true);
-        ctx->save_for_backward({x, w1, w2, r.h, r.pre});
+        const Fed r = mlp_fwd(x, w1, w2, opt(b1), opt(b2), act);
+        ctx->save_for_backward({x, w1, w2, r.h, opt(b1)});
         ctx->saved_data["act"] = act;
         // by argument: the edges that the engine asks for are numbered without the tensors that are not there
         int64_t wanted = 0, i = 0;
@@ -48,7 +47,7 @@ struct GatedMlpNode : public torch::autograd::Function<GatedMlpNode> {
         const Tensor dy = token_rows(grads[0]);
         ss2d_gated_mlp_bwd_params p = {};
         p.fwd = mlp_params(x, w1, w2, ctx->saved_data["act"].toInt());
-        p.fwd.h = s[3].data_ptr(); p.fwd.pre = s[4].data_ptr();
+        p.fwd.h = s[3].data_ptr(); p.fwd.b1 = ptr(s[4]);
         p.dy = dy.data_ptr();
         p.dy_row_stride = dy.size(0) == 1 ? dy.size(1) : dy.stride(0);
         Tensor d[5];
@@ -95,7 +94,7 @@ static Tensor gated_mlp_fn(const Tensor& x, const Tensor& w1, const Tensor& w2, 
     if (at::GradMode::is_enabled())
         for (const Tensor* t : {&x, &w1, &w2, &b1, &b2}) grad = grad || (t->defined() && t->requires_grad());
     if (grad) return GatedMlpNode::apply(rows, v1, v2, c1, c2, act).reshape(shape);
-    return mlp_fwd(rows, v1, v2, opt(c1), opt(c2), act, false).y.view(shape);
+    return mlp_fwd(rows, v1, v2, opt(c1), opt(c2), act).y.view(shape);
 }
 
 void bind_gated_mlp(pybind11::module_& m) {

@@ -1,0 +1,370 @@
+// Products of the gated feed-forward block on the 5th-generation tensor cores, 16-bit types: C (M x N) = A (M x K) . B (N x K)^T with the block's
+// epilogues on the accumulators.
+//
+// One persistent CTA per SM walks tiles of 128 rows.  Warp 0 brings 64 contraction elements of both operands at a time by TMA into a ring of stages, warp 1
+// issues the MMAs, two groups of four warps take the accumulators of alternate tiles (TMEM holds two tiles) and write results through shared memory by TMA,
+// 32 rows of 128 bytes a warp: with stores from registers, a row a lane, the load/store unit takes as long as the tile's MMAs.
+// An operand is read as it lies in memory: rows of the contraction index ("MN-major") or rows of M / N ("K-major"), so that no weight and no map is
+// transposed for any of the backward products.  Edges: TMA reads zeros and drops what it would write outside.
+//
+// Value and gate of a column come as two blocks of rows of the same operand, side by side in TMEM (EPI_GATE).  EPI_GRAD goes through two
+// contractions for a tile, x . w1 for value and gate and dy . w2 for the gradient of the hidden map, and forms the gradients of value and gate from the
+// three: they are computed again instead of kept, 4 more operations per weight and token in place of 16 bytes written and read per hidden element.
+//
+// Every wait is bounded; one that runs out raises the device's error flag (tc05.cuh), all roles leave and the TMEM is freed.
+#pragma once
+#include "gated_epilogue.cuh"
+#include "tc05.cuh"
+
+namespace ss2d {
+namespace ptc {
+
+using namespace tc05;
+
+constexpr int kRows = 128, kDepth = 64;                 // tile rows; contraction elements of a stage
+constexpr int kFirstEpi = 4, kEpiWarps = 8, kThreads = 32 * (kFirstEpi + kEpiWarps);
+
+struct Args {
+    int m_tiles, n_tiles, splits;
+    int blocks, per_split;          // stages of the first contraction; of a split
+    int blocks2;                    // EPI_GRAD: of the second one
+    int M, N, second;               // second: rows of B between value and gate
+    const void* bias;
+    int* error_flag;
+};
+
+// kCols: TMEM columns of a tile.  EPI_GATE: half value, half gate; EPI_GRAD: a third each of value, gate and hidden gradient.
+template <int EPI, int kCols> struct Shape {
+    static constexpr int kOut = EPI == EPI_GATE ? kCols / 2 : EPI == EPI_GRAD ? kCols / 3 : kCols;       // columns of the result
+    static constexpr int kB = EPI == EPI_GRAD ? 2 * kOut : kCols;                                        // rows of B of the (first) contraction
+    static constexpr int kABytes = kRows * kDepth * 2, kStage = kABytes + kB * kDepth * 2;
+    static constexpr int kOuts = EPI == EPI_GRAD ? 2 : 1;                                                // blocks of 32 rows that a warp stores at once
+    static constexpr int kStaging = kEpiWarps * kOuts * 4096;
+    static constexpr int kRoom = 232448 - 1024 - 256 - kStaging, kStages = kRoom / kStage > 8 ? 8 : kRoom / kStage;
+    static constexpr int kTmem = kCols > 128 ? 512 : kCols > 64 ? 256 : 128;                             // two tiles; a power of two
+    static constexpr int kPitch = kTmem / 2;
+    static constexpr int kBars = kStages * kStage + kStaging;
+    static constexpr size_t kBytes = kBars + 256 + 1024;
+    static_assert(kCols <= kPitch && kOut % 64 == 0 && kStages >= 3);
+};
+
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void* src, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z) : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void store_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void store_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+template <typename T, bool kAMN, bool kBMN, int EPI, int ACT, int kCols>
+__global__ void __launch_bounds__(kThreads, 1)
+product_tc05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmA2,
+                    const __grid_constant__ CUtensorMap tmB2, const __grid_constant__ CUtensorMap tmO, const __grid_constant__ CUtensorMap tmO2, const Args a) {
+    follow_previous();
+    using S = Shape<EPI, kCols>;
+    constexpr int NS = S::kStages;
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    unsigned char* const sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint64_t* const bars = reinterpret_cast<uint64_t*>(sm + S::kBars);
+    uint64_t *const full = bars, *const empty = bars + NS, *const acc_full = bars + 2 * NS, *const acc_empty = acc_full + 2;
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+    volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < NS; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(acc_full + i, 1); mbar_init(acc_empty + i, 4); }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) { tmem_alloc(tmem_slot, S::kTmem); tmem_relinquish(); }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const int tiles = a.m_tiles * a.n_tiles * a.splits;
+    struct Tile { int m, n, split, k0, k1; };
+    auto tile_at = [&](int i) {
+        Tile t;
+        t.n = i % a.n_tiles;
+        t.m = i / a.n_tiles % a.m_tiles;
+        t.split = i / (a.n_tiles * a.m_tiles);
+        t.k0 = t.split * a.per_split;
+        t.k1 = min(a.blocks, t.k0 + a.per_split);
+        return t;
+    };
+
+    if (warp == 0) {
+        // ---------------------------------------------------------------- TMA producer
+        if (lane == 0) {
+            int s = 0, round = 0;
+            bool ok = true;
+            auto slot = [&](uint32_t bytes) -> unsigned char* {
+                if (round > 0 && !mbar_wait_prompt(empty + s, (round - 1) & 1, abort_flag)) { ok = false; return nullptr; }
+                mbar_expect_tx(full + s, bytes);
+                return sm + s * S::kStage;
+            };
+            auto next = [&] { if (++s == NS) { s = 0; ++round; } };
+            for (int i = blockIdx.x; ok && i < tiles; i += gridDim.x) {
+                const Tile t = tile_at(i);
+                const int m0 = t.m * kRows, n0 = t.n * S::kOut;
+                for (int k = t.k0; k < t.k1; ++k) {
+                    unsigned char* st = slot(S::kStage);
+                    if (!ok) break;
+                    const int k0 = k * kDepth;
+                    if constexpr (kAMN) {
+                        tma_load_2d(st, &tmA, m0, k0, full + s);
+                        tma_load_2d(st + 8192, &tmA, m0 + 64, k0, full + s);
+                    } else
+                        tma_load_2d(st, &tmA, k0, m0, full + s);
+                    unsigned char* b = st + S::kABytes;
+                    if constexpr (EPI == EPI_GATE || EPI == EPI_GRAD) {            // value rows, gate rows
+                        tma_load_2d(b, &tmB, k0, n0, full + s);
+                        tma_load_2d(b + S::kOut * 128, &tmB, k0, a.second + n0, full + s);
+                    } else if constexpr (kBMN) {
+#pragma unroll
+                        for (int j = 0; j < S::kB / 64; ++j) tma_load_2d(b + j * 8192, &tmB, n0 + 64 * j, k0, full + s);
+                    } else
+                        tma_load_2d(b, &tmB, k0, n0, full + s);
+                    next();
+                }
+                if constexpr (EPI == EPI_GRAD)
+                    for (int k = 0; ok && k < a.blocks2; ++k) {
+                        unsigned char* st = slot(S::kABytes + S::kOut * 128);
+                        if (!ok) break;
+                        tma_load_2d(st, &tmA2, k * kDepth, m0, full + s);
+#pragma unroll
+                        for (int j = 0; j < S::kOut / 64; ++j) tma_load_2d(st + S::kABytes + j * 8192, &tmB2, n0 + 64 * j, k * kDepth, full + s);
+                        next();
+                    }
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------------------------------------------------------- MMA issuer
+        if (lane == 0) {
+            constexpr bool kDual = EPI == EPI_GRAD;
+            constexpr uint32_t idesc = instr_desc(Fmt<T>::id, kAMN, kRows, S::kB) | ((kBMN && !kDual ? 1u : 0u) << 16);
+            constexpr uint32_t idesc2 = instr_desc(Fmt<T>::id, false, kRows, S::kOut) | (1u << 16);
+            const uint32_t base = smem_u32(sm);
+            const uint64_t da0 = kAMN ? smem_desc(base, 8192, 1024, kSw128) : smem_desc(base, 16, 1024, kSw128);
+            const uint64_t db0 = kBMN && !kDual ? smem_desc(base + S::kABytes, 8192, 1024, kSw128) : smem_desc(base + S::kABytes, 16, 1024, kSw128);
+            const uint64_t db2 = smem_desc(base + S::kABytes, 8192, 1024, kSw128);
+            constexpr uint64_t stepA = (kAMN ? 2048 : 32) >> 4, stepB = (kBMN && !kDual ? 2048 : 32) >> 4;
+            int s = 0, round = 0, it = 0;
+            bool ok = true;
+            for (int i = blockIdx.x; ok && i < tiles; i += gridDim.x, ++it) {
+                const Tile t = tile_at(i);
+                const int buf = it & 1;
+                if (it >= 2 && !mbar_wait_prompt(acc_empty + buf, ((it >> 1) - 1) & 1, abort_flag)) break;
+                tc_fence_after();
+                const uint32_t acc = tmem + buf * S::kPitch;
+                for (int k = t.k0; k < t.k1; ++k) {
+                    if (!mbar_wait_prompt(full + s, round & 1, abort_flag)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint64_t off = (uint64_t)((uint32_t)(s * S::kStage) >> 4);
+#pragma unroll
+                    for (int j = 0; j < kDepth / 16; ++j) tc_mma(acc, da0 + off + j * stepA, db0 + off + j * stepB, idesc, k > t.k0 || j > 0 ? 1u : 0u);
+                    tc_commit(empty + s);
+                    if (++s == NS) { s = 0; ++round; }
+                }
+                if constexpr (kDual)
+                    for (int k = 0; ok && k < a.blocks2; ++k) {
+                        if (!mbar_wait_prompt(full + s, round & 1, abort_flag)) { ok = false; break; }
+                        tc_fence_after();
+                        const uint64_t off = (uint64_t)((uint32_t)(s * S::kStage) >> 4);
+#pragma unroll
+                        for (int j = 0; j < kDepth / 16; ++j) tc_mma(acc + S::kB, da0 + off + j * stepA, db2 + off + j * (2048 >> 4), idesc2, k > 0 || j > 0 ? 1u : 0u);
+                        tc_commit(empty + s);
+                        if (++s == NS) { s = 0; ++round; }
+                    }
+                if (ok) tc_commit(acc_full + buf);
+            }
+        }
+    } else if (warp >= kFirstEpi) {
+        // ---------------------------------------------------------------- epilogue: group `grp` of four warps has every second tile
+        const int grp = (warp - kFirstEpi) >> 2, quarter = warp & 3;
+        const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + grp * S::kPitch;
+        unsigned char* const stage = sm + NS * S::kStage + (warp - kFirstEpi) * S::kOuts * 4096;
+        unsigned char* const my_row = stage + lane * 128;
+        const T* const bias = (const T*)a.bias;
+        auto put = [&](int unit, uint4 w, int block = 0) { *reinterpret_cast<uint4*>(my_row + block * 4096 + ((unit ^ (lane & 7)) << 4)) = w; };
+        auto ready = [&] { if (lane == 0) store_read(); __syncwarp(); };           // the rows of the store before have been read
+        auto send = [&](int x, int y, int z) {
+            fence_async_smem();
+            __syncwarp();
+            if (x < a.N && y < a.M && lane == 0) {
+                tma_store_3d(&tmO, stage, x, y, z);
+                if constexpr (S::kOuts == 2) tma_store_3d(&tmO2, stage + 4096, x, y, z);
+            }
+        };
+        auto bias8 = [&](int n, int limit, float (&b)[8]) {                         // n and limit are multiples of 8
+            if (bias && n < limit) Vec<T, 8>::load(bias + n, b);
+            else
+#pragma unroll
+                for (int i = 0; i < 8; ++i) b[i] = 0.f;
+        };
+        int it = 0;
+        for (int i = blockIdx.x; i < tiles; i += gridDim.x, ++it) {
+            if ((it & 1) != grp) continue;
+            const Tile t = tile_at(i);
+            if (!mbar_wait_prompt(acc_full + grp, (it >> 1) & 1, abort_flag)) break;
+            __syncwarp();
+            tc_fence_after();
+            const int m0 = t.m * kRows + quarter * 32, n0 = t.n * S::kOut;
+            if constexpr (EPI == EPI_PART) {
+#pragma unroll 1
+                for (int c = 0; c < S::kOut; c += 32) {
+                    ready();
+#pragma unroll
+                    for (int q = 0; q < 32; q += 16) {
+                        uint32_t r[16];
+                        tmem_ld16(lane_base + c + q, r);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) put(q / 4 + u, make_uint4(r[4 * u], r[4 * u + 1], r[4 * u + 2], r[4 * u + 3]));
+                    }
+                    send(n0 + c, m0, t.split);
+                }
+            } else {
+#pragma unroll 1
+                for (int c = 0; c < S::kOut; c += 64) {
+                    ready();
+#pragma unroll
+                    for (int q = 0; q < 64; q += 16) {
+                        uint32_t x[16];
+                        tmem_ld16(lane_base + c + q, x);
+                        if constexpr (EPI == EPI_GATE || EPI == EPI_GRAD) {
+                            uint32_t y[16], z[16];
+                            tmem_ld16(lane_base + S::kOut + c + q, y);
+                            if constexpr (EPI == EPI_GRAD) tmem_ld16(lane_base + 2 * S::kOut + c + q, z);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int h = 0; h < 16; h += 8) {
+                                float bv[8], bg[8];
+                                bias8(n0 + c + q + h, a.N, bv);
+                                bias8(a.second + n0 + c + q + h, a.second + a.N, bg);
+                                uint32_t w[4], w2[4];
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    const int e = h + 2 * j;
+                                    const float2 v = __fadd2_rn(make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), make_float2(bv[2 * j], bv[2 * j + 1]));
+                                    const float2 g = __fadd2_rn(make_float2(__uint_as_float(y[e]), __uint_as_float(y[e + 1])), make_float2(bg[2 * j], bg[2 * j + 1]));
+                                    if constexpr (EPI == EPI_GATE) {
+                                        const float2 o = __fmul2_rn(v, act_pair<T, ACT>(g));
+                                        w[j] = Half2Of<T>::pack(o.x, o.y);
+                                    } else {
+                                        const float2 dh = make_float2(__uint_as_float(z[e]), __uint_as_float(z[e + 1]));
+                                        float2 act, slope;
+                                        act_grad_pair<T, ACT>(g, act, slope);
+                                        const float2 dv = __fmul2_rn(dh, act), dg = __fmul2_rn(__fmul2_rn(dh, v), slope);
+                                        w[j] = Half2Of<T>::pack(dv.x, dv.y);
+                                        w2[j] = Half2Of<T>::pack(dg.x, dg.y);
+                                    }
+                                }
+                                put((q + h) / 8, make_uint4(w[0], w[1], w[2], w[3]));
+                                if constexpr (EPI == EPI_GRAD) put((q + h) / 8, make_uint4(w2[0], w2[1], w2[2], w2[3]), 1);
+                            }
+                        } else {
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int h = 0; h < 16; h += 8) {
+                                float b[8];
+                                bias8(n0 + c + q + h, a.N, b);
+                                uint32_t w[4];
+#pragma unroll
+                                for (int j = 0; j < 4; ++j)
+                                    w[j] = Half2Of<T>::pack(__uint_as_float(x[h + 2 * j]) + b[2 * j], __uint_as_float(x[h + 2 * j + 1]) + b[2 * j + 1]);
+                                put((q + h) / 8, make_uint4(w[0], w[1], w[2], w[3]));
+                            }
+                        }
+                    }
+                    send(n0 + c, m0, 0);
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acc_empty + grp);
+        }
+        if (lane == 0) store_done();
+    }
+    // ---------------------------------------------------------------- teardown
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem, S::kTmem); }
+    if (threadIdx.x == 0 && *abort_flag) atomicExch(a.error_flag, 1);
+}
+
+// ---- host --------------------------------------------------------------------------------------------------------------
+// (splits, rows, cols) of T or fp32, rows `pitch` elements apart; box: 32 rows of 128 bytes
+template <typename E> bool make_out_map(CUtensorMap* m, const void* base, long long splits, long long rows, long long cols, long long pitch) {
+    EncodeFn enc = encode_fn();
+    if (!enc) return false;
+    CUtensorMapDataType dt;
+    if constexpr (sizeof(E) == 4) dt = CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+    else dt = Fmt<E>::tm;
+    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)splits};
+    const cuuint64_t strides[2] = {(cuuint64_t)(pitch * (long long)sizeof(E)), (cuuint64_t)(rows * pitch * (long long)sizeof(E))};
+    const cuuint32_t box[3] = {128 / sizeof(E), 32, 1}, estr[3] = {1, 1, 1};
+    return enc(m, dt, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// An operand of (rows of M or N, contraction) elements: `mn_major`: stored (contraction, rows)
+struct Operand {
+    const void* p;
+    long long pitch;
+};
+struct Product {
+    Operand a, b, a2, b2;
+    long long M, N, K, K2;          // N: columns of the result
+    long long b_rows;               // rows of B in memory (EPI_GATE, EPI_GRAD: 2 N)
+    const void* bias;
+    void *out, *out2;
+    long long out_pitch;
+    int splits, per_split;          // EPI_PART
+};
+
+inline int sm_count() {
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+    return sms;
+}
+
+template <typename T, bool kAMN, bool kBMN, int EPI, int ACT, int kCols> int run_product(const Product& p, cudaStream_t st) {
+    using S = Shape<EPI, kCols>;
+    constexpr bool kDual = EPI == EPI_GATE || EPI == EPI_GRAD;
+    constexpr auto sw = CU_TENSOR_MAP_SWIZZLE_128B;
+    // (in front of the maps: a thread that has made no runtime call yet, one of autograd's for instance, has no context for the driver to encode in)
+    int* host_flag = error_flag_for_current_device();
+    if (!host_flag || *host_flag) return SS2D_ECUDA;                            // no flag, or an earlier launch on this device gave up on a wait
+    int* dev_flag = nullptr;
+    if (cudaHostGetDevicePointer((void**)&dev_flag, host_flag, 0) != cudaSuccess) return SS2D_ECUDA;
+    CUtensorMap ta, tb, ta2, tb2, to, to2;
+    bool ok = kAMN ? make_map_pitched(&ta, Fmt<T>::tm, p.a.p, p.K, p.M, p.a.pitch, kDepth, 64, sw)
+                   : make_map_pitched(&ta, Fmt<T>::tm, p.a.p, p.M, p.K, p.a.pitch, kRows, kDepth, sw);
+    ok = ok && (kBMN && !kDual ? make_map_pitched(&tb, Fmt<T>::tm, p.b.p, p.K, p.N, p.b.pitch, kDepth, 64, sw)
+                               : make_map_pitched(&tb, Fmt<T>::tm, p.b.p, p.b_rows, p.K, p.b.pitch, kDual ? S::kOut : S::kB, kDepth, sw));
+    ta2 = ta; tb2 = tb;
+    if constexpr (EPI == EPI_GRAD)
+        ok = ok && make_map_pitched(&ta2, Fmt<T>::tm, p.a2.p, p.M, p.K2, p.a2.pitch, kRows, kDepth, sw) &&
+             make_map_pitched(&tb2, Fmt<T>::tm, p.b2.p, p.K2, p.N, p.b2.pitch, kDepth, 64, sw);
+    if constexpr (EPI == EPI_PART) ok = ok && make_out_map<float>(&to, p.out, p.splits, p.M, p.N, p.out_pitch);
+    else ok = ok && make_out_map<T>(&to, p.out, 1, p.M, p.N, p.out_pitch);
+    to2 = to;
+    if constexpr (EPI == EPI_GRAD) ok = ok && make_out_map<T>(&to2, p.out2, 1, p.M, p.N, p.out_pitch);
+    if (!ok) return SS2D_ECUDA;
+    auto kern = product_tc05_kernel<T, kAMN, kBMN, EPI, ACT, kCols>;
+    if (const int rc = allow_dynamic_smem(kern, S::kBytes)) return rc;
+    Args a = {};
+    a.m_tiles = (int)((p.M + kRows - 1) / kRows); a.n_tiles = (int)((p.N + S::kOut - 1) / S::kOut);
+    a.splits = EPI == EPI_PART ? p.splits : 1;
+    a.blocks = (int)((p.K + kDepth - 1) / kDepth); a.per_split = EPI == EPI_PART ? p.per_split : a.blocks;
+    a.blocks2 = (int)((p.K2 + kDepth - 1) / kDepth);
+    a.M = (int)p.M; a.N = (int)p.N; a.second = (int)p.N; a.bias = p.bias; a.error_flag = dev_flag;
+    const int tiles = a.m_tiles * a.n_tiles * a.splits, sms = sm_count();
+    if (!sms) return SS2D_ECUDA;
+    launch(kern, tiles < sms ? tiles : sms, kThreads, S::kBytes, st, ta, tb, ta2, tb2, to, to2, a);
+    count_launch();
+    return check_launch();
+}
+
+}  // namespace ptc
+}  // namespace ss2d

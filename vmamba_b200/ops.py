@@ -510,8 +510,8 @@ def gated_mlp_fn(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, b1=None, b
 
     x: (..., channels), w1: (2 * hidden, channels), w2: (outputs, hidden), b1: (2 * hidden,) or None, b2: (outputs,) or None, all of one dtype (float32, float16,
     bfloat16); act: "gelu" (erf) or "silu".  Returns (..., outputs).  Both projections, the activation and the product are one kernel; sums are fp32, the
-    hidden map is rounded to the inputs' type.  Differentiable in all tensors; the backward pass keeps x, the hidden map, and v and g in float32.
-    Repeated calls give bit-identical results."""
+    hidden map is rounded to the inputs' type.  Differentiable in all tensors; the backward pass keeps x and the hidden map and
+    computes v and g again.  Repeated calls give bit-identical results."""
     if act not in ("gelu", "silu"):
         raise ValueError(f"unknown activation {act!r}: expected 'gelu' or 'silu'")
     return _host.gated_mlp_fn(x, w1, w2, b1, b2, _ACTS[act])
