@@ -504,8 +504,8 @@ int ss2d_planes_to_pixels(const ss2d_relayout_params *p, void *cuda_stream);
  * q, k: (batch, seqlen, n_groups, dk), v: (batch, seqlen, heads, dv), of `dtype`, last dimension contiguous, the others strided (elements,
  * >= 0: heads that share rows have a stride of 0); log_decay: (batch, seqlen, heads) fp32, strided.  -inf resets the state; values are meant
  * to be <= 0.  out: (batch, seqlen, heads, dv) of `dtype`, dense; initial_state, final_state: (batch, heads, dk, dv) fp32, dense, NULL where
- * there is none.  chunk_states: NULL, or fp32 (batch, heads, ceil(seqlen / 64), dk, dv), the state in front of every 64th token, which the backward
- * call needs.  dk and dv up to 128 (else SS2D_ENOTSUP).  A value that is not finite may reach every output of its 64 tokens, also those in front
+ * there is none.  chunk_states: NULL, or ss2d_linear_attention_states_bytes() bytes, 16-byte aligned: the state in front of every 64th token, in the
+ * layout that the backward call reads.  dk and dv up to 128 (else SS2D_ENOTSUP).  A value that is not finite may reach every output of its 64 tokens, also those in front
  * of it.  workspace: ss2d_linear_attention_workspace_bytes() bytes, 16-byte aligned (0: none).  dense tensors are aligned to two elements (fp32 ones to 8 bytes).
  * No atomics: repeated calls give bit-identical results.
  * -------------------------------------------------------------------------------- */
@@ -525,6 +525,7 @@ typedef struct ss2d_linear_attention_params {
 
 int ss2d_linear_attention_fwd(const ss2d_linear_attention_params *p, void *cuda_stream);
 int64_t ss2d_linear_attention_workspace_bytes(const ss2d_linear_attention_params *p);    /* < 0: invalid arguments */
+int64_t ss2d_linear_attention_states_bytes(const ss2d_linear_attention_params *p);       /* the same */
 
 /* Its backward call: `fwd` as in the forward call, with the chunk_states that it wrote (out, final_state and initial_state are not read); dout of
  * `dtype`, (batch, seqlen, heads, dv), strided; dfinal_state fp32, NULL: zero.  Results, dense: dq, dk (batch, seqlen, n_groups, dk), summed over the heads of

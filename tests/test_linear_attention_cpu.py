@@ -26,7 +26,7 @@ def test_refusals_of_the_c_interface():
     p, a = params()
     assert call(p, None) == -2                                   # no token
     p.seqlen = 100
-    assert size(p) == 0
+    assert size(p) == 0 and L.ss2d_linear_attention_states_bytes(p) == 2 * 4 * 2 * 16 * 8 * 4 and L.ss2d_linear_attention_states_bytes(None) < 0
     for field, bad, code in (("q", None, -1), ("out", None, -1), ("dtype", 5, -3), ("heads", 5, -2), ("batch", 0, -2), ("dk", 129, -6), ("dv", 200, -6),
                              ("dk", 0, -2), ("v_token_stride", -1, -5), ("k", a + 1, -4), ("log_decay", a + 2, -4), ("out", a + 2, -4),
                              ("final_state", a + 4, -4), ("seqlen", 1 << 31, -6), ("batch", 1 << 30, -6)):

@@ -190,6 +190,7 @@ EXPORTS = {
     "ss2d_linear_fwd": (ctypes.c_int, [ctypes.POINTER(LinearParams), _vp]),
     "ss2d_linear_attention_fwd": (ctypes.c_int, [ctypes.POINTER(LinearAttentionParams), _vp]),
     "ss2d_linear_attention_workspace_bytes": (_i64, [ctypes.POINTER(LinearAttentionParams)]),
+    "ss2d_linear_attention_states_bytes": (_i64, [ctypes.POINTER(LinearAttentionParams)]),
     "ss2d_linear_attention_bwd": (ctypes.c_int, [ctypes.POINTER(LinearAttentionBwdParams), _vp]),
     "ss2d_linear_attention_bwd_workspace_bytes": (_i64, [ctypes.POINTER(LinearAttentionBwdParams)]),
     "ss2d_linear_attention_step": (ctypes.c_int, [ctypes.POINTER(LinearAttentionStepParams), _vp]),

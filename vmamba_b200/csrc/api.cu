@@ -46,6 +46,7 @@ int bias_act(const ss2d_pointwise_params* p, cudaStream_t st);
 int dwconv3x3_act(const ss2d_pointwise_params* p, cudaStream_t st);
 int linear_attention_fwd(const ss2d_linear_attention_params* p, cudaStream_t st);
 long long linear_attention_workspace_bytes(const ss2d_linear_attention_params* p);
+long long linear_attention_states_bytes(const ss2d_linear_attention_params* p);
 int linear_attention_bwd(const ss2d_linear_attention_bwd_params* p, cudaStream_t st);
 long long linear_attention_bwd_workspace_bytes(const ss2d_linear_attention_bwd_params* p);
 int linear_attention_step(const ss2d_linear_attention_step_params* p, cudaStream_t st);
@@ -220,6 +221,7 @@ int ss2d_linear_attention_fwd(const ss2d_linear_attention_params* p, void* strea
     return ss2d::linear_attention_fwd(p, (cudaStream_t)stream);
 }
 int64_t ss2d_linear_attention_workspace_bytes(const ss2d_linear_attention_params* p) { return ss2d::linear_attention_workspace_bytes(p); }
+int64_t ss2d_linear_attention_states_bytes(const ss2d_linear_attention_params* p) { return ss2d::linear_attention_states_bytes(p); }
 int ss2d_linear_attention_bwd(const ss2d_linear_attention_bwd_params* p, void* stream) {
     ss2d::Range nvtx_("ss2d_linear_attention_bwd");
     if (p) SS2D_CHECK_PTRS(p->fwd.q, p->fwd.k, p->fwd.v, p->fwd.log_decay, p->fwd.chunk_states, p->dout, p->dfinal_state, p->dq, p->dk, p->dv,

@@ -37,7 +37,7 @@ static Attended attention_fwd(const Tensor& q, const Tensor& k, const Tensor& v,
     p.out = r.out.data_ptr();
     p.initial_state = ptr(s0);
     if (final_state) { r.state = at::empty({p.batch, p.heads, p.dk, p.dv}, f32o); p.final_state = r.state.data_ptr(); }
-    if (train) { r.chunk_states = at::empty({p.batch, p.heads, (p.seqlen + 63) / 64, p.dk, p.dv}, f32o); p.chunk_states = r.chunk_states.data_ptr(); }
+    if (train) { r.chunk_states = bytes(std::max<int64_t>(ss2d_linear_attention_states_bytes(&p), 16), v); p.chunk_states = r.chunk_states.data_ptr(); }
     const int64_t need = ss2d_linear_attention_workspace_bytes(&p);
     Tensor ws;
     if (need > 0) { ws = bytes(need, v); p.workspace = ws.data_ptr(); p.workspace_bytes = need; }

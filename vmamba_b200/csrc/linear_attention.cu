@@ -30,7 +30,6 @@ namespace {
 using namespace mt;
 
 constexpr int kChunk = 64;
-constexpr int kSlice = 64;          // columns of v of a walking CTA
 constexpr int kSlab = 32;           // rows of the states that the gradient kernel holds at a time
 constexpr float kFloor = -200.f;    // 2^-200 is 0 in fp32
 
@@ -88,6 +87,9 @@ __device__ __forceinline__ void load_decays(float& g0, float& g1, const float* g
     g1 = t + 1 < L ? g[(t + 1) * stride] : 0.f;
 }
 
+// A state that the gradient kernel reads: rows of `state_row(dv)` elements, 4 bytes each: beside bf16 two planes of pieces, else fp32.  What is behind dv is zero.
+__host__ __device__ constexpr int state_row(int dv) { return (dv + 7) / 8 * 8; }
+
 // ---- walking a sequence ------------------------------------------------------------------------------------------------
 struct WalkArgs {
     Rows q, k, v;                   // kOut: q, k, v.  Otherwise the rows of the state's update: k (forwards) or q (backwards), and v or do
@@ -96,15 +98,15 @@ struct WalkArgs {
     const float* start;             // (B, H, segments, dk, dv) or NULL: zeros
     float* end;                     // the same, or NULL
     float* end_decay;               // (B, H, segments): log2 of the decay over the segment, or NULL
-    float* states;                  // (B, H, chunks, dk, dv): the state in front of every chunk (walking backwards: behind it), or NULL
+    void* states;                   // (B, H, chunks) states (below): in front of every chunk (walking backwards: behind it), or NULL
     void* o;                        // (B, L, H, dv)
     int H, rep, L, dk, dv, chunks, per_segment, segments, pairs;
     float scale;
 };
 
-template <typename T, int DK> struct WalkSmem {
+template <typename T, int DK, int DVT> struct WalkSmem {
     using P = typename Plane<T>::type;
-    static constexpr int kLdK = DK + 8, kLdV = kSlice + 8;
+    static constexpr int kLdK = DK + 8, kLdV = DVT + 8;
     static constexpr int kQ = kChunk * kLdK, kV = kChunk * kLdV;       // elements
     static constexpr size_t stage(bool out) { return ((out ? 2 : 1) * kQ + kV) * sizeof(T); }
     static constexpr size_t plane(bool out) { return out ? DK * kLdV * sizeof(P) : 0; }
@@ -112,19 +114,19 @@ template <typename T, int DK> struct WalkSmem {
 };
 
 // Four warps.  Outputs: a warp has 16 tokens.  State: a warp has DK / 4 of its rows, in accumulators, DK / 64 blocks of 16 (one for two warps at DK = 32).
-template <typename T, int DK, bool kOut, bool kBack>
+template <typename T, int DK, int DVT, bool kOut, bool kBack>
 __global__ void __launch_bounds__(128) la_walk_kernel(const WalkArgs a) {
     follow_previous();
-    using M = WalkSmem<T, DK>;
+    using M = WalkSmem<T, DK, DVT>;
     using P = typename M::P;
     extern __shared__ __align__(16) unsigned char smem[];
-    constexpr int kBlocks = (DK + 63) / 64;
+    constexpr int kBlocks = (DK + 63) / 64, NT = DVT / 8;
     T* const stage0 = reinterpret_cast<T*>(smem);
     P* const plane = reinterpret_cast<P*>(smem + 2 * M::stage(kOut));
     Decays* const decays = reinterpret_cast<Decays*>(smem + 2 * M::stage(kOut) + M::plane(kOut));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, t = lane & 3;
-    const int slices = (a.dv + kSlice - 1) / kSlice, slice = blockIdx.x % slices, bh = blockIdx.x / slices, seg = blockIdx.y;
-    const int v0 = slice * kSlice, dv = min(kSlice, a.dv - v0), b = bh / a.H, h = bh % a.H;
+    const int slices = (a.dv + DVT - 1) / DVT, slice = blockIdx.x % slices, bh = blockIdx.x / slices, seg = blockIdx.y;
+    const int v0 = slice * DVT, dv = min(DVT, a.dv - v0), b = bh / a.H, h = bh % a.H;
     const int c0 = seg * a.per_segment, c1 = min(a.chunks, c0 + a.per_segment);
     const T* const q = (const T*)a.q.p + b * a.q.b + (h / a.rep) * a.q.h;
     const T* const k = (const T*)a.k.p + b * a.k.b + (h / a.rep) * a.k.h;
@@ -132,14 +134,14 @@ __global__ void __launch_bounds__(128) la_walk_kernel(const WalkArgs a) {
     const float* const g = a.g + b * a.g_b + h * a.g_h;
     const long long state_size = (long long)a.dk * a.dv;
 
-    float S[kBlocks][8][4];
+    float S[kBlocks][NT][4];
     const int m_first = warp * 16;                         // first row of the warp's block 0; the next one is 64 rows on
     const bool holds = DK >= 64 || warp < DK / 16;
     auto for_state = [&](auto&& f) {                       // f(row, column, first of two accumulators)
 #pragma unroll
         for (int m = 0; m < kBlocks; ++m)
 #pragma unroll
-            for (int n = 0; n < 8; ++n)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int r = 0; r < 2; ++r) f(m_first + 64 * m + gq + 8 * r, 8 * n + 2 * t, S[m][n] + 2 * r);
     };
@@ -167,11 +169,19 @@ __global__ void __launch_bounds__(128) la_walk_kernel(const WalkArgs a) {
                 }
             });
     };
+    auto write_planes = [&](long long which) {
+        const int ld = state_row(a.dv);
+        P* const to = (P*)((char*)a.states + which * a.dk * ld * 4) + v0;
+        if (holds)
+            for_state([&](int row, int col, float* s) {
+                if (row < a.dk && v0 + col < ld) put2<T, 2>(to + row * ld + col, a.dk * ld, s[0], s[1]);
+            });
+    };
     auto fetch = [&](int c, int buf) {
         T* s = stage0 + buf * ((kOut ? 2 : 1) * M::kQ + M::kV);
         const int first = c * kChunk, rows = min(kChunk, a.L - first);
         fetch_rows<T, kChunk, DK>(s, M::kLdK, k + (long long)first * a.k.l, a.k.l, rows, a.dk, a.k.vec, tid, 128);
-        fetch_rows<T, kChunk, kSlice>(s + M::kQ, M::kLdV, v + (long long)first * a.v.l, a.v.l, rows, dv, a.v.vec, tid, 128);
+        fetch_rows<T, kChunk, DVT>(s + M::kQ, M::kLdV, v + (long long)first * a.v.l, a.v.l, rows, dv, a.v.vec, tid, 128);
         if constexpr (kOut) fetch_rows<T, kChunk, DK>(s + M::kQ + M::kV, M::kLdK, q + (long long)first * a.q.l, a.q.l, rows, a.dk, a.q.vec, tid, 128);
         commit_copies();
     };
@@ -193,13 +203,13 @@ __global__ void __launch_bounds__(128) la_walk_kernel(const WalkArgs a) {
             fetch(chunk_at(i + 1), buf ^ 1);
             load_decays(g0, g1, g, a.g_l, chunk_at(i + 1) * kChunk, a.L, lane);
         }
-        if (a.states) write_state(a.states + ((long long)bh * a.chunks + c) * state_size);
+        if (a.states) write_planes((long long)bh * a.chunks + c);
         const T* sk = stage0 + buf * ((kOut ? 2 : 1) * M::kQ + M::kV);
         const T* sv = sk + M::kQ;
         if constexpr (kOut) {
             const T* sq = sv + M::kV;
             const int r0 = warp * 16;
-            float p[8][4] = {}, o[8][4] = {};
+            float p[8][4] = {}, o[NT][4] = {};
 #pragma unroll
             for (int k0 = 0; k0 < DK; k0 += 16) {
                 const OpA<T> qa = load_a<false>(sq, M::kLdK, r0, k0, lane);
@@ -212,12 +222,12 @@ __global__ void __launch_bounds__(128) la_walk_kernel(const WalkArgs a) {
                         mma_exact(p[j + 1], qa, b1);
                     }
 #pragma unroll
-                for (int j = 0; j < 8; j += 2) mma_plane2<T, 1, true>(o[j], o[j + 1], qa, plane, 0, M::kLdV, 8 * j, k0, lane);
+                for (int j = 0; j < NT; j += 2) mma_plane2<T, 1, true>(o[j], o[j + 1], qa, plane, 0, M::kLdV, 8 * j, k0, lane);
             }
             const Cum lo = d.at(r0 + gq), hi = d.at(r0 + gq + 8);
             const float el = d.e[r0 + gq], eh = d.e[r0 + gq + 8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < NT; ++j) {
                 o[j][0] *= el; o[j][1] *= el; o[j][2] *= eh; o[j][3] *= eh;
             }
 #pragma unroll
@@ -235,7 +245,7 @@ __global__ void __launch_bounds__(128) la_walk_kernel(const WalkArgs a) {
                         }
                     const Derived<T, 1> pd = derive<T, 1>(x);
 #pragma unroll
-                    for (int u = 0; u < 8; u += 2) {
+                    for (int u = 0; u < NT; u += 2) {
                         OpB<T> b0, b1;
                         load_b2<true>(b0, b1, sv, M::kLdV, 8 * u, 8 * j, lane);
                         mma_derived<T, 1>(o[u], pd, b0);
@@ -250,7 +260,7 @@ __global__ void __launch_bounds__(128) la_walk_kernel(const WalkArgs a) {
                 if (row < rows) {
                     T* to = out + (long long)row * a.H * a.dv;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
+                    for (int j = 0; j < NT; ++j) {
                         const int col = 8 * j + 2 * t;
                         const float y[2] = {a.scale * o[j][2 * r], a.scale * o[j][2 * r + 1]};
                         if (a.pairs && col + 1 < dv) Vec<T, 2>::store(to + col, y);
@@ -269,7 +279,7 @@ __global__ void __launch_bounds__(128) la_walk_kernel(const WalkArgs a) {
             // a chunk's products are summed on their own: tensor cores cut sums off towards zero, which a state of thousands of tokens would collect
 #pragma unroll
             for (int m = 0; m < kBlocks; ++m) {
-                float add[8][4] = {};
+                float add[NT][4] = {};
 #pragma unroll
                 for (int k0 = 0; k0 < kChunk; k0 += 16) {
                     const float* w = kBack ? d.e : d.w;
@@ -284,7 +294,7 @@ __global__ void __launch_bounds__(128) la_walk_kernel(const WalkArgs a) {
                     for (int s = 0; s < 8; ++s) x[s] *= ws[(s & 1) + 2 * (s >> 2)];
                     const Derived<T, 2> kd = derive<T, 2>(x);       // two pieces: the state is an fp32 result
 #pragma unroll
-                    for (int j = 0; j < 8; j += 2) {
+                    for (int j = 0; j < NT; j += 2) {
                         OpB<T> b0, b1;
                         load_b2<true>(b0, b1, sv, M::kLdV, 8 * j, k0, lane);
                         mma_derived<T, 2>(add[j], kd, b0);
@@ -292,7 +302,7 @@ __global__ void __launch_bounds__(128) la_walk_kernel(const WalkArgs a) {
                     }
                 }
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
+                for (int j = 0; j < NT; ++j)
 #pragma unroll
                     for (int s = 0; s < 4; ++s) S[m][j][s] = fmaf(keep, S[m][j][s], add[j][s]);
             }
@@ -319,11 +329,23 @@ __global__ void __launch_bounds__(256) la_join_kernel(const JoinArgs a) {
     const long long blocks = (a.size + 255) / 256, bh = blockIdx.x / blocks, e = blockIdx.x % blocks * 256 + threadIdx.x;
     if (e >= a.size) return;
     float s = a.first ? a.first[bh * a.size + e] : 0.f;
-    for (int i = 0; i < a.segments; ++i) {
-        const long long at = bh * a.segments + (a.back ? a.segments - 1 - i : i);
-        const float x = a.part[at * a.size + e];
-        a.part[at * a.size + e] = s;
-        s = fmaf(ex2_approx(a.decay[at]), s, x);
+    constexpr int kAhead = 8;               // what several segments have gathered, read side by side
+    for (int i0 = 0; i0 < a.segments; i0 += kAhead) {
+        float x[kAhead], d[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            if (i0 + i < a.segments) {
+                const long long at = bh * a.segments + (a.back ? a.segments - 1 - i0 - i : i0 + i);
+                x[i] = a.part[at * a.size + e];
+                d[i] = a.decay[at];
+            }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            if (i0 + i < a.segments) {
+                const long long at = bh * a.segments + (a.back ? a.segments - 1 - i0 - i : i0 + i);
+                a.part[at * a.size + e] = s;
+                s = fmaf(ex2_approx(d[i]), s, x[i]);
+            }
     }
     if (a.last) a.last[bh * a.size + e] = s;
 }
@@ -333,217 +355,233 @@ struct GradArgs {
     Rows q, k, v, dy;
     const float* g;
     long long g_b, g_l, g_h;
-    const float *states, *dstates;  // (B, H, chunks, dk, dv): in front of the chunk; gradient of the state behind it
+    const void *states, *dstates;   // (B, H, chunks) states: in front of the chunk; gradient of the state behind it
     void *dq, *dk_, *dv_;           // dense
     float* dg;                      // (B, L, H)
-    float *sum_q, *sum_k;           // (B, L, G, dk) where heads share their keys
     int G, rep, L, dk, dv, chunks, pairs_k, pairs_v;
     float scale;
 };
 
-template <typename T, int DK, int DV> struct GradSmem {
+template <typename T, int DK, int DV> struct GradShape {
     using P = typename Plane<T>::type;
-    static constexpr int kParts = 2, kPlanes = Plane<T>::kSplit ? kParts : 1;
-    static constexpr int kLdK = DK + 8, kLdV = DV + 8;
-    static constexpr int kK = kChunk * kLdK, kV = kChunk * kLdV, kPlane = kSlab * kLdV;
-    static constexpr size_t kRowBytes = (2 * kK + 2 * kV) * sizeof(T), kStateBytes = 2 * kPlanes * kPlane * sizeof(P);
-    static constexpr size_t bytes() { return kRowBytes + kStateBytes + sizeof(Decays) + (4 * kChunk + 8) * sizeof(float); }
+    static constexpr int kPlanes = Plane<T>::kSplit ? 2 : 1;
+    static constexpr int kGroups = DK == 128 || DV == 128 ? 3 : 2;      // groups of four warps: dq; dk and dv, apart where both would not stay in registers
+    static constexpr int kThreads = 128 * kGroups, kSlabs = DK / kSlab;
+    static constexpr int kLdK = DK + 8, kLdV = DV + 8, kLdP = kChunk + 8;
+    static constexpr int kK = kChunk * kLdK, kV = kChunk * kLdV, kPair = kChunk * kLdP, kPlane = kSlab * kLdV;
+    static constexpr size_t kRowBytes = (2 * kK + 2 * kV) * sizeof(T), kPairBytes = 2 * kPair * sizeof(P), kSlabBytes = 2 * kPlanes * kPlane * sizeof(P);
+    static constexpr size_t kSums = (3 + 4 + 2) * kChunk * sizeof(float) + 64;
+    static constexpr size_t kFixed = kRowBytes + kPairBytes + sizeof(Decays) + kSums;
+    static constexpr int kStages = kSlabs == 1 || kFixed + 2 * kSlabBytes > 232448 ? 1 : 2;
+    static constexpr size_t kBytes = kFixed + kStages * kSlabBytes;
+    static constexpr int kResident = 2 * (kBytes + 1024) <= 233472 && kGroups == 2 ? 2 : 1;
+    static_assert(kBytes <= 232448);
 };
 
-// Eight warps: four have 16 queries each, the other four 16 keys each and the transposed products.  The states pass in slabs of 32 rows.
+// Pairs first: the 16 x 16 blocks of the lower triangle go round the warps, each gives decayed q . k and do . v, their sums by row and column, and both as operands in
+// shared memory.  Then a group of warps has dq, 16 queries a warp, another dk and dv, 16 keys a warp; the states pass in slabs of 32 rows.  Heads that share
+// their keys follow one another with dq and dk in accumulators.
 template <typename T, int DK, int DV>
-__global__ void __launch_bounds__(256) la_grad_kernel(const GradArgs a) {
+__global__ void __launch_bounds__(GradShape<T, DK, DV>::kThreads, GradShape<T, DK, DV>::kResident) la_grad_kernel(const GradArgs a) {
     follow_previous();
-    using M = GradSmem<T, DK, DV>;
+    using M = GradShape<T, DK, DV>;
     using P = typename M::P;
-    constexpr int kLdK = M::kLdK, kLdV = M::kLdV, kParts = M::kParts;
+    constexpr int kLdK = M::kLdK, kLdV = M::kLdV, kLdP = M::kLdP, kThreads = M::kThreads, kGroups = M::kGroups;
     extern __shared__ __align__(16) unsigned char smem[];
     T *const sq = reinterpret_cast<T*>(smem), *const sk = sq + M::kK, *const sv = sk + M::kK, *const sy = sv + M::kV;
-    P *const s_in = reinterpret_cast<P*>(smem + M::kRowBytes), *const s_out = s_in + M::kPlanes * M::kPlane;
-    Decays& d = *reinterpret_cast<Decays*>(smem + M::kRowBytes + M::kStateBytes);
-    float *const row_sum = reinterpret_cast<float*>(&d + 1), *const col_sum = row_sum + kChunk, *const into = col_sum + kChunk,
-                *const from = into + kChunk, *const cross = from + kChunk;
+    P *const s_w = reinterpret_cast<P*>(smem + M::kRowBytes), *const s_a = s_w + M::kPair, *const slabs = s_a + M::kPair;
+    Decays& d = *reinterpret_cast<Decays*>(smem + M::kRowBytes + M::kPairBytes + M::kStages * M::kSlabBytes);
+    float *const row_sum = reinterpret_cast<float*>(&d + 1), *const col_sum = row_sum + 3 * kChunk, *const into = col_sum + 4 * kChunk, *const from = into + kChunk,
+                *const cross = from + kChunk;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, t = lane & 3;
-    const bool keys = warp >= 4;
-    const int w4 = warp & 3, r0 = 16 * w4;
+    const int group = warp >> 2, w4 = warp & 3, r0 = 16 * w4;
     const int c = blockIdx.x % a.chunks, bg = blockIdx.x / a.chunks, b = bg / a.G, grp = bg % a.G, H = a.G * a.rep;
     const int first = c * kChunk, rows = min(kChunk, a.L - first);
+    const int ld = state_row(a.dv), n_slabs = (a.dk + kSlab - 1) / kSlab;
     auto src = [&](const Rows& r, int head) { return (const T*)r.p + b * r.b + (long long)first * r.l + head * r.h; };
-    fetch_rows<T, kChunk, DK>(sq, kLdK, src(a.q, grp), a.q.l, rows, a.dk, a.q.vec, tid, 256);
-    fetch_rows<T, kChunk, DK>(sk, kLdK, src(a.k, grp), a.k.l, rows, a.dk, a.k.vec, tid, 256);
+    // what the group computes for its rows (queries for dq, keys for dk and dv); dq and dk of all heads, dv of one
+    const bool has_dq = group == 0, has_dk = group == 1, has_dv = group == kGroups - 1;
+    // dq or dk in blocks of 8 columns, and behind them dv; in their place where the groups of warps are three and none has both
+    constexpr int kDv = kGroups == 3 ? 0 : DK / 8;
+    float acc_all[(kGroups == 3 ? (DK > DV ? DK : DV) / 8 : DK / 8 + DV / 8)][4] = {};
+    fetch_rows<T, kChunk, DK>(sq, kLdK, src(a.q, grp), a.q.l, rows, a.dk, a.q.vec, tid, kThreads);
+    fetch_rows<T, kChunk, DK>(sk, kLdK, src(a.k, grp), a.k.l, rows, a.dk, a.k.vec, tid, kThreads);
     for (int hh = 0; hh < a.rep; ++hh) {
         const int h = grp * a.rep + hh;
         if (hh) __syncthreads();
-        fetch_rows<T, kChunk, DV>(sv, kLdV, src(a.v, h), a.v.l, rows, a.dv, a.v.vec, tid, 256);
-        fetch_rows<T, kChunk, DV>(sy, kLdV, src(a.dy, h), a.dy.l, rows, a.dv, a.dy.vec, tid, 256);
-        commit_copies();
+        fetch_rows<T, kChunk, DV>(sv, kLdV, src(a.v, h), a.v.l, rows, a.dv, a.v.vec, tid, kThreads);
+        fetch_rows<T, kChunk, DV>(sy, kLdV, src(a.dy, h), a.dy.l, rows, a.dv, a.dy.vec, tid, kThreads);
+        const long long at = ((long long)(b * H + h) * a.chunks + c) * a.dk * ld * 4;
+        auto fetch_slab = [&](int s) {
+            if (s < n_slabs) {
+                P* to = slabs + (s % M::kStages) * (2 * M::kPlanes * M::kPlane);
+#pragma unroll
+                for (int p = 0; p < 2 * M::kPlanes; ++p) {
+                    const P* g = (const P*)((const char*)(p < M::kPlanes ? a.states : a.dstates) + at) + (p % M::kPlanes) * a.dk * ld + s * kSlab * ld;
+                    fetch_rows<P, kSlab, DV>(to + p * M::kPlane, kLdV, g, ld, a.dk - s * kSlab, ld, true, tid, kThreads);
+                }
+            }
+            commit_copies();
+        };
+        fetch_slab(0);
+        if constexpr (M::kStages == 2) fetch_slab(1);
         if (warp == 0) {
             float g0, g1;
             load_decays(g0, g1, a.g + b * a.g_b + h * a.g_h, a.g_l, first, a.L, lane);
             fill_decays(d, g0, g1, lane);
         }
-        wait_copies();
+        wait_copies<M::kStages - 1>();
         __syncthreads();
-        // rows of the warp: queries (columns: keys) or keys (columns: queries)
-        float qk[8][4] = {}, yv[8][4] = {};
         {
-            const T *const A = keys ? sk : sq, *const B = keys ? sq : sk, *const Ay = keys ? sv : sy, *const By = keys ? sy : sv;
-            auto live = [&](int j) { return keys ? j >= 2 * w4 : j <= 2 * w4; };      // pairs of column blocks
-#pragma unroll
-            for (int k0 = 0; k0 < DK; k0 += 16) {
-                const OpA<T> x = load_a<false>(A, kLdK, r0, k0, lane);
-#pragma unroll
-                for (int j = 0; j < 8; j += 2)
-                    if (live(j)) {
-                        OpB<T> b0, b1;
-                        load_b2<false>(b0, b1, B, kLdK, 8 * j, k0, lane);
-                        mma_exact(qk[j], x, b0);
-                        mma_exact(qk[j + 1], x, b1);
-                    }
-            }
-#pragma unroll
-            for (int k0 = 0; k0 < DV; k0 += 16) {
-                const OpA<T> x = load_a<false>(Ay, kLdV, r0, k0, lane);
-#pragma unroll
-                for (int j = 0; j < 8; j += 2)
-                    if (live(j)) {
-                        OpB<T> b0, b1;
-                        load_b2<false>(b0, b1, By, kLdV, 8 * j, k0, lane);
-                        mma_exact(yv[j], x, b0);
-                        mma_exact(yv[j + 1], x, b1);
-                    }
-            }
-            // pairs: decays, and the sums of what crosses (the pair of a token with itself crosses nothing)
             float sum[2] = {0.f, 0.f};
             const Cum own[2] = {d.at(r0 + gq), d.at(r0 + gq + 8)};
+            for (int cb = group; cb <= w4; cb += kGroups) {
+                float qk[2][4] = {}, yv[2][4] = {};
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
+                for (int k0 = 0; k0 < DK; k0 += 16) {
+                    OpB<T> b0, b1;
+                    const OpA<T> x = load_a<false>(sq, kLdK, r0, k0, lane);
+                    load_b2<false>(b0, b1, sk, kLdK, 16 * cb, k0, lane);
+                    mma_exact(qk[0], x, b0);
+                    mma_exact(qk[1], x, b1);
+                }
 #pragma unroll
-                for (int r = 0; r < 2; ++r)
+                for (int k0 = 0; k0 < DV; k0 += 16) {
+                    OpB<T> b0, b1;
+                    const OpA<T> x = load_a<false>(sy, kLdV, r0, k0, lane);
+                    load_b2<false>(b0, b1, sv, kLdV, 16 * cb, k0, lane);
+                    mma_exact(yv[0], x, b0);
+                    mma_exact(yv[1], x, b1);
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    float col[2] = {0.f, 0.f};
+                    const int n = 16 * cb + 8 * u + 2 * t;
+                    const Cum to[2] = {d.at(n), d.at(n + 1)};
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const int m = r0 + gq + 8 * r;
+                        float x[2], y[2];
+#pragma unroll
+                        for (int s = 0; s < 2; ++s) {
+                            const float D = n + s <= m ? a.scale * exp_diff(own[r], to[s]) : 0.f;
+                            x[s] = D * qk[u][2 * r + s];
+                            y[s] = D * yv[u][2 * r + s];
+                            // the pair of a token with itself crosses nothing
+                            const float w = n + s < m ? x[s] * yv[u][2 * r + s] : 0.f;
+                            sum[r] += w;
+                            col[s] += w;
+                        }
+                        put2<T, 1>(s_w + m * kLdP + n, 0, x[0], x[1]);
+                        put2<T, 1>(s_a + m * kLdP + n, 0, y[0], y[1]);
+                    }
 #pragma unroll
                     for (int s = 0; s < 2; ++s) {
-                        const int row = r0 + gq + 8 * r, col = 8 * j + 2 * t + s;
-                        const bool in = keys ? col >= row : col <= row;
-                        const Cum at = d.at(col);
-                        const float D = in ? a.scale * (keys ? exp_diff(at, own[r]) : exp_diff(own[r], at)) : 0.f;
-                        float &x = qk[j][2 * r + s], &y = yv[j][2 * r + s];
-                        if (in && col != row) sum[r] = fmaf(D * x, y, sum[r]);
-                        x *= D;
-                        y *= D;
+#pragma unroll
+                        for (int off = 4; off < 32; off <<= 1) col[s] += __shfl_xor_sync(0xffffffffu, col[s], off);
+                        if (gq == 0) col_sum[w4 * kChunk + n + s] = col[s];
                     }
+                }
+            }
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
                 sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
-                if (t == 0) (keys ? col_sum : row_sum)[r0 + gq + 8 * r] = sum[r];
+                if (t == 0) row_sum[group * kChunk + r0 + gq + 8 * r] = sum[r];
             }
         }
-        const long long at = ((long long)(b * H + h) * a.chunks + c) * a.dk * a.dv;
-        const float wl = (keys ? d.w : d.e)[r0 + gq] * (keys ? 1.f : a.scale), wh = (keys ? d.w : d.e)[r0 + gq + 8] * (keys ? 1.f : a.scale);
-        float dv[DV / 8][4] = {};
+        __syncthreads();
+        const float wl = (has_dq ? a.scale * d.e[r0 + gq] : d.w[r0 + gq]), wh = (has_dq ? a.scale * d.e[r0 + gq + 8] : d.w[r0 + gq + 8]);
+        float (*const total)[4] = acc_all, (*const dv)[4] = acc_all + kDv;
+        if (has_dv) {
+#pragma unroll
+            for (int j = 0; j < DV / 8; ++j)
+#pragma unroll
+                for (int s = 0; s < 4; ++s) dv[j][s] = 0.f;
+        }
         float through[2] = {0.f, 0.f}, both = 0.f;
-        const T *const X = keys ? sv : sy, *const Own = keys ? sk : sq, *const Other = keys ? sq : sk;
-        for (int m0 = 0; m0 < a.dk; m0 += kSlab) {
-            __syncthreads();
-            for (int i = tid; i < kSlab * DV / 2; i += 256) {
-                const int m = i / (DV / 2), n = (i % (DV / 2)) * 2;
-                float x[2] = {0.f, 0.f}, y[2] = {0.f, 0.f};
-                if (m0 + m < a.dk && n < a.dv) {
-                    const long long p = at + (long long)(m0 + m) * a.dv + n;
-                    if (a.pairs_v) { Vec<float, 2>::load(a.states + p, x); Vec<float, 2>::load(a.dstates + p, y); }
-                    else {
-                        x[0] = a.states[p]; y[0] = a.dstates[p];
-                        if (n + 1 < a.dv) { x[1] = a.states[p + 1]; y[1] = a.dstates[p + 1]; }
+        const T *const X = has_dq ? sy : sv, *const Own = has_dq ? sq : sk, *const Other = has_dq ? sk : sq;
+#pragma unroll
+        for (int s = 0; s < M::kSlabs; ++s) {
+            if (s < n_slabs) {
+                const int m0 = s * kSlab;
+                if (s) {
+                    wait_copies<M::kStages - 1>();
+                    __syncthreads();
+                }
+                const P *const s_in = slabs + (s % M::kStages) * (2 * M::kPlanes * M::kPlane), *const s_out = s_in + M::kPlanes * M::kPlane;
+                for (int i = tid; i < kSlab * DV / 2; i += kThreads) {
+                    const int at = i / (DV / 2) * kLdV + i % (DV / 2) * 2;
+                    if constexpr (Plane<T>::kSplit) {
+                        auto two = [&](const P* p) {
+                            const float2 u = Half2Of<P>::unpack(*reinterpret_cast<const uint32_t*>(p)), v = Half2Of<P>::unpack(*reinterpret_cast<const uint32_t*>(p + M::kPlane));
+                            return make_float2(u.x + v.x, u.y + v.y);
+                        };
+                        const float2 x = two(s_in + at), y = two(s_out + at);
+                        both = fmaf(x.x, y.x, fmaf(x.y, y.y, both));
+                    } else
+                        both = fmaf(s_in[at], s_out[at], fmaf(s_in[at + 1], s_out[at + 1], both));
+                }
+                if (has_dq || has_dk) {
+                    const P* const S = has_dq ? s_in : s_out;
+                    float acc[4][4] = {};
+#pragma unroll
+                    for (int k0 = 0; k0 < DV; k0 += 16) {
+                        const OpA<T> x = load_a<false>(X, kLdV, r0, k0, lane);
+#pragma unroll
+                        for (int j = 0; j < 4; j += 2) mma_plane2<T, 2, false>(acc[j], acc[j + 1], x, S, M::kPlane, kLdV, 8 * j, k0, lane);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            const T* p = Own + (r0 + gq + 8 * r) * kLdK + m0 + 8 * j + 2 * t;
+                            through[r] = fmaf(to_f<T>(p[0]), acc[j][2 * r], fmaf(to_f<T>(p[1]), acc[j][2 * r + 1], through[r]));
+                            total[4 * s + j][2 * r] = fmaf(r ? wh : wl, acc[j][2 * r], total[4 * s + j][2 * r]);
+                            total[4 * s + j][2 * r + 1] = fmaf(r ? wh : wl, acc[j][2 * r + 1], total[4 * s + j][2 * r + 1]);
+                        }
+                    for (int kb = has_dq ? 0 : w4; kb <= (has_dq ? w4 : 3); ++kb) {
+                        const OpA<P> x = has_dq ? load_a<false>(s_a, kLdP, r0, 16 * kb, lane) : load_a<true>(s_a, kLdP, r0, 16 * kb, lane);
+#pragma unroll
+                        for (int u = 0; u < 4; u += 2) {
+                            OpB<T> b0, b1;
+                            load_b2<true>(b0, b1, Other, kLdK, m0 + 8 * u, 16 * kb, lane);
+                            mma_plane_a<T>(total[4 * s + u], x, b0);
+                            mma_plane_a<T>(total[4 * s + u + 1], x, b1);
+                        }
                     }
                 }
-                both = fmaf(x[0], y[0], fmaf(x[1], y[1], both));
-                put2<T, kParts>(s_in + m * kLdV + n, M::kPlane, x[0], x[1]);
-                put2<T, kParts>(s_out + m * kLdV + n, M::kPlane, y[0], y[1]);
-            }
-            __syncthreads();
-            const P* const S = keys ? s_out : s_in;
-            float acc[4][4] = {};
+                if (has_dv) {
 #pragma unroll
-            for (int k0 = 0; k0 < DV; k0 += 16) {
-                const OpA<T> x = load_a<false>(X, kLdV, r0, k0, lane);
+                    for (int k0 = 0; k0 < kSlab; k0 += 16) {
+                        const OpA<T> x = load_a<false>(sk, kLdK, r0, m0 + k0, lane);
 #pragma unroll
-                for (int j = 0; j < 4; j += 2) mma_plane2<T, kParts, false>(acc[j], acc[j + 1], x, S, M::kPlane, kLdV, 8 * j, k0, lane);
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const T* p = Own + (r0 + gq + 8 * r) * kLdK + m0 + 8 * j + 2 * t;
-                    through[r] = fmaf(to_f<T>(p[0]), acc[j][2 * r], fmaf(to_f<T>(p[1]), acc[j][2 * r + 1], through[r]));
-                    acc[j][2 * r] *= r ? wh : wl;
-                    acc[j][2 * r + 1] *= r ? wh : wl;
-                }
-#pragma unroll
-            for (int j = 0; j < 8; j += 2)
-                if (keys ? j >= 2 * w4 : j <= 2 * w4) {
-                    const float x[8] = {yv[j][0], yv[j][1], yv[j][2], yv[j][3], yv[j + 1][0], yv[j + 1][1], yv[j + 1][2], yv[j + 1][3]};
-                    const Derived<T, 1> xd = derive<T, 1>(x);
-#pragma unroll
-                    for (int u = 0; u < 4; u += 2) {
-                        OpB<T> b0, b1;
-                        load_b2<true>(b0, b1, Other, kLdK, m0 + 8 * u, 8 * j, lane);
-                        mma_derived<T, 1>(acc[u], xd, b0);
-                        mma_derived<T, 1>(acc[u + 1], xd, b1);
+                        for (int j = 0; j < DV / 8; j += 2) mma_plane2<T, 1, true>(dv[j], dv[j + 1], x, s_out, M::kPlane, kLdV, 8 * j, k0, lane);
                     }
                 }
-            if (keys) {
-#pragma unroll
-                for (int k0 = 0; k0 < kSlab; k0 += 16) {
-                    const OpA<T> x = load_a<false>(sk, kLdK, r0, m0 + k0, lane);
-#pragma unroll
-                    for (int j = 0; j < DV / 8; j += 2) mma_plane2<T, 1, true>(dv[j], dv[j + 1], x, s_out, M::kPlane, kLdV, 8 * j, k0, lane);
-                }
-            }
-            T* const to = (T*)(keys ? a.dk_ : a.dq);
-            float* const part = keys ? a.sum_k : a.sum_q;
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int row = r0 + gq + 8 * r;
-                if (row >= rows) continue;
-                const long long p = (((long long)b * a.L + first + row) * a.G + grp) * a.dk + m0;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int col = 8 * j + 2 * t;
-                    float y[2] = {acc[j][2 * r], acc[j][2 * r + 1]};
-                    if (a.pairs_k && m0 + col + 1 < a.dk) {
-                        if (hh) { float z[2]; Vec<float, 2>::load(part + p + col, z); y[0] += z[0]; y[1] += z[1]; }
-                        if (hh + 1 < a.rep) Vec<float, 2>::store(part + p + col, y);
-                        else Vec<T, 2>::store(to + p + col, y);
-                    } else {
-#pragma unroll
-                        for (int s = 0; s < 2; ++s)
-                            if (m0 + col + s < a.dk) {
-                                if (hh) y[s] += part[p + col + s];
-                                if (hh + 1 < a.rep) part[p + col + s] = y[s];
-                                else to[p + col + s] = from_f<T>(y[s]);
-                            }
-                    }
-                }
+                if (s + M::kStages < M::kSlabs) {
+                    __syncthreads();
+                    fetch_slab(s + M::kStages);
+                } else if constexpr (M::kStages == 2)
+                    commit_copies();                       // keeps the count of groups behind a slab
             }
         }
-        if (keys) {
+        if (has_dv) {
+            const float vl = d.w[r0 + gq], vh = d.w[r0 + gq + 8];
 #pragma unroll
             for (int j = 0; j < DV / 8; ++j) {
-                dv[j][0] *= wl; dv[j][1] *= wl; dv[j][2] *= wh; dv[j][3] *= wh;
+                dv[j][0] *= vl; dv[j][1] *= vl; dv[j][2] *= vh; dv[j][3] *= vh;
             }
+            for (int kb = w4; kb < 4; ++kb) {
+                const OpA<P> x = load_a<true>(s_w, kLdP, r0, 16 * kb, lane);
 #pragma unroll
-            for (int j = 0; j < 8; j += 2)
-                if (j >= 2 * w4) {
-                    const float x[8] = {qk[j][0], qk[j][1], qk[j][2], qk[j][3], qk[j + 1][0], qk[j + 1][1], qk[j + 1][2], qk[j + 1][3]};
-                    const Derived<T, 1> xd = derive<T, 1>(x);
-#pragma unroll
-                    for (int u = 0; u < DV / 8; u += 2) {
-                        OpB<T> b0, b1;
-                        load_b2<true>(b0, b1, sy, kLdV, 8 * u, 8 * j, lane);
-                        mma_derived<T, 1>(dv[u], xd, b0);
-                        mma_derived<T, 1>(dv[u + 1], xd, b1);
-                    }
+                for (int u = 0; u < DV / 8; u += 2) {
+                    OpB<T> b0, b1;
+                    load_b2<true>(b0, b1, sy, kLdV, 8 * u, 16 * kb, lane);
+                    mma_plane_a<T>(dv[u], x, b0);
+                    mma_plane_a<T>(dv[u + 1], x, b1);
                 }
+            }
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 const int row = r0 + gq + 8 * r;
@@ -561,26 +599,72 @@ __global__ void __launch_bounds__(256) la_grad_kernel(const GradArgs a) {
                 }
             }
         }
+        if (has_dq || has_dk) {
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            through[r] *= r ? wh : wl;
-            through[r] += __shfl_xor_sync(0xffffffffu, through[r], 1);
-            through[r] += __shfl_xor_sync(0xffffffffu, through[r], 2);
-            if (t == 0) (keys ? from : into)[r0 + gq + 8 * r] = through[r];
+            for (int r = 0; r < 2; ++r) {
+                through[r] *= r ? wh : wl;
+                through[r] += __shfl_xor_sync(0xffffffffu, through[r], 1);
+                through[r] += __shfl_xor_sync(0xffffffffu, through[r], 2);
+                if (t == 0) (has_dq ? into : from)[r0 + gq + 8 * r] = through[r];
+            }
         }
 #pragma unroll
         for (int off = 16; off; off >>= 1) both += __shfl_xor_sync(0xffffffffu, both, off);
         if (lane == 0) cross[warp] = both;
         __syncthreads();
-        if (tid < rows) {
-            float x = 0.f;
-            for (int i = 0; i < 8; ++i) x += cross[i];
+        if (warp == 0) {
+            // tokens 2 lane and 2 lane + 1: suffix sums of what reaches them from in front, prefix sums of what leaves them
+            float x = 0.f, in[2], out[2];
+            for (int i = 0; i < 4 * kGroups; ++i) x += cross[i];
             x *= d.total;
-            for (int s = tid; s < kChunk; ++s) x += into[s] + (row_sum[s] - col_sum[s]);
-            for (int r = 0; r < tid; ++r) x += from[r];
-            // nothing crosses a reset; the pairs in front of it and behind it have cancelled to rounding only
-            const bool reset = d.n[tid] - (tid ? d.n[tid - 1] : 0.f) <= kFloor;
-            a.dg[((long long)b * a.L + first + tid) * H + h] = reset ? 0.f : x;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const int i = 2 * lane + s;
+                in[s] = into[i];
+                out[s] = from[i];
+                float pairs = 0.f;
+                for (int p = 0; p < kGroups; ++p) pairs += row_sum[p * kChunk + i];
+                for (int r = i / 16; r < 4; ++r) pairs -= col_sum[r * kChunk + i];
+                in[s] += pairs;
+            }
+            float suffix = in[0] + in[1], prefix = out[0] + out[1];
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const float u = __shfl_down_sync(0xffffffffu, suffix, off), v = __shfl_up_sync(0xffffffffu, prefix, off);
+                if (lane + off < 32) suffix += u;
+                if (lane >= off) prefix += v;
+            }
+            const float after = __shfl_down_sync(0xffffffffu, suffix, 1), before = __shfl_up_sync(0xffffffffu, prefix, 1);
+            const float s1 = in[1] + (lane < 31 ? after : 0.f), p0 = lane ? before : 0.f;
+            const float y[2] = {x + s1 + in[0] + p0, x + s1 + p0 + out[0]};
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const int i = 2 * lane + s;
+                // nothing crosses a reset; the pairs in front of it and behind it have cancelled to rounding only
+                const bool reset = d.n[i] - (i ? d.n[i - 1] : 0.f) <= kFloor;
+                if (i < rows) a.dg[((long long)b * a.L + first + i) * H + h] = reset ? 0.f : y[s];
+            }
+        }
+    }
+    if (has_dq || has_dk) {
+        T* const out = (T*)(has_dq ? a.dq : a.dk_);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int row = r0 + gq + 8 * r;
+            if (row >= rows) continue;
+            T* const to = out + (((long long)b * a.L + first + row) * a.G + grp) * a.dk;
+#pragma unroll
+            for (int s = 0; s < M::kSlabs; ++s)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int col = s * kSlab + 8 * j + 2 * t;
+                    const float y[2] = {acc_all[4 * s + j][2 * r], acc_all[4 * s + j][2 * r + 1]};
+                    if (a.pairs_k && col + 1 < a.dk) Vec<T, 2>::store(to + col, y);
+                    else {
+                        if (col < a.dk) to[col] = from_f<T>(y[0]);
+                        if (col + 1 < a.dk) to[col + 1] = from_f<T>(y[1]);
+                    }
+                }
         }
     }
 }
@@ -666,19 +750,24 @@ Rows rows_of(const void* p, int64_t b, int64_t l, int64_t h, int dtype) {
 }
 long long chunks_of(const ss2d_linear_attention_params& p) { return (p.seqlen + kChunk - 1) / kChunk; }
 
+// columns of v of a walking CTA: fp32 operands in pieces beside 128 rows of 64 columns of state would not stay in registers
+int slice_of(const ss2d_linear_attention_params& p) { return p.dv <= 32 || (p.dtype == SS2D_F32 && p.dk > 64) ? 32 : 64; }
+
 // Segments of a sequence: where sequences, heads and slices leave SMs without a CTA, sequences are cut, and each segment's own state is gathered by a
-// walk of its own first.
+// walk of its own first.  As many as are resident at once (two CTAs an SM with 128 rows of state, three with fewer): one more round of few CTAs would take as
+// long as all others.
 int segments_of(const ss2d_linear_attention_params& p) {
-    const long long ctas = p.batch * p.heads * ((p.dv + kSlice - 1) / kSlice), chunks = chunks_of(p);
-    const long long want = (2 * 148 + ctas - 1) / ctas;
-    if (want < 3 || chunks < 8) return 1;
-    const long long seg = want < chunks / 2 ? want : chunks / 2, per = (chunks + seg - 1) / seg;
+    const long long ctas = p.batch * p.heads * ((p.dv + slice_of(p) - 1) / slice_of(p)), chunks = chunks_of(p);
+    const long long room = 148 * (p.dk > 64 ? 2 : 3) / ctas;
+    if (room < 2 || chunks < 8) return 1;
+    const long long seg = room < chunks / 2 ? room : chunks / 2, per = (chunks + seg - 1) / seg;
     return (int)((chunks + per - 1) / per);
 }
 long long segment_bytes(const ss2d_linear_attention_params& p) {
     const long long seg = segments_of(p);
     return seg == 1 ? 0 : 4 * p.batch * p.heads * seg * (p.dk * p.dv + 4);
 }
+long long states_bytes(const ss2d_linear_attention_params& p) { return 4 * p.batch * p.heads * chunks_of(p) * p.dk * state_row((int)p.dv); }
 
 template <typename F> int for_type(int dtype, F&& f) {
     switch (dtype) {
@@ -693,23 +782,23 @@ template <typename F> int for_dk(int64_t dk, F&& f) {
     return f(std::integral_constant<int, 128>());
 }
 
-template <typename T, int DK, bool kOut, bool kBack> int launch_walk(const WalkArgs& a, long long bh, cudaStream_t st) {
-    auto kern = la_walk_kernel<T, DK, kOut, kBack>;
-    const size_t smem = WalkSmem<T, DK>::bytes(kOut);
+template <typename T, int DK, int DVT, bool kOut, bool kBack> int launch_walk(const WalkArgs& a, long long bh, cudaStream_t st) {
+    auto kern = la_walk_kernel<T, DK, DVT, kOut, kBack>;
+    const size_t smem = WalkSmem<T, DK, DVT>::bytes(kOut);
     if (const int rc = allow_dynamic_smem(kern, smem)) return rc;
-    launch(kern, dim3((unsigned)(bh * ((a.dv + kSlice - 1) / kSlice)), a.segments), 128, smem, st, a);
+    launch(kern, dim3((unsigned)(bh * ((a.dv + DVT - 1) / DVT)), a.segments), 128, smem, st, a);
     count_launch();
     return check_launch();
 }
 
 // One pass over the sequences: gathers the segments' states first where there are several.  `first` and `last`: states before and behind the whole walk
-template <typename T, int DK, bool kOut, bool kBack>
+template <typename T, int DK, int DVT, bool kOut, bool kBack>
 int walk(WalkArgs a, const float* first, float* last, void* workspace, long long bh, cudaStream_t st) {
     const int seg = a.segments;
     if (seg == 1) {
         a.per_segment = a.chunks;
         a.start = first; a.end = last;
-        return launch_walk<T, DK, kOut, kBack>(a, bh, st);
+        return launch_walk<T, DK, DVT, kOut, kBack>(a, bh, st);
     }
     float* part = (float*)workspace;
     float* decay = part + bh * seg * a.dk * a.dv;
@@ -717,14 +806,14 @@ int walk(WalkArgs a, const float* first, float* last, void* workspace, long long
     WalkArgs g = a;
     if constexpr (kOut) g.q = Rows{};
     g.states = nullptr; g.start = nullptr; g.end = part; g.end_decay = decay;
-    if (const int rc = launch_walk<T, DK, false, kBack>(g, bh, st)) return rc;
+    if (const int rc = launch_walk<T, DK, DVT, false, kBack>(g, bh, st)) return rc;
     JoinArgs j = {first, part, decay, last, (long long)a.dk * a.dv, seg, kBack};
     launch(la_join_kernel, (unsigned)(bh * ((j.size + 255) / 256)), 256, 0, st, j);
     count_launch();
     if (const int rc = check_launch()) return rc;
     if (!kOut && !a.states) return SS2D_OK;
     a.start = part; a.end = nullptr;
-    return launch_walk<T, DK, kOut, kBack>(a, bh, st);
+    return launch_walk<T, DK, DVT, kOut, kBack>(a, bh, st);
 }
 
 WalkArgs walk_args(const ss2d_linear_attention_params& p) {
@@ -739,6 +828,11 @@ WalkArgs walk_args(const ss2d_linear_attention_params& p) {
 
 }  // namespace
 
+long long linear_attention_states_bytes(const ss2d_linear_attention_params* p) {
+    if (!p || check_common(*p) != SS2D_OK) return -1;
+    return states_bytes(*p);
+}
+
 long long linear_attention_workspace_bytes(const ss2d_linear_attention_params* p) {
     if (!p || check_common(*p) != SS2D_OK) return -1;
     return segment_bytes(*p);
@@ -748,7 +842,7 @@ int linear_attention_fwd(const ss2d_linear_attention_params* p, cudaStream_t st)
     if (!p) return SS2D_EINVAL_NULL;
     if (const int rc = check_common(*p)) return rc;
     if (!p->out) return SS2D_EINVAL_NULL;
-    if (!aligned_to(p->out, 2 * dtype_size(p->dtype)) || !aligned_to(p->initial_state, 4) || !aligned_to(p->final_state, 8) || !aligned_to(p->chunk_states, 8))
+    if (!aligned_to(p->out, 2 * dtype_size(p->dtype)) || !aligned_to(p->initial_state, 4) || !aligned_to(p->final_state, 8) || !aligned_to(p->chunk_states, 16))
         return SS2D_EINVAL_ALIGN;
     const long long need = segment_bytes(*p), bh = p->batch * p->heads;
     if (need && (!p->workspace || p->workspace_bytes < need || !aligned_to(p->workspace, 16))) return SS2D_EWORKSPACE;
@@ -757,29 +851,34 @@ int linear_attention_fwd(const ss2d_linear_attention_params* p, cudaStream_t st)
     a.k = rows_of(p->k, p->k_batch_stride, p->k_token_stride, p->k_head_stride, p->dtype);
     a.v = rows_of(p->v, p->v_batch_stride, p->v_token_stride, p->v_head_stride, p->dtype);
     a.o = p->out;
-    a.states = (float*)p->chunk_states;
+    a.states = p->chunk_states;
     return for_type(p->dtype, [&](auto z) {
         return for_dk(p->dk, [&](auto n) {
-            return walk<decltype(z), decltype(n)::value, true, false>(a, (const float*)p->initial_state, (float*)p->final_state, p->workspace, bh, st);
+            using T = decltype(z);
+            constexpr int DK = decltype(n)::value;
+            const float* first = (const float*)p->initial_state;
+            float* last = (float*)p->final_state;
+            if constexpr (sizeof(T) == 2 || DK <= 64)
+                if (slice_of(*p) == 64) return walk<T, DK, 64, true, false>(a, first, last, p->workspace, bh, st);
+            return walk<T, DK, 32, true, false>(a, first, last, p->workspace, bh, st);
         });
     });
 }
 
 namespace {
-struct BwdPlan { long long segments, dstates, sums, total; };
+struct BwdPlan { long long segments, dstates, total; };
 BwdPlan bwd_plan(const ss2d_linear_attention_params& p) {
     BwdPlan b = {};
     b.segments = (segment_bytes(p) + 255) / 256 * 256;
-    b.dstates = (4 * p.batch * p.heads * chunks_of(p) * p.dk * p.dv + 255) / 256 * 256;
-    b.sums = p.heads == p.n_groups ? 0 : (4 * p.batch * p.seqlen * p.n_groups * p.dk + 255) / 256 * 256;
-    b.total = b.segments + b.dstates + 2 * b.sums;
+    b.dstates = states_bytes(p);
+    b.total = b.segments + b.dstates;
     return b;
 }
 template <typename T, int DK, int DV> int launch_grad(const GradArgs& a, long long groups, cudaStream_t st) {
     auto kern = la_grad_kernel<T, DK, DV>;
-    const size_t smem = GradSmem<T, DK, DV>::bytes();
+    constexpr size_t smem = GradShape<T, DK, DV>::kBytes;
     if (const int rc = allow_dynamic_smem(kern, smem)) return rc;
-    launch(kern, (unsigned)(groups * a.chunks), 256, smem, st, a);
+    launch(kern, (unsigned)(groups * a.chunks), GradShape<T, DK, DV>::kThreads, smem, st, a);
     count_launch();
     return check_launch();
 }
@@ -798,13 +897,13 @@ int linear_attention_bwd(const ss2d_linear_attention_bwd_params* p, cudaStream_t
     if (p->dout_batch_stride < 0 || p->dout_token_stride < 0 || p->dout_head_stride < 0) return SS2D_EINVAL_STRIDE;
     const size_t e = dtype_size(f.dtype);
     if (!aligned_to(p->dout, e) || !aligned_to(p->dq, 2 * e) || !aligned_to(p->dk, 2 * e) || !aligned_to(p->dv, 2 * e) || !aligned_to(p->dlog_decay, 4) ||
-        !aligned_to(f.chunk_states, 8) || !aligned_to(p->dfinal_state, 4) || !aligned_to(p->dinitial_state, 8))
+        !aligned_to(f.chunk_states, 16) || !aligned_to(p->dfinal_state, 4) || !aligned_to(p->dinitial_state, 8))
         return SS2D_EINVAL_ALIGN;
     const BwdPlan plan = bwd_plan(f);
     if (!p->workspace || p->workspace_bytes < plan.total || !aligned_to(p->workspace, 16)) return SS2D_EWORKSPACE;
     const long long bh = f.batch * f.heads;
     char* ws = (char*)p->workspace;
-    float* dstates = (float*)(ws + plan.segments);
+    void* dstates = ws + plan.segments;
     WalkArgs w = walk_args(f);
     w.k = rows_of(f.q, f.q_batch_stride, f.q_token_stride, f.q_head_stride, f.dtype);
     w.v = rows_of(p->dout, p->dout_batch_stride, p->dout_token_stride, p->dout_head_stride, f.dtype);
@@ -814,17 +913,26 @@ int linear_attention_bwd(const ss2d_linear_attention_bwd_params* p, cudaStream_t
     a.k = rows_of(f.k, f.k_batch_stride, f.k_token_stride, f.k_head_stride, f.dtype);
     a.v = rows_of(f.v, f.v_batch_stride, f.v_token_stride, f.v_head_stride, f.dtype);
     a.g = w.g; a.g_b = w.g_b; a.g_l = w.g_l; a.g_h = w.g_h;
-    a.states = (const float*)f.chunk_states; a.dstates = dstates;
+    a.states = f.chunk_states; a.dstates = dstates;
     a.dq = p->dq; a.dk_ = p->dk; a.dv_ = p->dv; a.dg = (float*)p->dlog_decay;
-    a.sum_q = (float*)(ws + plan.segments + plan.dstates); a.sum_k = (float*)(ws + plan.segments + plan.dstates + plan.sums);
     a.G = (int)f.n_groups; a.rep = w.rep; a.L = w.L; a.dk = w.dk; a.dv = w.dv; a.chunks = w.chunks; a.scale = f.scale;
     a.pairs_k = a.dk % 2 == 0; a.pairs_v = a.dv % 2 == 0;
     return for_type(f.dtype, [&](auto z) {
         using T = decltype(z);
         return for_dk(f.dk, [&](auto n) {
             constexpr int DK = decltype(n)::value;
-            if (const int rc = walk<T, DK, false, true>(w, (const float*)p->dfinal_state, (float*)p->dinitial_state, ws, bh, st)) return rc;
-            return f.dv <= 64 ? launch_grad<T, DK, 64>(a, f.batch * f.n_groups, st) : launch_grad<T, DK, 128>(a, f.batch * f.n_groups, st);
+            const float* first = (const float*)p->dfinal_state;
+            float* last = (float*)p->dinitial_state;
+            int rc = SS2D_OK;
+            bool wide = false;
+            if constexpr (sizeof(T) == 2 || DK <= 64) {
+                wide = slice_of(f) == 64;
+                if (wide) rc = walk<T, DK, 64, false, true>(w, first, last, ws, bh, st);
+            }
+            if (!wide) rc = walk<T, DK, 32, false, true>(w, first, last, ws, bh, st);
+            if (rc != SS2D_OK) return rc;
+            const long long groups = f.batch * f.n_groups;
+            return f.dv <= 32 ? launch_grad<T, DK, 32>(a, groups, st) : f.dv <= 64 ? launch_grad<T, DK, 64>(a, groups, st) : launch_grad<T, DK, 128>(a, groups, st);
         });
     });
 }

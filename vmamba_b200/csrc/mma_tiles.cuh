@@ -198,6 +198,15 @@ __device__ __forceinline__ void mma_plane2(float (&c0)[4], float (&c1)[4], const
         mma_values<kA, kB>(c1, v, b1.v);
     }
 }
+// derived A out of shared memory (one piece) times exact
+template <typename T> __device__ __forceinline__ void mma_plane_a(float (&c)[4], const OpA<typename Plane<T>::type>& a, const OpB<T>& b) {
+    if constexpr (Plane<T>::kSplit) MmaK16<T>::run(c, a.r, b.r);
+    else {
+        float w[4];
+        values(b, w);
+        mma_values<sizeof(T) == 4 ? 2 : 1, sizeof(T) == 4 ? 2 : 1>(c, a.v, w);
+    }
+}
 // two neighbouring values into the planes
 template <typename T, int kParts> __device__ __forceinline__ void put2(typename Plane<T>::type* s, int plane, float a, float b) {
     if constexpr (Plane<T>::kSplit) {
