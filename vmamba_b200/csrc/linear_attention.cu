@@ -53,9 +53,12 @@ __device__ __forceinline__ Cum cum_add(Cum a, Cum b) {
 }
 __device__ __forceinline__ float exp_diff(Cum a, Cum b) { return ex2_approx((a.n - b.n) + (a.f - b.f)); }
 
-struct Decays {
+struct alignas(16) Decays {
     float n[kChunk], f[kChunk];     // cumulative sums
     float e[kChunk], w[kChunk];     // 2^G_i, 2^(G_C - G_i)
+    // Pairs in different blocks of 16 tokens: 2^(G_i - G_j) = near[i] far[block of i][j], both at most 1 where decays are, G at the block's first token
+    // between them: one exponential a token in place of one a pair.
+    float near[kChunk], far[4][kChunk];
     float total_n, total_f, total;  // G_C, 2^G_C
     __device__ __forceinline__ Cum at(int i) const { return {n[i], f[i]}; }
 };
@@ -79,6 +82,12 @@ __device__ __forceinline__ void fill_decays(Decays& d, float g0, float g1, int l
     d.w[2 * lane] = exp_diff(all, first);
     d.w[2 * lane + 1] = exp_diff(all, s);
     if (lane == 0) { d.total_n = all.n; d.total_f = all.f; d.total = ex2_approx(all.n + all.f); }
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+        const Cum start = {__shfl_sync(0xffffffffu, first.n, 8 * b), __shfl_sync(0xffffffffu, first.f, 8 * b)};
+        if (lane / 8 == b) { d.near[2 * lane] = exp_diff(first, start); d.near[2 * lane + 1] = exp_diff(s, start); }
+        if (lane / 8 < b) { d.far[b][2 * lane] = exp_diff(start, first); d.far[b][2 * lane + 1] = exp_diff(start, s); }
+    }
 }
 // a token past the end decays nothing
 __device__ __forceinline__ void load_decays(float& g0, float& g1, const float* g, long long stride, int first, int L, int lane) {
@@ -189,20 +198,24 @@ __global__ void __launch_bounds__(128) la_walk_kernel(const WalkArgs a) {
     const int n = c1 - c0;
     auto chunk_at = [&](int i) { return kBack ? c1 - 1 - i : c0 + i; };
     float g0 = 0.f, g1 = 0.f;
+    auto next_decays = [&](int i) {                        // by warp 0, which has the fewest pairs: chunk i's, and the loads for the one behind it
+        if (warp == 0 && i < n) {
+            fill_decays(decays[i & 1], g0, g1, lane);
+            if (i + 1 < n) load_decays(g0, g1, g, a.g_l, chunk_at(i + 1) * kChunk, a.L, lane);
+        }
+    };
     fetch(chunk_at(0), 0);
-    load_decays(g0, g1, g, a.g_l, chunk_at(0) * kChunk, a.L, lane);
+    if (warp == 0) load_decays(g0, g1, g, a.g_l, chunk_at(0) * kChunk, a.L, lane);
+    next_decays(0);
     put_plane();
     Cum over = {0.f, 0.f};
     for (int i = 0; i < n; ++i) {
         const int c = chunk_at(i), buf = i & 1;
         Decays& d = decays[buf];
-        if (warp == 0) fill_decays(d, g0, g1, lane);
         wait_copies();
         __syncthreads();
-        if (i + 1 < n) {
-            fetch(chunk_at(i + 1), buf ^ 1);
-            load_decays(g0, g1, g, a.g_l, chunk_at(i + 1) * kChunk, a.L, lane);
-        }
+        if (i + 1 < n) fetch(chunk_at(i + 1), buf ^ 1);
+        next_decays(i + 1);
         if (a.states) write_planes((long long)bh * a.chunks + c);
         const T* sk = stage0 + buf * ((kOut ? 2 : 1) * M::kQ + M::kV);
         const T* sv = sk + M::kQ;
@@ -225,7 +238,7 @@ __global__ void __launch_bounds__(128) la_walk_kernel(const WalkArgs a) {
                 for (int j = 0; j < NT; j += 2) mma_plane2<T, 1, true>(o[j], o[j + 1], qa, plane, 0, M::kLdV, 8 * j, k0, lane);
             }
             const Cum lo = d.at(r0 + gq), hi = d.at(r0 + gq + 8);
-            const float el = d.e[r0 + gq], eh = d.e[r0 + gq + 8];
+            const float el = d.e[r0 + gq], eh = d.e[r0 + gq + 8], nl = d.near[r0 + gq], nh = d.near[r0 + gq + 8];
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
                 o[j][0] *= el; o[j][1] *= el; o[j][2] *= eh; o[j][3] *= eh;
@@ -234,15 +247,24 @@ __global__ void __launch_bounds__(128) la_walk_kernel(const WalkArgs a) {
             for (int j = 0; j < 8; j += 2)
                 if (j <= 2 * warp) {
                     float x[8];
+                    if (j < 2 * warp) {
 #pragma unroll
-                    for (int u = 0; u < 2; ++u)
-#pragma unroll
-                        for (int s = 0; s < 2; ++s) {
-                            const int col = 8 * (j + u) + 2 * t + s;
-                            const Cum at = d.at(col);
-                            x[4 * u + s] = col <= r0 + gq ? p[j + u][s] * exp_diff(lo, at) : 0.f;
-                            x[4 * u + 2 + s] = col <= r0 + gq + 8 ? p[j + u][2 + s] * exp_diff(hi, at) : 0.f;
+                        for (int u = 0; u < 2; ++u) {
+                            const float2 f = *reinterpret_cast<const float2*>(d.far[warp] + 8 * (j + u) + 2 * t);
+                            x[4 * u] = p[j + u][0] * (nl * f.x); x[4 * u + 1] = p[j + u][1] * (nl * f.y);
+                            x[4 * u + 2] = p[j + u][2] * (nh * f.x); x[4 * u + 3] = p[j + u][3] * (nh * f.y);
                         }
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int s = 0; s < 2; ++s) {
+                                const int col = 8 * (j + u) + 2 * t + s;
+                                const Cum at = d.at(col);
+                                x[4 * u + s] = col <= r0 + gq ? p[j + u][s] * exp_diff(lo, at) : 0.f;
+                                x[4 * u + 2 + s] = col <= r0 + gq + 8 ? p[j + u][2 + s] * exp_diff(hi, at) : 0.f;
+                            }
+                    }
                     const Derived<T, 1> pd = derive<T, 1>(x);
 #pragma unroll
                     for (int u = 0; u < NT; u += 2) {
@@ -435,6 +457,7 @@ __global__ void __launch_bounds__(GradShape<T, DK, DV>::kThreads, GradShape<T, D
         {
             float sum[2] = {0.f, 0.f};
             const Cum own[2] = {d.at(r0 + gq), d.at(r0 + gq + 8)};
+            const float near[2] = {a.scale * d.near[r0 + gq], a.scale * d.near[r0 + gq + 8]};
             for (int cb = group; cb <= w4; cb += kGroups) {
                 float qk[2][4] = {}, yv[2][4] = {};
 #pragma unroll
@@ -457,14 +480,14 @@ __global__ void __launch_bounds__(GradShape<T, DK, DV>::kThreads, GradShape<T, D
                 for (int u = 0; u < 2; ++u) {
                     float col[2] = {0.f, 0.f};
                     const int n = 16 * cb + 8 * u + 2 * t;
-                    const Cum to[2] = {d.at(n), d.at(n + 1)};
+                    const float2 far = *reinterpret_cast<const float2*>(d.far[w4] + n);
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
                         const int m = r0 + gq + 8 * r;
                         float x[2], y[2];
 #pragma unroll
                         for (int s = 0; s < 2; ++s) {
-                            const float D = n + s <= m ? a.scale * exp_diff(own[r], to[s]) : 0.f;
+                            const float D = cb < w4 ? near[r] * (s ? far.y : far.x) : n + s <= m ? a.scale * exp_diff(own[r], d.at(n + s)) : 0.f;
                             x[s] = D * qk[u][2 * r + s];
                             y[s] = D * yv[u][2 * r + s];
                             // the pair of a token with itself crosses nothing
@@ -753,12 +776,14 @@ long long chunks_of(const ss2d_linear_attention_params& p) { return (p.seqlen + 
 // columns of v of a walking CTA: fp32 operands in pieces beside 128 rows of 64 columns of state would not stay in registers
 int slice_of(const ss2d_linear_attention_params& p) { return p.dv <= 32 || (p.dtype == SS2D_F32 && p.dk > 64) ? 32 : 64; }
 
-// Segments of a sequence: where sequences, heads and slices leave SMs without a CTA, sequences are cut, and each segment's own state is gathered by a
-// walk of its own first.  As many as are resident at once (two CTAs an SM with 128 rows of state, three with fewer): one more round of few CTAs would take as
-// long as all others.
+// Segments of a sequence: where sequences, heads and slices leave room on the chip, sequences are cut, and each segment's own state is gathered by a
+// walk of its own first.  As many as are resident at once (two CTAs an SM with 128 rows of state, four with fewer): one more round of few CTAs would take as
+// long as all others.  us with 1 / 2 / 3 / 4 / 8 / 12 segments: 16 385 tokens of 16 heads of 128 x 128, forward 1134 / 873 / 587 / 448 / 288 / 349 (9 of them: 257);
+// 2 x 4 096 tokens, training 845 / 713 / 666 / 573 / 586 / 611 (4); 16 x 3 136 tokens of 12 heads of 64 x 32, training 550 / 543 / 488 / 513 / 502 / 505 (3);
+// 16 x 784 tokens of 24 heads, forward 73 / 115 / 113 / 111 (1).
 int segments_of(const ss2d_linear_attention_params& p) {
     const long long ctas = p.batch * p.heads * ((p.dv + slice_of(p) - 1) / slice_of(p)), chunks = chunks_of(p);
-    const long long room = 148 * (p.dk > 64 ? 2 : 3) / ctas;
+    const long long room = 148 * (p.dk > 64 ? 2 : 4) / ctas;
     if (room < 2 || chunks < 8) return 1;
     const long long seg = room < chunks / 2 ? room : chunks / 2, per = (chunks + seg - 1) / seg;
     return (int)((chunks + per - 1) / per);
