@@ -290,6 +290,21 @@ inline void launch(void (*kern)(P...), dim3 grid, dim3 block, size_t smem, cudaS
     cudaLaunchKernelEx(&c, kern, P(args)...);
 }
 
+// The same for clusters of two CTAs along x
+template <typename... P, typename... A>
+inline void launch_pairs(void (*kern)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A&&... args) {
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    cudaLaunchAttribute at[2] = {};
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 2; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t c = {};
+    c.gridDim = grid; c.blockDim = block; c.dynamicSmemBytes = smem; c.stream = st;
+    c.attrs = at; c.numAttrs = 1 + (cudaStreamIsCapturing(st, &capture) == cudaSuccess && capture == cudaStreamCaptureStatusNone);
+    cudaLaunchKernelEx(&c, kern, P(args)...);
+}
+
 // ---- host-side helpers ---------------------------------------------------------------------
 inline size_t dtype_size(int dt) { return dt == SS2D_F32 ? 4 : 2; }
 inline bool dtype_ok(int dt) { return dt == SS2D_F32 || dt == SS2D_F16 || dt == SS2D_BF16; }

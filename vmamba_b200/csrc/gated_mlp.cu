@@ -112,31 +112,67 @@ __global__ void __launch_bounds__(128) product_kernel(const ProductArgs p) {
 }
 
 // ---- sums ---------------------------------------------------------------------------------------------------------------
-// Column sums of a (rows, cols) matrix over spans of rows, fp32: part[span][col]
+// Column sums of two (rows, cols) matrices (the second may have none) over spans of rows, fp32: part[span][cols of both].  A warp has 32 kVec columns, eight warps
+// every eighth row.
 constexpr int kSpan = 256;
-template <typename T> __global__ void __launch_bounds__(256) column_sums_kernel(const T* a, long long ld, long long rows, int cols, float* part) {
+struct SumArgs {
+    const void* a[2];
+    long long ld[2], rows;
+    int cols[2], blocks;        // CTAs of the first matrix
+    float* part;
+    void* out[2];
+    int spans;
+};
+template <typename T, int kVec> __global__ void __launch_bounds__(256) column_sums_kernel(const SumArgs s) {
     follow_previous();
-    __shared__ float s[8][32];
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, c = blockIdx.x * 32 + tx;
-    const long long r0 = (long long)blockIdx.y * kSpan, r1 = r0 + kSpan < rows ? r0 + kSpan : rows;
-    float x = 0.f;
-    if (c < cols)
-        for (long long r = r0 + ty; r < r1; r += 8) x += to_f<T>(a[r * ld + c]);
-    s[ty][tx] = x;
+    __shared__ __align__(16) float sums[8][32 * kVec];
+    const int which = (int)blockIdx.x >= s.blocks, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int c0 = ((int)blockIdx.x - which * s.blocks) * 32 * kVec, c = c0 + lane * kVec, cols = s.cols[which];
+    const T* const a = (const T*)s.a[which];
+    const long long ld = s.ld[which], r0 = (long long)blockIdx.y * kSpan, r1 = r0 + kSpan < s.rows ? r0 + kSpan : s.rows;
+    float x[kVec] = {};
+    if (c < cols) {
+#pragma unroll 4
+        for (long long r = r0 + warp; r < r1; r += 8) {
+            float y[kVec];
+            Vec<T, kVec>::load(a + r * ld + c, y);
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) x[i] += y[i];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) sums[warp][lane * kVec + i] = x[i];
     __syncthreads();
-    if (ty == 0 && c < cols) {
-        for (int i = 1; i < 8; ++i) x += s[i][tx];
-        part[(long long)blockIdx.y * cols + c] = x;
+    for (int i = threadIdx.x; i < 32 * kVec && c0 + i < cols; i += 256) {
+        float y = 0.f;
+        for (int w = 0; w < 8; ++w) y += sums[w][i];
+        s.part[(long long)blockIdx.y * (s.cols[0] + s.cols[1]) + which * s.cols[0] + c0 + i] = y;
     }
 }
-// out[i] = sum over parts, in order
-template <typename T> __global__ void __launch_bounds__(256) add_parts_kernel(const float* part, T* out, long long n, int parts) {
+template <typename T> __global__ void __launch_bounds__(256) add_columns_kernel(const SumArgs s) {
     follow_previous();
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    const int i = blockIdx.x * 256 + threadIdx.x, n = s.cols[0] + s.cols[1];
     if (i >= n) return;
     float x = 0.f;
-    for (int p = 0; p < parts; ++p) x += part[p * n + i];
-    out[i] = from_f<T>(x);
+#pragma unroll 8
+    for (int p = 0; p < s.spans; ++p) x += s.part[(long long)p * n + i];
+    const int which = i >= s.cols[0];
+    ((T*)s.out[which])[i - which * s.cols[0]] = from_f<T>(x);
+}
+// out[i] = sum over parts, in order
+template <typename T, int kVec> __global__ void __launch_bounds__(256) add_parts_kernel(const float* part, T* out, long long n, int parts) {
+    follow_previous();
+    const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * kVec;
+    if (i >= n) return;
+    float x[kVec] = {};
+#pragma unroll 4
+    for (int p = 0; p < parts; ++p) {
+        float y[kVec];
+        Vec<float, kVec>::load(part + p * n + i, y);
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) x[j] += y[j];
+    }
+    Vec<T, kVec>::store(out + i, x);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
@@ -164,7 +200,8 @@ int splits_of(long long M, long long N, long long K) {
     return s < 1 ? 1 : s > 64 ? 64 : (int)s;
 }
 template <typename T> int add_parts(const float* part, void* out, long long n, int parts, cudaStream_t st) {
-    launch(add_parts_kernel<T>, (unsigned)((n + 255) / 256), 256, 0, st, part, (T*)out, n, parts);
+    if (n % 4 == 0 && aligned_to(out, 4 * sizeof(T))) launch(add_parts_kernel<T, 4>, (unsigned)((n / 4 + 255) / 256), 256, 0, st, part, (T*)out, n, parts);
+    else launch(add_parts_kernel<T, 1>, (unsigned)((n + 255) / 256), 256, 0, st, part, (T*)out, n, parts);
     count_launch();
     return check_launch();
 }
@@ -184,12 +221,21 @@ template <typename T> int weight_gradient(const void* a, long long lda, const vo
     if (const int rc = launch_product<T, true, true, EPI_PART, ACT_NONE>(p, splits, st)) return rc;
     return add_parts<T>(part, out, M * N, splits, st);
 }
-template <typename T> int column_sums(const void* a, long long ld, long long rows, int cols, void* out, float* part, cudaStream_t st) {
-    const long long spans = (rows + kSpan - 1) / kSpan;
-    launch(column_sums_kernel<T>, dim3((cols + 31) / 32, (unsigned)spans), 256, 0, st, (const T*)a, ld, rows, cols, part);
+template <typename T> int column_sums(SumArgs s, cudaStream_t st) {
+    s.spans = (int)((s.rows + kSpan - 1) / kSpan);
+    constexpr int kMost = 16 / (int)sizeof(T);
+    bool vec = true;
+    for (int i = 0; i < 2; ++i) vec = vec && (!s.cols[i] || (aligned_to(s.a[i], 16) && s.ld[i] % kMost == 0 && s.cols[i] % kMost == 0));
+    const int per = 32 * (vec ? kMost : 1);
+    s.blocks = (s.cols[0] + per - 1) / per;
+    const dim3 grid(s.blocks + (s.cols[1] + per - 1) / per, s.spans);
+    if (vec) launch(column_sums_kernel<T, kMost>, grid, 256, 0, st, s);
+    else launch(column_sums_kernel<T, 1>, grid, 256, 0, st, s);
     count_launch();
     if (const int rc = check_launch()) return rc;
-    return add_parts<T>(part, out, cols, (int)spans, st);
+    launch(add_columns_kernel<T>, (unsigned)((s.cols[0] + s.cols[1] + 255) / 256), 256, 0, st, s);
+    count_launch();
+    return check_launch();
 }
 
 int check_common(const ss2d_gated_mlp_params& p) {
@@ -226,43 +272,61 @@ bool tc_fits(const ss2d_gated_mlp_params& p) {
     return true;
 }
 
-// Time of a tensor-core product in cycles, for the choice among its tiles: rounds of tiles over the SMs, each as long as its MMAs (a step of 64 of the contraction
-// takes as many cycles as it has columns, and no fewer than 128 columns' worth) and a fixed part for filling the ring and the last tile's epilogue.
-double tc_cycles(long long tiles, long long steps, int columns) {
-    const long long rounds = (tiles + 147) / 148;
-    return (double)rounds * steps * (columns < 128 ? 128 : columns) + 1500.0;
+// Tiles of the tensor-core kernels: columns in TMEM, and whether two CTAs share one of 256 rows.
+enum Form { kNarrow, kWide, kPairNarrow, kPairWide, kForms };
+constexpr int kFormCols[kForms] = {128, 256, 128, 256}, kFormCtas[kForms] = {1, 1, 2, 2};
+// Time of a product in cycles, for the choice among them: rounds of tiles over the SMs, a step of 64 of the contraction as long as its operands take from L2 with all
+// SMs reading (40 bytes a cycle and SM; at least its columns), and a fixed part for filling the ring and the last tile's epilogue.
+double tc_cycles(int form, long long M, long long N, int out, long long steps, long long splits) {
+    const int ctas = kFormCtas[form], cols = kFormCols[form];
+    const long long tiles = ((M + ptc::kRows * ctas - 1) / (ptc::kRows * ctas)) * ((N + out - 1) / out) * splits, at_once = 148 / ctas;
+    const double step = (ptc::kRows + cols / ctas) * 128 / 40.0;
+    return (double)((tiles + at_once - 1) / at_once) * steps * (step < cols ? cols : step) + 1500.0;
 }
-long long tc_tiles(long long M, long long N, int out) { return ((M + ptc::kRows - 1) / ptc::kRows) * ((N + out - 1) / out); }
+int best_form(long long M, long long N, bool gate, long long K) {
+    const long long steps = (K + ptc::kDepth - 1) / ptc::kDepth;
+    int best = 0;
+    double least = 1e30;
+    for (int f = 0; f < kForms; ++f) {
+        const double t = tc_cycles(f, M, N, gate ? kFormCols[f] / 2 : kFormCols[f], steps, 1);
+        if (t < least) { least = t; best = f; }
+    }
+    return best;
+}
+template <typename T, bool kAMN, bool kBMN, int EPI, int ACT> int run_form(int form, const ptc::Product& p, cudaStream_t st) {
+    switch (form) {
+        case kNarrow: return ptc::run_product<T, kAMN, kBMN, EPI, ACT, 128, false>(p, st);
+        case kWide: return ptc::run_product<T, kAMN, kBMN, EPI, ACT, 256, false>(p, st);
+        case kPairNarrow: return ptc::run_product<T, kAMN, kBMN, EPI, ACT, 128, true>(p, st);
+        default: return ptc::run_product<T, kAMN, kBMN, EPI, ACT, 256, true>(p, st);
+    }
+}
 
 template <typename T, int ACT> int tc_forward(const ss2d_gated_mlp_params& p, cudaStream_t st) {
     ptc::Product a = {};
     a.a = {p.x, p.x_row_stride}; a.b = {p.w1, p.channels};
     a.M = p.tokens; a.N = p.hidden; a.K = p.channels; a.b_rows = 2 * p.hidden;
     a.bias = p.b1; a.out = p.h; a.out_pitch = p.hidden;
-    const long long steps = (p.channels + ptc::kDepth - 1) / ptc::kDepth;
-    const bool wide = tc_cycles(tc_tiles(a.M, a.N, 128), steps, 256) <= tc_cycles(tc_tiles(a.M, a.N, 64), steps, 128);
-    if (const int rc = wide ? ptc::run_product<T, false, false, EPI_GATE, ACT, 256>(a, st) : ptc::run_product<T, false, false, EPI_GATE, ACT, 128>(a, st)) return rc;
+    if (const int rc = run_form<T, false, false, EPI_GATE, ACT>(best_form(a.M, a.N, true, a.K), a, st)) return rc;
     ptc::Product b = {};
     b.a = {p.h, p.hidden}; b.b = {p.w2, p.hidden};
     b.M = p.tokens; b.N = p.outputs; b.K = p.hidden; b.b_rows = p.outputs;
     b.bias = p.b2; b.out = p.y; b.out_pitch = p.outputs;
-    const long long steps2 = (p.hidden + ptc::kDepth - 1) / ptc::kDepth;
-    const bool wide2 = tc_cycles(tc_tiles(b.M, b.N, 256), steps2, 256) <= tc_cycles(tc_tiles(b.M, b.N, 128), steps2, 128);
-    return wide2 ? ptc::run_product<T, false, false, EPI_OUT, ACT_NONE, 256>(b, st) : ptc::run_product<T, false, false, EPI_OUT, ACT_NONE, 128>(b, st);
+    return run_form<T, false, false, EPI_OUT, ACT_NONE>(best_form(b.M, b.N, false, b.K), b, st);
 }
 
 // Splits of a weight gradient's contraction over the tokens, and its tile: the fewest cycles, with the partial sums' way to memory and back (8 bytes an element
 // and split at about 3 300 bytes a cycle)
-struct WeightPlan { int splits, per_split; bool wide; };
+struct WeightPlan { int splits, per_split, form; };
 WeightPlan tc_weight_plan(long long M, long long N, long long K) {
     const long long steps = (K + ptc::kDepth - 1) / ptc::kDepth;
-    WeightPlan best = {1, (int)steps, false};
+    WeightPlan best = {1, (int)steps, 0};
     double least = 1e30;
-    for (int wide = 0; wide < 2; ++wide)
+    for (int f = 0; f < kForms; ++f)
         for (long long s = 1; s <= 64 && s <= steps; ++s) {
             const long long per = (steps + s - 1) / s, splits = (steps + per - 1) / per;
-            const double t = tc_cycles(tc_tiles(M, N, wide ? 256 : 128) * splits, per, wide ? 256 : 128) + (splits > 1 ? 3000.0 + 8.0 * splits * M * N / 3300.0 : 0.0);
-            if (t < least) { least = t; best = {(int)splits, (int)per, wide != 0}; }
+            const double t = tc_cycles(f, M, N, kFormCols[f], per, splits) + (splits > 1 ? 3000.0 + 8.0 * splits * M * N / 3300.0 : 0.0);
+            if (t < least) { least = t; best = {(int)splits, (int)per, f}; }
         }
     return best;
 }
@@ -273,10 +337,10 @@ template <typename T> int tc_weight_gradient(const void* a, long long lda, const
     p.M = M; p.N = N; p.K = K; p.b_rows = N; p.out_pitch = N;
     if (w.splits == 1) {
         p.out = out;
-        return w.wide ? ptc::run_product<T, true, true, EPI_OUT, ACT_NONE, 256>(p, st) : ptc::run_product<T, true, true, EPI_OUT, ACT_NONE, 128>(p, st);
+        return run_form<T, true, true, EPI_OUT, ACT_NONE>(w.form, p, st);
     }
     p.out = part; p.splits = w.splits; p.per_split = w.per_split;
-    if (const int rc = w.wide ? ptc::run_product<T, true, true, EPI_PART, ACT_NONE, 256>(p, st) : ptc::run_product<T, true, true, EPI_PART, ACT_NONE, 128>(p, st)) return rc;
+    if (const int rc = run_form<T, true, true, EPI_PART, ACT_NONE>(w.form, p, st)) return rc;
     return add_parts<T>(part, out, M * N, w.splits, st);
 }
 
@@ -285,7 +349,7 @@ BwdPlan bwd_plan(const ss2d_gated_mlp_params& p) {
     BwdPlan b;
     b.dz = up(2 * p.tokens * p.hidden * (long long)dtype_size(p.dtype));
     const long long spans = (p.tokens + kSpan - 1) / kSpan;
-    long long most = spans * (2 * p.hidden > p.outputs ? 2 * p.hidden : p.outputs);
+    long long most = spans * (2 * p.hidden + p.outputs);
     const long long M1 = 2 * p.hidden, N1 = p.channels, M2 = p.outputs, N2 = p.hidden;
     for (long long n : {splits_of(M1, N1, p.tokens) * M1 * N1, splits_of(M2, N2, p.tokens) * M2 * N2, tc_weight_plan(M1, N1, p.tokens).splits * M1 * N1,
                         tc_weight_plan(M2, N2, p.tokens).splits * M2 * N2})
@@ -315,7 +379,9 @@ template <typename T, int ACT> int backward(const ss2d_gated_mlp_bwd_params& p, 
                 a.a = {f.x, f.x_row_stride}; a.b = {f.w1, f.channels}; a.a2 = {p.dy, p.dy_row_stride}; a.b2 = {f.w2, H};
                 a.M = f.tokens; a.N = H; a.K = f.channels; a.K2 = f.outputs; a.b_rows = H2; a.bias = f.b1;
                 a.out = dz; a.out2 = (T*)dz + H; a.out_pitch = H2;
-                if (const int rc = ptc::run_product<T, false, true, EPI_GRAD, ACT, 192>(a, st)) return rc;
+                // pairs with tiles of 128 columns where there is a round of them, 64 columns otherwise
+                const bool pair = ((f.tokens + 255) / 256) * ((H + 127) / 128) >= 74;
+                if (const int rc = pair ? ptc::run_product<T, false, true, EPI_GRAD, ACT, 384, true>(a, st) : ptc::run_product<T, false, true, EPI_GRAD, ACT, 192, false>(a, st)) return rc;
             }
         if (!tc) {
             ProductArgs g = product_args<T>(f.x, f.x_row_stride, f.w1, f.channels, f.tokens, H, f.channels);
@@ -333,9 +399,7 @@ template <typename T, int ACT> int backward(const ss2d_gated_mlp_bwd_params& p, 
                 ptc::Product a = {};
                 a.a = {dz, H2}; a.b = {f.w1, f.channels};
                 a.M = f.tokens; a.N = f.channels; a.K = H2; a.b_rows = f.channels; a.out = p.dx; a.out_pitch = f.channels;
-                const long long steps = (H2 + ptc::kDepth - 1) / ptc::kDepth;
-                const bool wide = tc_cycles(tc_tiles(a.M, a.N, 256), steps, 256) <= tc_cycles(tc_tiles(a.M, a.N, 128), steps, 128);
-                if (const int rc = wide ? ptc::run_product<T, false, true, EPI_OUT, ACT_NONE, 256>(a, st) : ptc::run_product<T, false, true, EPI_OUT, ACT_NONE, 128>(a, st)) return rc;
+                if (const int rc = run_form<T, false, true, EPI_OUT, ACT_NONE>(best_form(a.M, a.N, false, a.K), a, st)) return rc;
             }
         if (!tc) {
             ProductArgs a = product_args<T>(dz, H2, f.w1, f.channels, f.tokens, f.channels, H2);
@@ -352,10 +416,17 @@ template <typename T, int ACT> int backward(const ss2d_gated_mlp_bwd_params& p, 
         if (const int rc = weight(dz, H2, f.x, f.x_row_stride, H2, f.channels, p.dw1)) return rc;
     if (p.dw2)
         if (const int rc = weight(p.dy, p.dy_row_stride, f.h, H, f.outputs, H, p.dw2)) return rc;
-    if (p.db1)
-        if (const int rc = column_sums<T>(dz, H2, f.tokens, (int)H2, p.db1, part, st)) return rc;
-    if (p.db2)
-        if (const int rc = column_sums<T>(p.dy, p.dy_row_stride, f.tokens, (int)f.outputs, p.db2, part, st)) return rc;
+    if (p.db1 || p.db2) {
+        SumArgs sums = {};
+        int n = 0;
+        auto add = [&](const void* m, long long ld, long long cols, void* out) {
+            sums.a[n] = m; sums.ld[n] = ld; sums.cols[n] = (int)cols; sums.out[n++] = out;
+        };
+        if (p.db1) add(dz, H2, H2, p.db1);
+        if (p.db2) add(p.dy, p.dy_row_stride, f.outputs, p.db2);
+        sums.rows = f.tokens; sums.part = part;
+        if (const int rc = column_sums<T>(sums, st)) return rc;
+    }
     return SS2D_OK;
 }
 

@@ -11,6 +11,10 @@
 // contractions for a tile, x . w1 for value and gate and dy . w2 for the gradient of the hidden map, and forms the gradients of value and gate from the
 // three: they are computed again instead of kept, 4 more operations per weight and token in place of 16 bytes written and read per hidden element.
 //
+// What bounds the large ones is the way of the operands from L2 to the SMs, about 40 bytes a cycle and SM with all of them reading: a tile of 128 x 128 spends
+// 32 KB on a step that takes the tensor core 128 cycles.  Pairs of CTAs (kPair) share a tile of 256 rows, each with its own half of A's rows and of
+// B's: 32 KB for 128 x 256 results, in place of 48.
+//
 // Every wait is bounded; one that runs out raises the device's error flag (tc05.cuh), all roles leave and the TMEM is freed.
 #pragma once
 #include "gated_epilogue.cuh"
@@ -34,34 +38,38 @@ struct Args {
 };
 
 // kCols: TMEM columns of a tile.  EPI_GATE: half value, half gate; EPI_GRAD: a third each of value, gate and hidden gradient.
-template <int EPI, int kCols> struct Shape {
+template <int EPI, int kCols, bool kPair> struct Shape {
     static constexpr int kOut = EPI == EPI_GATE ? kCols / 2 : EPI == EPI_GRAD ? kCols / 3 : kCols;       // columns of the result
     static constexpr int kB = EPI == EPI_GRAD ? 2 * kOut : kCols;                                        // rows of B of the (first) contraction
-    static constexpr int kABytes = kRows * kDepth * 2, kStage = kABytes + kB * kDepth * 2;
+    static constexpr int kShare = kPair ? 2 : 1;                                                         // CTAs among which they are divided
+    static constexpr int kABytes = kRows * kDepth * 2, kStage = kABytes + kB / kShare * kDepth * 2;
+    static constexpr int kBufs = kCols <= 256 ? 2 : 1;                                                   // tiles in TMEM
     static constexpr int kOuts = EPI == EPI_GRAD ? 2 : 1;                                                // blocks of 32 rows that a warp stores at once
-    static constexpr int kStaging = kEpiWarps * kOuts * 4096;
-    static constexpr int kRoom = 232448 - 1024 - 256 - kStaging, kStages = kRoom / kStage > 8 ? 8 : kRoom / kStage;
-    static constexpr int kTmem = kCols > 128 ? 512 : kCols > 64 ? 256 : 128;                             // two tiles; a power of two
-    static constexpr int kPitch = kTmem / 2;
-    static constexpr int kBars = kStages * kStage + kStaging;
-    static constexpr size_t kBytes = kBars + 256 + 1024;
-    static_assert(kCols <= kPitch && kOut % 64 == 0 && kStages >= 3);
+    static constexpr int kHalves = kOuts == 1 && kOut >= 128 ? 2 : 1;                                    // one is filled while the other is read
+    static constexpr int kWarpStaging = kOuts * kHalves * 4096, kStaging = kEpiWarps * kWarpStaging;
+    static constexpr int kBiasFloats = EPI == EPI_PART ? 0 : EPI == EPI_OUT ? kOut : kBufs == 2 ? 2 * kOut : kOut;      // of a group of epilogue warps
+    static constexpr int kBias = 2 * 2 * kBiasFloats * 4;
+    static constexpr int kRoom = 232448 - 1024 - 256 - kStaging - kBias, kStages = kRoom / kStage > 8 ? 8 : kRoom / kStage;
+    static constexpr int kTmem = kCols > 128 ? 512 : kCols > 64 ? 256 : 128;                             // a power of two
+    static constexpr int kPitch = kTmem / kBufs;
+    static constexpr int kBars = kStages * kStage + kStaging, kBiasAt = kBars + 256;
+    static constexpr size_t kBytes = kBiasAt + kBias + 1024;
+    static_assert(kCols <= kPitch && kOut % 64 == 0 && kStages >= 3 && (kB / kShare) % 64 == 0);
+    static_assert(kBufs == 2 || kOut == 128, "with one tile in TMEM the two groups of epilogue warps have 64 columns each");
 };
 
 __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void* src, int x, int y, int z) {
     asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z) : "memory");
-    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
-__device__ __forceinline__ void store_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void store_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
-template <typename T, bool kAMN, bool kBMN, int EPI, int ACT, int kCols>
+template <typename T, bool kAMN, bool kBMN, int EPI, int ACT, int kCols, bool kPair>
 __global__ void __launch_bounds__(kThreads, 1)
 product_tc05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmA2,
                     const __grid_constant__ CUtensorMap tmB2, const __grid_constant__ CUtensorMap tmO, const __grid_constant__ CUtensorMap tmO2, const Args a) {
     follow_previous();
-    using S = Shape<EPI, kCols>;
-    constexpr int NS = S::kStages;
+    using S = Shape<EPI, kCols, kPair>;
+    constexpr int NS = S::kStages, NB = S::kBufs;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* const sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint64_t* const bars = reinterpret_cast<uint64_t*>(sm + S::kBars);
@@ -69,23 +77,28 @@ product_tc05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
     volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = kPair ? (int)cluster_rank() : 0;
     if (threadIdx.x == 0) {
         for (int i = 0; i < NS; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(acc_full + i, 1); mbar_init(acc_empty + i, 4); }
+        for (int i = 0; i < 2; ++i) { mbar_init(acc_full + i, 1); mbar_init(acc_empty + i, (NB == 2 ? 4 : 8) * S::kShare); }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 1) { tmem_alloc(tmem_slot, S::kTmem); tmem_relinquish(); }
+    if (warp == 1) {
+        if constexpr (kPair) tmem_alloc_pair(tmem_slot, S::kTmem);
+        else { tmem_alloc(tmem_slot, S::kTmem); tmem_relinquish(); }
+    }
     tc_fence_before();
     __syncthreads();
+    if constexpr (kPair) cluster_sync();                 // the other CTA's barriers and TMEM are there
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const int tiles = a.m_tiles * a.n_tiles * a.splits;
-    struct Tile { int m, n, split, k0, k1; };
+    const int tiles = a.m_tiles * a.n_tiles * a.splits, walker = blockIdx.x / S::kShare, walkers = gridDim.x / S::kShare;
+    struct Tile { int m0, n0, split, k0, k1; };
     auto tile_at = [&](int i) {
         Tile t;
-        t.n = i % a.n_tiles;
-        t.m = i / a.n_tiles % a.m_tiles;
+        t.n0 = i % a.n_tiles * S::kOut;
+        t.m0 = (i / a.n_tiles % a.m_tiles * S::kShare + rank) * kRows;
         t.split = i / (a.n_tiles * a.m_tiles);
         t.k0 = t.split * a.per_split;
         t.k1 = min(a.blocks, t.k0 + a.per_split);
@@ -97,63 +110,83 @@ product_tc05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         if (lane == 0) {
             int s = 0, round = 0;
             bool ok = true;
+            // the first CTA's barrier counts the bytes of both
             auto slot = [&](uint32_t bytes) -> unsigned char* {
                 if (round > 0 && !mbar_wait_prompt(empty + s, (round - 1) & 1, abort_flag)) { ok = false; return nullptr; }
-                mbar_expect_tx(full + s, bytes);
+                if (rank == 0) mbar_expect_tx(full + s, bytes * S::kShare);
                 return sm + s * S::kStage;
             };
             auto next = [&] { if (++s == NS) { s = 0; ++round; } };
-            for (int i = blockIdx.x; ok && i < tiles; i += gridDim.x) {
+            auto load = [&](unsigned char* dst, const CUtensorMap* map, int x, int y) {
+                if constexpr (kPair) tma_load_2d_pair(dst, map, x, y, in_rank(full + s, 0));
+                else tma_load_2d(dst, map, x, y, full + s);
+            };
+            constexpr int kHalf = S::kB / S::kShare;     // rows of B in this CTA
+            for (int i = walker; ok && i < tiles; i += walkers) {
                 const Tile t = tile_at(i);
-                const int m0 = t.m * kRows, n0 = t.n * S::kOut;
                 for (int k = t.k0; k < t.k1; ++k) {
                     unsigned char* st = slot(S::kStage);
                     if (!ok) break;
                     const int k0 = k * kDepth;
                     if constexpr (kAMN) {
-                        tma_load_2d(st, &tmA, m0, k0, full + s);
-                        tma_load_2d(st + 8192, &tmA, m0 + 64, k0, full + s);
+                        load(st, &tmA, t.m0, k0);
+                        load(st + 8192, &tmA, t.m0 + 64, k0);
                     } else
-                        tma_load_2d(st, &tmA, k0, m0, full + s);
+                        load(st, &tmA, k0, t.m0);
                     unsigned char* b = st + S::kABytes;
-                    if constexpr (EPI == EPI_GATE || EPI == EPI_GRAD) {            // value rows, gate rows
-                        tma_load_2d(b, &tmB, k0, n0, full + s);
-                        tma_load_2d(b + S::kOut * 128, &tmB, k0, a.second + n0, full + s);
+                    if constexpr (EPI == EPI_GATE || EPI == EPI_GRAD) {            // value rows, gate rows; of a pair one has those and one these
+                        if (rank == 0) load(b, &tmB, k0, t.n0);
+                        if (!kPair || rank == 1) load(b + (kPair ? 0 : S::kOut * 128), &tmB, k0, a.second + t.n0);
                     } else if constexpr (kBMN) {
 #pragma unroll
-                        for (int j = 0; j < S::kB / 64; ++j) tma_load_2d(b + j * 8192, &tmB, n0 + 64 * j, k0, full + s);
+                        for (int j = 0; j < kHalf / 64; ++j) load(b + j * 8192, &tmB, t.n0 + rank * kHalf + 64 * j, k0);
                     } else
-                        tma_load_2d(b, &tmB, k0, n0, full + s);
+                        load(b, &tmB, k0, t.n0 + rank * kHalf);
                     next();
                 }
-                if constexpr (EPI == EPI_GRAD)
+                if constexpr (EPI == EPI_GRAD) {
+                    constexpr int kHalf2 = S::kOut / S::kShare;
                     for (int k = 0; ok && k < a.blocks2; ++k) {
-                        unsigned char* st = slot(S::kABytes + S::kOut * 128);
+                        unsigned char* st = slot(S::kABytes + kHalf2 * 128);
                         if (!ok) break;
-                        tma_load_2d(st, &tmA2, k * kDepth, m0, full + s);
+                        load(st, &tmA2, k * kDepth, t.m0);
 #pragma unroll
-                        for (int j = 0; j < S::kOut / 64; ++j) tma_load_2d(st + S::kABytes + j * 8192, &tmB2, n0 + 64 * j, k * kDepth, full + s);
+                        for (int j = 0; j < kHalf2 / 64; ++j) load(st + S::kABytes + j * 8192, &tmB2, t.n0 + rank * kHalf2 + 64 * j, k * kDepth);
                         next();
                     }
+                }
+            }
+            // what is in flight has been read, and the other CTA's last arrivals are here, before this one leaves
+            for (int j = 0; ok && j < NS; ++j) {
+                if (round > 0) ok = mbar_wait_prompt(empty + s, (round - 1) & 1, abort_flag);
+                next();
             }
         }
     } else if (warp == 1) {
         // ---------------------------------------------------------------- MMA issuer
-        if (lane == 0) {
+        if (lane == 0 && rank == 0) {
             constexpr bool kDual = EPI == EPI_GRAD;
-            constexpr uint32_t idesc = instr_desc(Fmt<T>::id, kAMN, kRows, S::kB) | ((kBMN && !kDual ? 1u : 0u) << 16);
-            constexpr uint32_t idesc2 = instr_desc(Fmt<T>::id, false, kRows, S::kOut) | (1u << 16);
+            constexpr uint32_t idesc = instr_desc(Fmt<T>::id, kAMN, kRows * S::kShare, S::kB) | ((kBMN && !kDual ? 1u : 0u) << 16);
+            constexpr uint32_t idesc2 = instr_desc(Fmt<T>::id, false, kRows * S::kShare, S::kOut) | (1u << 16);
             const uint32_t base = smem_u32(sm);
             const uint64_t da0 = kAMN ? smem_desc(base, 8192, 1024, kSw128) : smem_desc(base, 16, 1024, kSw128);
             const uint64_t db0 = kBMN && !kDual ? smem_desc(base + S::kABytes, 8192, 1024, kSw128) : smem_desc(base + S::kABytes, 16, 1024, kSw128);
             const uint64_t db2 = smem_desc(base + S::kABytes, 8192, 1024, kSw128);
             constexpr uint64_t stepA = (kAMN ? 2048 : 32) >> 4, stepB = (kBMN && !kDual ? 2048 : 32) >> 4;
+            auto mma = [&](uint32_t d, uint64_t x, uint64_t y, uint32_t id, uint32_t more) {
+                if constexpr (kPair) tc_mma_pair(d, x, y, id, more);
+                else tc_mma(d, x, y, id, more);
+            };
+            auto commit = [&](uint64_t* bar) {
+                if constexpr (kPair) tc_commit_pair(bar);
+                else tc_commit(bar);
+            };
             int s = 0, round = 0, it = 0;
             bool ok = true;
-            for (int i = blockIdx.x; ok && i < tiles; i += gridDim.x, ++it) {
+            for (int i = walker; ok && i < tiles; i += walkers, ++it) {
                 const Tile t = tile_at(i);
-                const int buf = it & 1;
-                if (it >= 2 && !mbar_wait_prompt(acc_empty + buf, ((it >> 1) - 1) & 1, abort_flag)) break;
+                const int buf = it % NB;
+                if (it >= NB && !mbar_wait_prompt(acc_empty + buf, (it / NB - 1) & 1, abort_flag)) break;
                 tc_fence_after();
                 const uint32_t acc = tmem + buf * S::kPitch;
                 for (int k = t.k0; k < t.k1; ++k) {
@@ -161,8 +194,8 @@ product_tc05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                     tc_fence_after();
                     const uint64_t off = (uint64_t)((uint32_t)(s * S::kStage) >> 4);
 #pragma unroll
-                    for (int j = 0; j < kDepth / 16; ++j) tc_mma(acc, da0 + off + j * stepA, db0 + off + j * stepB, idesc, k > t.k0 || j > 0 ? 1u : 0u);
-                    tc_commit(empty + s);
+                    for (int j = 0; j < kDepth / 16; ++j) mma(acc, da0 + off + j * stepA, db0 + off + j * stepB, idesc, k > t.k0 || j > 0 ? 1u : 0u);
+                    commit(empty + s);
                     if (++s == NS) { s = 0; ++round; }
                 }
                 if constexpr (kDual)
@@ -171,109 +204,121 @@ product_tc05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                         tc_fence_after();
                         const uint64_t off = (uint64_t)((uint32_t)(s * S::kStage) >> 4);
 #pragma unroll
-                        for (int j = 0; j < kDepth / 16; ++j) tc_mma(acc + S::kB, da0 + off + j * stepA, db2 + off + j * (2048 >> 4), idesc2, k > 0 || j > 0 ? 1u : 0u);
-                        tc_commit(empty + s);
+                        for (int j = 0; j < kDepth / 16; ++j) mma(acc + S::kB, da0 + off + j * stepA, db2 + off + j * (2048 >> 4), idesc2, k > 0 || j > 0 ? 1u : 0u);
+                        commit(empty + s);
                         if (++s == NS) { s = 0; ++round; }
                     }
-                if (ok) tc_commit(acc_full + buf);
+                if (ok) commit(acc_full + buf);
             }
         }
     } else if (warp >= kFirstEpi) {
-        // ---------------------------------------------------------------- epilogue: group `grp` of four warps has every second tile
+        // ---------------------------------------------------------------- epilogue: group `grp` of four warps has every second tile, or half the columns
         const int grp = (warp - kFirstEpi) >> 2, quarter = warp & 3;
-        const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + grp * S::kPitch;
-        unsigned char* const stage = sm + NS * S::kStage + (warp - kFirstEpi) * S::kOuts * 4096;
-        unsigned char* const my_row = stage + lane * 128;
-        const T* const bias = (const T*)a.bias;
-        auto put = [&](int unit, uint4 w, int block = 0) { *reinterpret_cast<uint4*>(my_row + block * 4096 + ((unit ^ (lane & 7)) << 4)) = w; };
-        auto ready = [&] { if (lane == 0) store_read(); __syncwarp(); };           // the rows of the store before have been read
+        const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + (NB == 2 ? grp * S::kPitch : 0);
+        unsigned char* const staging = sm + NS * S::kStage + (warp - kFirstEpi) * S::kWarpStaging;
+        int half = 0;                                                               // of the staging: where the next 32 rows go
+        auto put = [&](int unit, uint4 w, int block = 0) {
+            *reinterpret_cast<uint4*>(staging + (half + block) * 4096 + lane * 128 + ((unit ^ (lane & 7)) << 4)) = w;
+        };
+        auto ready = [&] {                                                          // what was stored from there has been read
+            if (lane == 0) {
+                if constexpr (S::kHalves == 2) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+                else asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            }
+            __syncwarp();
+        };
         auto send = [&](int x, int y, int z) {
             fence_async_smem();
             __syncwarp();
-            if (x < a.N && y < a.M && lane == 0) {
-                tma_store_3d(&tmO, stage, x, y, z);
-                if constexpr (S::kOuts == 2) tma_store_3d(&tmO2, stage + 4096, x, y, z);
+            if (lane == 0) {
+                if (x < a.N && y < a.M) {
+                    tma_store_3d(&tmO, staging + half * 4096, x, y, z);
+                    if constexpr (S::kOuts == 2) tma_store_3d(&tmO2, staging + 4096, x, y, z);
+                }
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             }
+            half ^= S::kHalves - 1;
         };
-        auto bias8 = [&](int n, int limit, float (&b)[8]) {                         // n and limit are multiples of 8
-            if (bias && n < limit) Vec<T, 8>::load(bias + n, b);
-            else
-#pragma unroll
-                for (int i = 0; i < 8; ++i) b[i] = 0.f;
+        // biases of the tile's columns, fp32: (EPI_GATE, EPI_GRAD) value and gate.  Two buffers, so that one barrier a tile is enough.
+        float* const bias_at = reinterpret_cast<float*>(sm + S::kBiasAt) + grp * 2 * S::kBiasFloats;
+        constexpr int kBiasCols = EPI == EPI_OUT ? S::kBiasFloats : S::kBiasFloats / 2;
+        auto fill_bias = [&](float* to, int n0) {
+            const T* const bias = (const T*)a.bias;
+            for (int i = threadIdx.x & 127; i < S::kBiasFloats; i += 128) {
+                const int gate = i >= kBiasCols, n = n0 + i - gate * kBiasCols;
+                to[i] = bias && n < a.N ? to_f<T>(bias[n + gate * a.second]) : 0.f;
+            }
+            asm volatile("bar.sync %0, 128;" ::"r"(1 + grp) : "memory");
         };
         int it = 0;
-        for (int i = blockIdx.x; i < tiles; i += gridDim.x, ++it) {
-            if ((it & 1) != grp) continue;
+        for (int i = walker; i < tiles; i += walkers, ++it) {
+            if (NB == 2 && (it & 1) != grp) continue;
             const Tile t = tile_at(i);
-            if (!mbar_wait_prompt(acc_full + grp, (it >> 1) & 1, abort_flag)) break;
+            const int m0 = t.m0 + quarter * 32, n0 = t.n0, first = NB == 2 ? 0 : 64 * grp;
+            float* const bias = bias_at + (it / NB & 1) * S::kBiasFloats;
+            if constexpr (EPI != EPI_PART) fill_bias(bias, n0 + first);
+            if (!mbar_wait_prompt(acc_full + it % NB, (it / NB) & 1, abort_flag)) break;
             __syncwarp();
             tc_fence_after();
-            const int m0 = t.m * kRows + quarter * 32, n0 = t.n * S::kOut;
             if constexpr (EPI == EPI_PART) {
 #pragma unroll 1
                 for (int c = 0; c < S::kOut; c += 32) {
+                    uint32_t r[2][16];
                     ready();
+                    tmem_ld16(lane_base + c, r[0]);
+                    tmem_ld16(lane_base + c + 16, r[1]);
+                    tmem_ld_wait();
 #pragma unroll
-                    for (int q = 0; q < 32; q += 16) {
-                        uint32_t r[16];
-                        tmem_ld16(lane_base + c + q, r);
-                        tmem_ld_wait();
+                    for (int q = 0; q < 2; ++q)
 #pragma unroll
-                        for (int u = 0; u < 4; ++u) put(q / 4 + u, make_uint4(r[4 * u], r[4 * u + 1], r[4 * u + 2], r[4 * u + 3]));
-                    }
+                        for (int u = 0; u < 4; ++u) put(4 * q + u, make_uint4(r[q][4 * u], r[q][4 * u + 1], r[q][4 * u + 2], r[q][4 * u + 3]));
                     send(n0 + c, m0, t.split);
                 }
             } else {
+                // 16 columns at a time; the next ones leave TMEM while these are worked on
+                constexpr int kIn = EPI == EPI_OUT ? 1 : EPI == EPI_GATE ? 2 : 3;
 #pragma unroll 1
-                for (int c = 0; c < S::kOut; c += 64) {
+                for (int c = first; c < S::kOut; c += NB == 2 ? 64 : 128) {
+                    uint32_t r[2][kIn][16];
+                    auto load = [&](int q) {
+#pragma unroll
+                        for (int j = 0; j < kIn; ++j) tmem_ld16(lane_base + j * S::kOut + c + 16 * q, r[q & 1][j]);
+                    };
                     ready();
+                    load(0);
 #pragma unroll
-                    for (int q = 0; q < 64; q += 16) {
-                        uint32_t x[16];
-                        tmem_ld16(lane_base + c + q, x);
-                        if constexpr (EPI == EPI_GATE || EPI == EPI_GRAD) {
-                            uint32_t y[16], z[16];
-                            tmem_ld16(lane_base + S::kOut + c + q, y);
-                            if constexpr (EPI == EPI_GRAD) tmem_ld16(lane_base + 2 * S::kOut + c + q, z);
-                            tmem_ld_wait();
+                    for (int q = 0; q < 4; ++q) {
+                        tmem_ld_wait();
+                        if (q < 3) load(q + 1);
+                        const auto& x = r[q & 1];
+                        const float* const b = bias + c - first + 16 * q;
+                        uint32_t w[8], w2[8];
 #pragma unroll
-                            for (int h = 0; h < 16; h += 8) {
-                                float bv[8], bg[8];
-                                bias8(n0 + c + q + h, a.N, bv);
-                                bias8(a.second + n0 + c + q + h, a.second + a.N, bg);
-                                uint32_t w[4], w2[4];
-#pragma unroll
-                                for (int j = 0; j < 4; ++j) {
-                                    const int e = h + 2 * j;
-                                    const float2 v = __fadd2_rn(make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), make_float2(bv[2 * j], bv[2 * j + 1]));
-                                    const float2 g = __fadd2_rn(make_float2(__uint_as_float(y[e]), __uint_as_float(y[e + 1])), make_float2(bg[2 * j], bg[2 * j + 1]));
-                                    if constexpr (EPI == EPI_GATE) {
-                                        const float2 o = __fmul2_rn(v, act_pair<T, ACT>(g));
-                                        w[j] = Half2Of<T>::pack(o.x, o.y);
-                                    } else {
-                                        const float2 dh = make_float2(__uint_as_float(z[e]), __uint_as_float(z[e + 1]));
-                                        float2 act, slope;
-                                        act_grad_pair<T, ACT>(g, act, slope);
-                                        const float2 dv = __fmul2_rn(dh, act), dg = __fmul2_rn(__fmul2_rn(dh, v), slope);
-                                        w[j] = Half2Of<T>::pack(dv.x, dv.y);
-                                        w2[j] = Half2Of<T>::pack(dg.x, dg.y);
-                                    }
+                        for (int j = 0; j < 8; ++j) {
+                            const int e = 2 * j;
+                            const float2 v = __fadd2_rn(make_float2(__uint_as_float(x[0][e]), __uint_as_float(x[0][e + 1])), *reinterpret_cast<const float2*>(b + e));
+                            if constexpr (EPI == EPI_OUT) w[j] = Half2Of<T>::pack(v.x, v.y);
+                            else {
+                                const float2 g = __fadd2_rn(make_float2(__uint_as_float(x[1][e]), __uint_as_float(x[1][e + 1])),
+                                                            *reinterpret_cast<const float2*>(b + kBiasCols + e));
+                                if constexpr (EPI == EPI_GATE) {
+                                    const float2 o = __fmul2_rn(v, act_pair<T, ACT>(g));
+                                    w[j] = Half2Of<T>::pack(o.x, o.y);
+                                } else {
+                                    const float2 dh = make_float2(__uint_as_float(x[kIn - 1][e]), __uint_as_float(x[kIn - 1][e + 1]));
+                                    float2 act, slope;
+                                    act_grad_pair<T, ACT>(g, act, slope);
+                                    const float2 dv = __fmul2_rn(dh, act), dg = __fmul2_rn(__fmul2_rn(dh, v), slope);
+                                    w[j] = Half2Of<T>::pack(dv.x, dv.y);
+                                    w2[j] = Half2Of<T>::pack(dg.x, dg.y);
                                 }
-                                put((q + h) / 8, make_uint4(w[0], w[1], w[2], w[3]));
-                                if constexpr (EPI == EPI_GRAD) put((q + h) / 8, make_uint4(w2[0], w2[1], w2[2], w2[3]), 1);
                             }
-                        } else {
-                            tmem_ld_wait();
-#pragma unroll
-                            for (int h = 0; h < 16; h += 8) {
-                                float b[8];
-                                bias8(n0 + c + q + h, a.N, b);
-                                uint32_t w[4];
-#pragma unroll
-                                for (int j = 0; j < 4; ++j)
-                                    w[j] = Half2Of<T>::pack(__uint_as_float(x[h + 2 * j]) + b[2 * j], __uint_as_float(x[h + 2 * j + 1]) + b[2 * j + 1]);
-                                put((q + h) / 8, make_uint4(w[0], w[1], w[2], w[3]));
-                            }
+                        }
+                        put(2 * q, make_uint4(w[0], w[1], w[2], w[3]));
+                        put(2 * q + 1, make_uint4(w[4], w[5], w[6], w[7]));
+                        if constexpr (EPI == EPI_GRAD) {
+                            put(2 * q, make_uint4(w2[0], w2[1], w2[2], w2[3]), 1);
+                            put(2 * q + 1, make_uint4(w2[4], w2[5], w2[6], w2[7]), 1);
                         }
                     }
                     send(n0 + c, m0, 0);
@@ -281,14 +326,22 @@ product_tc05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(acc_empty + grp);
+            if (lane == 0) {
+                if constexpr (kPair) mbar_arrive_at(in_rank(acc_empty + it % NB, 0));
+                else mbar_arrive(acc_empty + it % NB);
+            }
         }
         if (lane == 0) store_done();
     }
     // ---------------------------------------------------------------- teardown
     tc_fence_before();
     __syncthreads();
-    if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem, S::kTmem); }
+    if constexpr (kPair) cluster_sync();
+    if (warp == 1) {
+        tc_fence_after();
+        if constexpr (kPair) tmem_dealloc_pair(tmem, S::kTmem);
+        else tmem_dealloc(tmem, S::kTmem);
+    }
     if (threadIdx.x == 0 && *abort_flag) atomicExch(a.error_flag, 1);
 }
 
@@ -328,8 +381,8 @@ inline int sm_count() {
     return sms;
 }
 
-template <typename T, bool kAMN, bool kBMN, int EPI, int ACT, int kCols> int run_product(const Product& p, cudaStream_t st) {
-    using S = Shape<EPI, kCols>;
+template <typename T, bool kAMN, bool kBMN, int EPI, int ACT, int kCols, bool kPair> int run_product(const Product& p, cudaStream_t st) {
+    using S = Shape<EPI, kCols, kPair>;
     constexpr bool kDual = EPI == EPI_GATE || EPI == EPI_GRAD;
     constexpr auto sw = CU_TENSOR_MAP_SWIZZLE_128B;
     // (in front of the maps: a thread that has made no runtime call yet, one of autograd's for instance, has no context for the driver to encode in)
@@ -341,7 +394,7 @@ template <typename T, bool kAMN, bool kBMN, int EPI, int ACT, int kCols> int run
     bool ok = kAMN ? make_map_pitched(&ta, Fmt<T>::tm, p.a.p, p.K, p.M, p.a.pitch, kDepth, 64, sw)
                    : make_map_pitched(&ta, Fmt<T>::tm, p.a.p, p.M, p.K, p.a.pitch, kRows, kDepth, sw);
     ok = ok && (kBMN && !kDual ? make_map_pitched(&tb, Fmt<T>::tm, p.b.p, p.K, p.N, p.b.pitch, kDepth, 64, sw)
-                               : make_map_pitched(&tb, Fmt<T>::tm, p.b.p, p.b_rows, p.K, p.b.pitch, kDual ? S::kOut : S::kB, kDepth, sw));
+                               : make_map_pitched(&tb, Fmt<T>::tm, p.b.p, p.b_rows, p.K, p.b.pitch, kDual ? S::kOut : S::kB / S::kShare, kDepth, sw));
     ta2 = ta; tb2 = tb;
     if constexpr (EPI == EPI_GRAD)
         ok = ok && make_map_pitched(&ta2, Fmt<T>::tm, p.a2.p, p.M, p.K2, p.a2.pitch, kRows, kDepth, sw) &&
@@ -351,17 +404,19 @@ template <typename T, bool kAMN, bool kBMN, int EPI, int ACT, int kCols> int run
     to2 = to;
     if constexpr (EPI == EPI_GRAD) ok = ok && make_out_map<T>(&to2, p.out2, 1, p.M, p.N, p.out_pitch);
     if (!ok) return SS2D_ECUDA;
-    auto kern = product_tc05_kernel<T, kAMN, kBMN, EPI, ACT, kCols>;
+    auto kern = product_tc05_kernel<T, kAMN, kBMN, EPI, ACT, kCols, kPair>;
     if (const int rc = allow_dynamic_smem(kern, S::kBytes)) return rc;
     Args a = {};
-    a.m_tiles = (int)((p.M + kRows - 1) / kRows); a.n_tiles = (int)((p.N + S::kOut - 1) / S::kOut);
+    a.m_tiles = (int)((p.M + kRows * S::kShare - 1) / (kRows * S::kShare)); a.n_tiles = (int)((p.N + S::kOut - 1) / S::kOut);
     a.splits = EPI == EPI_PART ? p.splits : 1;
     a.blocks = (int)((p.K + kDepth - 1) / kDepth); a.per_split = EPI == EPI_PART ? p.per_split : a.blocks;
     a.blocks2 = (int)((p.K2 + kDepth - 1) / kDepth);
     a.M = (int)p.M; a.N = (int)p.N; a.second = (int)p.N; a.bias = p.bias; a.error_flag = dev_flag;
     const int tiles = a.m_tiles * a.n_tiles * a.splits, sms = sm_count();
     if (!sms) return SS2D_ECUDA;
-    launch(kern, tiles < sms ? tiles : sms, kThreads, S::kBytes, st, ta, tb, ta2, tb2, to, to2, a);
+    const int walkers = tiles < sms / S::kShare ? tiles : sms / S::kShare;
+    if constexpr (kPair) launch_pairs(kern, walkers * 2, kThreads, S::kBytes, st, ta, tb, ta2, tb2, to, to2, a);
+    else launch(kern, walkers, kThreads, S::kBytes, st, ta, tb, ta2, tb2, to, to2, a);
     count_launch();
     return check_launch();
 }
