@@ -560,18 +560,20 @@ int ss2d_linear_attention_step(const ss2d_linear_attention_step_params *p, void 
  *   [v g] = x w1^T + b1;  h = v * act(g);  y = h w2^T + b2
  * x: (tokens, channels), rows x_row_stride elements apart; w1: (2 hidden, channels), the rows of the values first; w2: (outputs, hidden); b1 (2 hidden) and
  * b2 (outputs) or NULL; y: (tokens, outputs).  All of `dtype`; dense but for x's rows.  act: 1 GELU (erf), 2 SiLU.  h: (tokens, hidden) of `dtype`,
- * written by the forward call, 16-byte aligned.  Sums are fp32; no atomics: repeated calls give bit-identical results.
+ * written by the forward call, 16-byte aligned.  workspace: ss2d_gated_mlp_workspace_bytes() bytes, 16-byte aligned (0: none), a size of the shape alone.  Sums are fp32; no atomics: repeated calls give bit-identical results.
  * -------------------------------------------------------------------------------- */
 typedef struct ss2d_gated_mlp_params {
     const void *x, *w1, *b1, *w2, *b2;
-    void *h, *y;
+    void *h, *y, *workspace;
+    int64_t workspace_bytes;
     int64_t tokens, channels, hidden, outputs, x_row_stride;
     int32_t dtype, act;
 } ss2d_gated_mlp_params;
 
 int ss2d_gated_mlp_fwd(const ss2d_gated_mlp_params *p, void *cuda_stream);
+int64_t ss2d_gated_mlp_workspace_bytes(const ss2d_gated_mlp_params *p);      /* < 0: invalid arguments */
 
-/* Its backward call: `fwd` with h as the forward call left it (y and b2 are not read); dy (tokens, outputs) of `dtype`, rows dy_row_stride
+/* Its backward call: `fwd` with h as the forward call left it (y, b2 and its workspace are not read); dy (tokens, outputs) of `dtype`, rows dy_row_stride
  * elements apart.  dx (tokens, channels), dw1, dw2, db1, db2 as the tensors that they belong to, dense; NULL: not asked for. */
 typedef struct ss2d_gated_mlp_bwd_params {
     ss2d_gated_mlp_params fwd;

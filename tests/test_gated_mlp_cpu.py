@@ -26,6 +26,13 @@ def test_refusals_of_the_c_interface():
     call = L.ss2d_gated_mlp_fwd
     assert call(None, None) == -1
     p, a = params()
+    assert L.ss2d_gated_mlp_workspace_bytes(p) == 0 and L.ss2d_gated_mlp_workspace_bytes(None) < 0
+    p.hidden, p.tokens = 4096, 100                                # few tiles, a long contraction: split, its parts in a workspace
+    need = L.ss2d_gated_mlp_workspace_bytes(p)
+    assert need >= 2 * 4 * 100 * 16 and call(p, None) == -8
+    p.workspace, p.workspace_bytes = a, need - 1
+    assert call(p, None) == -8
+    p, a = params()
     for field, bad, code in (("x", None, -1), ("w2", None, -1), ("h", None, -1), ("y", None, -1), ("dtype", 9, -3), ("act", 0, -6), ("act", 3, -6),
                              ("tokens", 0, -2), ("hidden", -1, -2), ("x_row_stride", 15, -5), ("w1", a + 1, -4), ("h", a + 8, -4), ("b1", a + 1, -4),
                              ("y", a + 2, -4), ("tokens", 1 << 40, -6)):

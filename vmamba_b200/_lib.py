@@ -144,8 +144,8 @@ class LinearAttentionStepParams(ctypes.Structure):
 
 
 class GatedMlpParams(ctypes.Structure):
-    _fields_ = [(n, _vp) for n in ("x", "w1", "b1", "w2", "b2", "h", "y")] + \
-               [(n, _i64) for n in ("tokens", "channels", "hidden", "outputs", "x_row_stride")] + [("dtype", _i32), ("act", _i32)]
+    _fields_ = [(n, _vp) for n in ("x", "w1", "b1", "w2", "b2", "h", "y", "workspace")] + \
+               [(n, _i64) for n in ("workspace_bytes", "tokens", "channels", "hidden", "outputs", "x_row_stride")] + [("dtype", _i32), ("act", _i32)]
 
 
 class GatedMlpBwdParams(ctypes.Structure):
@@ -195,6 +195,7 @@ EXPORTS = {
     "ss2d_linear_attention_bwd_workspace_bytes": (_i64, [ctypes.POINTER(LinearAttentionBwdParams)]),
     "ss2d_linear_attention_step": (ctypes.c_int, [ctypes.POINTER(LinearAttentionStepParams), _vp]),
     "ss2d_gated_mlp_fwd": (ctypes.c_int, [ctypes.POINTER(GatedMlpParams), _vp]),
+    "ss2d_gated_mlp_workspace_bytes": (_i64, [ctypes.POINTER(GatedMlpParams)]),
     "ss2d_gated_mlp_bwd": (ctypes.c_int, [ctypes.POINTER(GatedMlpBwdParams), _vp]),
     "ss2d_gated_mlp_bwd_workspace_bytes": (_i64, [ctypes.POINTER(GatedMlpBwdParams)]),
     "ss2d_set_debug_checks": (ctypes.c_int, [ctypes.c_int]),

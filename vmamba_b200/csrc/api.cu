@@ -53,6 +53,7 @@ int linear_attention_step(const ss2d_linear_attention_step_params* p, cudaStream
 int gated_mlp_fwd(const ss2d_gated_mlp_params* p, cudaStream_t st);
 int gated_mlp_bwd(const ss2d_gated_mlp_bwd_params* p, cudaStream_t st);
 long long gated_mlp_bwd_workspace_bytes(const ss2d_gated_mlp_bwd_params* p);
+long long gated_mlp_workspace_bytes(const ss2d_gated_mlp_params* p);
 
 static std::atomic<long long> g_launches{0};
 static std::atomic<int> g_debug_checks{[] { const char* v = std::getenv("SS2D_DEBUG_CHECKS"); return (v && v[0] == '1') ? 1 : 0; }()};
@@ -236,9 +237,10 @@ int ss2d_linear_attention_step(const ss2d_linear_attention_step_params* p, void*
 }
 int ss2d_gated_mlp_fwd(const ss2d_gated_mlp_params* p, void* stream) {
     ss2d::Range nvtx_("ss2d_gated_mlp_fwd");
-    if (p) SS2D_CHECK_PTRS(p->x, p->w1, p->b1, p->w2, p->b2, p->h, p->y);
+    if (p) SS2D_CHECK_PTRS(p->x, p->w1, p->b1, p->w2, p->b2, p->h, p->y, p->workspace);
     return ss2d::gated_mlp_fwd(p, (cudaStream_t)stream);
 }
+int64_t ss2d_gated_mlp_workspace_bytes(const ss2d_gated_mlp_params* p) { return ss2d::gated_mlp_workspace_bytes(p); }
 int ss2d_gated_mlp_bwd(const ss2d_gated_mlp_bwd_params* p, void* stream) {
     ss2d::Range nvtx_("ss2d_gated_mlp_bwd");
     if (p) SS2D_CHECK_PTRS(p->fwd.x, p->fwd.w1, p->fwd.w2, p->fwd.b1, p->fwd.h, p->dy, p->dx, p->dw1, p->db1, p->dw2, p->db2, p->workspace);

@@ -111,10 +111,77 @@ __global__ void __launch_bounds__(128) product_kernel(const ProductArgs p) {
         }
 }
 
+// ---- few tokens ---------------------------------------------------------------------------------------------------------
+// Up to 16 tokens of 16-bit types: the weights' way from memory is the whole time, and every SM has to take part in it.  A CTA has kRows rows of the weights (of value and
+// gate alike), its eight warps every eighth 32 elements of them, straight from memory into the A operand of mma.sync: a lane reads 16 bytes, 8 contraction elements in a row,
+// and the products take them in that order (the tokens' elements come the same way).  The warps' sums meet in shared memory.  us of both launches with 1 / 8 / 16 tokens, and
+// of the tensor-core kernels with 33: 768 channels and 2 048 hidden 9.3 / 9.0 / 12.4, 15.9; 384 and 1 536 5.4 / 5.9 / 8.8, 14.0; 1 024 and 4 096, from memory, 18 / 18 / 24, 19.
+constexpr int kFew = 16;
+struct FewArgs {
+    const void *x, *w, *bias;
+    void* out;
+    long long ldx, second;      // second: rows between value and gate
+    int M, N, K;
+};
+template <typename T, int kTiles, int kRows, int EPI, int ACT>
+__global__ void __launch_bounds__(256) few_tokens_kernel(const FewArgs a) {
+    follow_previous();
+    constexpr int kMats = EPI == EPI_GATE ? 2 : 1, kBlocks = kRows / 8;
+    __shared__ float sums[8][kMats][kTiles][kRows][9];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3, n0 = blockIdx.x * kRows;
+    float acc[kMats][kTiles][4] = {};
+    const T *const x = (const T*)a.x, *const w = (const T*)a.w;
+    constexpr int kAhead = 16 / (kMats * kBlocks);          // 16 loads of weights on their way
+#pragma unroll kAhead
+    for (int k = warp * 32 + 8 * t; k < (a.K + 31) / 32 * 32; k += 256) {
+        const uint4 none = make_uint4(0, 0, 0, 0);
+        uint4 wr[kMats][2], xr[kTiles];
+#pragma unroll
+        for (int m = 0; m < kMats; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int row = n0 + g + 8 * h;
+                wr[m][h] = h < kBlocks && k < a.K && row < a.N ? *reinterpret_cast<const uint4*>(w + (row + m * a.second) * a.K + k) : none;
+            }
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i)
+            xr[i] = k < a.K && 8 * i + g < a.M ? *reinterpret_cast<const uint4*>(x + (8 * i + g) * a.ldx + k) : none;
+#pragma unroll
+        for (int m = 0; m < kMats; ++m) {
+            const uint32_t lo[4] = {wr[m][0].x, wr[m][1].x, wr[m][0].y, wr[m][1].y}, hi[4] = {wr[m][0].z, wr[m][1].z, wr[m][0].w, wr[m][1].w};
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) {
+                const uint32_t b0[2] = {xr[i].x, xr[i].y}, b1[2] = {xr[i].z, xr[i].w};
+                MmaK16<T>::run(acc[m][i], lo, b0);
+                MmaK16<T>::run(acc[m][i], hi, b1);
+            }
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < kMats; ++m)
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+            for (int j = 0; j < 2 * kBlocks; ++j) sums[warp][m][i][g + 8 * (j >> 1)][2 * t + (j & 1)] = acc[m][i][j];
+    __syncthreads();
+    for (int i = tid; i < kRows * 8 * kTiles; i += 256) {
+        const int row = i % kRows, token = i / kRows, n = n0 + row;
+        if (n >= a.N || token >= a.M) continue;
+        float y[kMats];
+#pragma unroll
+        for (int m = 0; m < kMats; ++m) {
+            y[m] = a.bias ? to_f<T>(((const T*)a.bias)[n + m * a.second]) : 0.f;
+            for (int v = 0; v < 8; ++v) y[m] += sums[v][m][token / 8][row][token % 8];
+        }
+        if constexpr (EPI == EPI_GATE) y[0] *= gate_act<ACT>(y[1]);
+        ((T*)a.out)[(long long)token * a.N + n] = from_f<T>(y[0]);
+    }
+}
+
 // ---- sums ---------------------------------------------------------------------------------------------------------------
 // Column sums of two (rows, cols) matrices (the second may have none) over spans of rows, fp32: part[span][cols of both].  A warp has 32 kVec columns, eight warps
 // every eighth row.
-constexpr int kSpan = 256;
+constexpr int kSpan = 128;
 struct SumArgs {
     const void* a[2];
     long long ld[2], rows;
@@ -132,7 +199,7 @@ template <typename T, int kVec> __global__ void __launch_bounds__(256) column_su
     const long long ld = s.ld[which], r0 = (long long)blockIdx.y * kSpan, r1 = r0 + kSpan < s.rows ? r0 + kSpan : s.rows;
     float x[kVec] = {};
     if (c < cols) {
-#pragma unroll 4
+#pragma unroll 8
         for (long long r = r0 + warp; r < r1; r += 8) {
             float y[kVec];
             Vec<T, kVec>::load(a + r * ld + c, y);
@@ -160,11 +227,13 @@ template <typename T> __global__ void __launch_bounds__(256) add_columns_kernel(
     ((T*)s.out[which])[i - which * s.cols[0]] = from_f<T>(x);
 }
 // out[i] = sum over parts, in order
-template <typename T, int kVec> __global__ void __launch_bounds__(256) add_parts_kernel(const float* part, T* out, long long n, int parts) {
+// (+ bias of the column, rows of `cols`)
+template <typename T, int kVec> __global__ void __launch_bounds__(256) add_parts_kernel(const float* part, T* out, long long n, int parts, const T* bias, int cols) {
     follow_previous();
     const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * kVec;
     if (i >= n) return;
     float x[kVec] = {};
+    if (bias) Vec<T, kVec>::load(bias + i % cols, x);
 #pragma unroll 4
     for (int p = 0; p < parts; ++p) {
         float y[kVec];
@@ -192,21 +261,23 @@ template <typename T> ProductArgs product_args(const void* a, long long lda, con
     p.per_split = (p.K + kStep - 1) / kStep * kStep;
     return p;
 }
-// Splits of a contraction over the tokens whose result has few tiles: enough for two CTAs an SM, each with 8 steps at least
+// Splits of a contraction whose result has few tiles: enough for two CTAs an SM, each with 4 steps at least
 int splits_of(long long M, long long N, long long K) {
     const long long tiles = ((M + kTile - 1) / kTile) * ((N + kTile - 1) / kTile), steps = (K + kStep - 1) / kStep;
     long long s = (2 * 148 + tiles - 1) / tiles;
-    if (s > steps / 8) s = steps / 8;
+    if (s > steps / 4) s = steps / 4;
     return s < 1 ? 1 : s > 64 ? 64 : (int)s;
 }
-template <typename T> int add_parts(const float* part, void* out, long long n, int parts, cudaStream_t st) {
-    if (n % 4 == 0 && aligned_to(out, 4 * sizeof(T))) launch(add_parts_kernel<T, 4>, (unsigned)((n / 4 + 255) / 256), 256, 0, st, part, (T*)out, n, parts);
-    else launch(add_parts_kernel<T, 1>, (unsigned)((n + 255) / 256), 256, 0, st, part, (T*)out, n, parts);
+template <typename T> int add_parts(const float* part, void* out, long long n, int parts, const void* bias, long long cols, cudaStream_t st) {
+    if (cols % 4 == 0 && n % 4 == 0 && aligned_to(out, 4 * sizeof(T)) && aligned_to(bias, 4 * sizeof(T)))
+        launch(add_parts_kernel<T, 4>, (unsigned)((n / 4 + 255) / 256), 256, 0, st, part, (T*)out, n, parts, (const T*)bias, (int)cols);
+    else launch(add_parts_kernel<T, 1>, (unsigned)((n + 255) / 256), 256, 0, st, part, (T*)out, n, parts, (const T*)bias, (int)cols);
     count_launch();
     return check_launch();
 }
-// out (M x N) = A^T B over K tokens, rows of A and B contiguous
-template <typename T> int weight_gradient(const void* a, long long lda, const void* b, long long ldb, long long M, long long N, long long K, void* out, float* part, cudaStream_t st) {
+// out (M x N, dense) = A B^T (+ bias)
+template <typename T, bool kAK, bool kBK>
+int product(const void* a, long long lda, const void* b, long long ldb, long long M, long long N, long long K, const void* bias, void* out, float* part, cudaStream_t st) {
     ProductArgs p = product_args<T>(a, lda, b, ldb, M, N, K);
     p.e.pairs = N % 2 == 0;
     const int want = splits_of(M, N, K);
@@ -214,12 +285,12 @@ template <typename T> int weight_gradient(const void* a, long long lda, const vo
     p.per_split = (p.per_split + kStep - 1) / kStep * kStep;
     const int splits = (p.K + p.per_split - 1) / p.per_split;
     if (splits == 1) {
-        p.e.out = out; p.e.ld = N;
-        return launch_product<T, true, true, EPI_OUT, ACT_NONE>(p, 1, st);
+        p.e.bias = bias; p.e.out = out; p.e.ld = N;
+        return launch_product<T, kAK, kBK, EPI_OUT, ACT_NONE>(p, 1, st);
     }
     p.e.part = part;
-    if (const int rc = launch_product<T, true, true, EPI_PART, ACT_NONE>(p, splits, st)) return rc;
-    return add_parts<T>(part, out, M * N, splits, st);
+    if (const int rc = launch_product<T, kAK, kBK, EPI_PART, ACT_NONE>(p, splits, st)) return rc;
+    return add_parts<T>(part, out, M * N, splits, bias, N, st);
 }
 template <typename T> int column_sums(SumArgs s, cudaStream_t st) {
     s.spans = (int)((s.rows + kSpan - 1) / kSpan);
@@ -257,12 +328,8 @@ template <typename T, int ACT> int plain_forward(const ss2d_gated_mlp_params& p,
     a.second = (int)p.hidden;
     a.e.bias = p.b1; a.e.out = p.h; a.e.ld = p.hidden; a.e.hidden = (int)p.hidden; a.e.pairs = p.hidden % 2 == 0;
     if (const int rc = launch_product<T, false, false, EPI_GATE, ACT>(a, 1, st)) return rc;
-    ProductArgs b = product_args<T>(p.h, p.hidden, p.w2, p.hidden, p.tokens, p.outputs, p.hidden);
-    b.e.bias = p.b2; b.e.out = p.y; b.e.ld = p.outputs; b.e.pairs = p.outputs % 2 == 0;
-    return launch_product<T, false, false, EPI_OUT, ACT_NONE>(b, 1, st);
+    return product<T, false, false>(p.h, p.hidden, p.w2, p.hidden, p.tokens, p.outputs, p.hidden, p.b2, p.y, (float*)p.workspace, st);
 }
-
-struct BwdPlan { long long dz, part, pre, total; };
 
 // 16-bit operands whose rows TMA can read: the tensor-core kernels.
 bool tc_fits(const ss2d_gated_mlp_params& p) {
@@ -272,78 +339,91 @@ bool tc_fits(const ss2d_gated_mlp_params& p) {
     return true;
 }
 
-// Tiles of the tensor-core kernels: columns in TMEM, and whether two CTAs share one of 256 rows.
-enum Form { kNarrow, kWide, kPairNarrow, kPairWide, kForms };
-constexpr int kFormCols[kForms] = {128, 256, 128, 256}, kFormCtas[kForms] = {1, 1, 2, 2};
-// Time of a product in cycles, for the choice among them: rounds of tiles over the SMs, a step of 64 of the contraction as long as its operands take from L2 with all
-// SMs reading (40 bytes a cycle and SM; at least its columns), and a fixed part for filling the ring and the last tile's epilogue.
-double tc_cycles(int form, long long M, long long N, int out, long long steps, long long splits) {
-    const int ctas = kFormCtas[form], cols = kFormCols[form];
-    const long long tiles = ((M + ptc::kRows * ctas - 1) / (ptc::kRows * ctas)) * ((N + out - 1) / out) * splits, at_once = 148 / ctas;
-    const double step = (ptc::kRows + cols / ctas) * 128 / 40.0;
-    return (double)((tiles + at_once - 1) / at_once) * steps * (step < cols ? cols : step) + 1500.0;
-}
-int best_form(long long M, long long N, bool gate, long long K) {
+// Tiles of the tensor-core kernels: 128 x 128, 128 x 256 (in TMEM; EPI_GATE gives half as many columns) by one CTA, 256 x 256 by two.
+enum Form { kNarrow, kWide, kPair, kForms };
+constexpr int kFormRows[kForms] = {128, 128, 256}, kFormCols[kForms] = {128, 256, 256}, kFormCtas[kForms] = {1, 1, 2};
+// Cycles that a step of 64 of the contraction takes them, measured with all SMs at it (us of h / y / dx of 16 384 tokens, 1 024 channels and 2 728 hidden: 194 / 121 / 189,
+// 132 / 114 / 164, 119 / 87 / 134; of 6 272, 384 and 1 536: 22.0 / 11.5 / 18.1, 16.9 / 15.1 / 21.7, 21.0 / 14.6 / 20.9: rounds of tiles over the SMs decide there).
+constexpr double kFormStep[kForms] = {660, 950, 800};
+
+struct Plan { int form, splits, per_split; };
+// The fewest cycles: rounds of tiles, their steps, and a fixed part for filling the ring and the last tile's epilogue.  A contraction is split, if it may be, where there
+// are few tiles: the partial sums are written and read again (8 bytes an element and split at about 3 300 bytes a cycle) by a launch of its own.
+Plan plan_of(long long M, long long N, long long K, bool gate, bool may_split) {
     const long long steps = (K + ptc::kDepth - 1) / ptc::kDepth;
-    int best = 0;
+    Plan best = {0, 1, (int)steps};
     double least = 1e30;
     for (int f = 0; f < kForms; ++f) {
-        const double t = tc_cycles(f, M, N, gate ? kFormCols[f] / 2 : kFormCols[f], steps, 1);
-        if (t < least) { least = t; best = f; }
+        const long long out = gate ? kFormCols[f] / 2 : kFormCols[f], at_once = 148 / kFormCtas[f];
+        const long long tiles = ((M + kFormRows[f] - 1) / kFormRows[f]) * ((N + out - 1) / out);
+        for (long long s = 1; s <= (may_split ? 64 : 1) && s <= steps; ++s) {
+            const long long per = (steps + s - 1) / s, splits = (steps + per - 1) / per;
+            const double t = (double)((tiles * splits + at_once - 1) / at_once) * per * kFormStep[f] + (splits > 1 ? 4500.0 + 8.0 * splits * M * N / 3300.0 : 0.0);
+            if (t < least) { least = t; best = {f, (int)splits, (int)per}; }
+        }
     }
     return best;
+}
+long long part_elements(long long M, long long N, long long K) {
+    const Plan w = plan_of(M, N, K, false, true);
+    return w.splits > 1 ? w.splits * M * N : 0;
 }
 template <typename T, bool kAMN, bool kBMN, int EPI, int ACT> int run_form(int form, const ptc::Product& p, cudaStream_t st) {
     switch (form) {
         case kNarrow: return ptc::run_product<T, kAMN, kBMN, EPI, ACT, 128, false>(p, st);
         case kWide: return ptc::run_product<T, kAMN, kBMN, EPI, ACT, 256, false>(p, st);
-        case kPairNarrow: return ptc::run_product<T, kAMN, kBMN, EPI, ACT, 128, true>(p, st);
         default: return ptc::run_product<T, kAMN, kBMN, EPI, ACT, 256, true>(p, st);
     }
 }
+// out (M x N, dense) = A B^T (+ bias)
+template <typename T, bool kAMN, bool kBMN> int tc_product(ptc::Operand a, ptc::Operand b, long long M, long long N, long long K, const void* bias, void* out, float* part, cudaStream_t st) {
+    const Plan w = plan_of(M, N, K, false, true);
+    ptc::Product p = {};
+    p.a = a; p.b = b;
+    p.M = M; p.N = N; p.K = K; p.b_rows = N; p.out_pitch = N;
+    if (w.splits == 1) {
+        p.bias = bias; p.out = out;
+        return run_form<T, kAMN, kBMN, EPI_OUT, ACT_NONE>(w.form, p, st);
+    }
+    p.out = part; p.splits = w.splits; p.per_split = w.per_split;
+    if (const int rc = run_form<T, kAMN, kBMN, EPI_PART, ACT_NONE>(w.form, p, st)) return rc;
+    return add_parts<T>(part, out, M * N, w.splits, bias, N, st);
+}
+
+template <typename T, int EPI, int ACT> int launch_few(const FewArgs& a, cudaStream_t st) {
+    auto go = [&](auto tiles, auto rows) {
+        constexpr int kTiles = decltype(tiles)::value, kRows = decltype(rows)::value;
+        launch(few_tokens_kernel<T, kTiles, kRows, EPI, ACT>, (a.N + kRows - 1) / kRows, 256, 0, st, a);
+        count_launch();
+        return check_launch();
+    };
+    auto with = [&](auto tiles) {       // rows of a CTA: 16, or 8 where that leaves SMs without one
+        return (a.N + 15) / 16 < 148 ? go(tiles, std::integral_constant<int, 8>()) : go(tiles, std::integral_constant<int, 16>());
+    };
+    return a.M <= 8 ? with(std::integral_constant<int, 1>()) : with(std::integral_constant<int, 2>());
+}
+template <typename T, int ACT> int few_forward(const ss2d_gated_mlp_params& p, cudaStream_t st) {
+    if (const int rc = launch_few<T, EPI_GATE, ACT>({p.x, p.w1, p.b1, p.h, p.x_row_stride, p.hidden, (int)p.tokens, (int)p.hidden, (int)p.channels}, st)) return rc;
+    return launch_few<T, EPI_OUT, ACT_NONE>({p.h, p.w2, p.b2, p.y, p.hidden, 0, (int)p.tokens, (int)p.outputs, (int)p.hidden}, st);
+}
 
 template <typename T, int ACT> int tc_forward(const ss2d_gated_mlp_params& p, cudaStream_t st) {
+    if (p.tokens <= kFew) return few_forward<T, ACT>(p, st);
     ptc::Product a = {};
     a.a = {p.x, p.x_row_stride}; a.b = {p.w1, p.channels};
     a.M = p.tokens; a.N = p.hidden; a.K = p.channels; a.b_rows = 2 * p.hidden;
     a.bias = p.b1; a.out = p.h; a.out_pitch = p.hidden;
-    if (const int rc = run_form<T, false, false, EPI_GATE, ACT>(best_form(a.M, a.N, true, a.K), a, st)) return rc;
-    ptc::Product b = {};
-    b.a = {p.h, p.hidden}; b.b = {p.w2, p.hidden};
-    b.M = p.tokens; b.N = p.outputs; b.K = p.hidden; b.b_rows = p.outputs;
-    b.bias = p.b2; b.out = p.y; b.out_pitch = p.outputs;
-    return run_form<T, false, false, EPI_OUT, ACT_NONE>(best_form(b.M, b.N, false, b.K), b, st);
+    if (const int rc = run_form<T, false, false, EPI_GATE, ACT>(plan_of(a.M, a.N, a.K, true, false).form, a, st)) return rc;
+    return tc_product<T, false, false>({p.h, p.hidden}, {p.w2, p.hidden}, p.tokens, p.outputs, p.hidden, p.b2, p.y, (float*)p.workspace, st);
+}
+// of either kind of kernel: which one takes a call also depends on where its tensors start
+long long fwd_workspace(const ss2d_gated_mlp_params& p) {
+    const long long s = splits_of(p.tokens, p.outputs, p.hidden), plain = s > 1 ? s * p.tokens * p.outputs : 0;
+    const long long tc = p.dtype == SS2D_F32 || p.tokens <= kFew ? 0 : part_elements(p.tokens, p.outputs, p.hidden);
+    return 4 * (plain > tc ? plain : tc);
 }
 
-// Splits of a weight gradient's contraction over the tokens, and its tile: the fewest cycles, with the partial sums' way to memory and back (8 bytes an element
-// and split at about 3 300 bytes a cycle)
-struct WeightPlan { int splits, per_split, form; };
-WeightPlan tc_weight_plan(long long M, long long N, long long K) {
-    const long long steps = (K + ptc::kDepth - 1) / ptc::kDepth;
-    WeightPlan best = {1, (int)steps, 0};
-    double least = 1e30;
-    for (int f = 0; f < kForms; ++f)
-        for (long long s = 1; s <= 64 && s <= steps; ++s) {
-            const long long per = (steps + s - 1) / s, splits = (steps + per - 1) / per;
-            const double t = tc_cycles(f, M, N, kFormCols[f], per, splits) + (splits > 1 ? 3000.0 + 8.0 * splits * M * N / 3300.0 : 0.0);
-            if (t < least) { least = t; best = {(int)splits, (int)per, f}; }
-        }
-    return best;
-}
-template <typename T> int tc_weight_gradient(const void* a, long long lda, const void* b, long long ldb, long long M, long long N, long long K, void* out, float* part, cudaStream_t st) {
-    const WeightPlan w = tc_weight_plan(M, N, K);
-    ptc::Product p = {};
-    p.a = {a, lda}; p.b = {b, ldb};
-    p.M = M; p.N = N; p.K = K; p.b_rows = N; p.out_pitch = N;
-    if (w.splits == 1) {
-        p.out = out;
-        return run_form<T, true, true, EPI_OUT, ACT_NONE>(w.form, p, st);
-    }
-    p.out = part; p.splits = w.splits; p.per_split = w.per_split;
-    if (const int rc = run_form<T, true, true, EPI_PART, ACT_NONE>(w.form, p, st)) return rc;
-    return add_parts<T>(part, out, M * N, w.splits, st);
-}
-
+struct BwdPlan { long long dz, part, pre, total; };
 BwdPlan bwd_plan(const ss2d_gated_mlp_params& p) {
     auto up = [](long long n) { return (n + 255) / 256 * 256; };
     BwdPlan b;
@@ -351,8 +431,8 @@ BwdPlan bwd_plan(const ss2d_gated_mlp_params& p) {
     const long long spans = (p.tokens + kSpan - 1) / kSpan;
     long long most = spans * (2 * p.hidden + p.outputs);
     const long long M1 = 2 * p.hidden, N1 = p.channels, M2 = p.outputs, N2 = p.hidden;
-    for (long long n : {splits_of(M1, N1, p.tokens) * M1 * N1, splits_of(M2, N2, p.tokens) * M2 * N2, tc_weight_plan(M1, N1, p.tokens).splits * M1 * N1,
-                        tc_weight_plan(M2, N2, p.tokens).splits * M2 * N2})
+    for (long long n : {splits_of(M1, N1, p.tokens) * M1 * N1, splits_of(M2, N2, p.tokens) * M2 * N2, (long long)(splits_of(p.tokens, p.channels, M1) * p.tokens * p.channels), part_elements(M1, N1, p.tokens),
+                        part_elements(M2, N2, p.tokens), part_elements(p.tokens, p.channels, M1)})
         if (n > most) most = n;
     b.part = up(4 * most);
     b.pre = up(8 * p.tokens * p.hidden);                      // of calls that the tensor-core kernels do not take, wherever their tensors start
@@ -379,9 +459,10 @@ template <typename T, int ACT> int backward(const ss2d_gated_mlp_bwd_params& p, 
                 a.a = {f.x, f.x_row_stride}; a.b = {f.w1, f.channels}; a.a2 = {p.dy, p.dy_row_stride}; a.b2 = {f.w2, H};
                 a.M = f.tokens; a.N = H; a.K = f.channels; a.K2 = f.outputs; a.b_rows = H2; a.bias = f.b1;
                 a.out = dz; a.out2 = (T*)dz + H; a.out_pitch = H2;
-                // pairs with tiles of 128 columns where there is a round of them, 64 columns otherwise
-                const bool pair = ((f.tokens + 255) / 256) * ((H + 127) / 128) >= 74;
-                if (const int rc = pair ? ptc::run_product<T, false, true, EPI_GRAD, ACT, 384, true>(a, st) : ptc::run_product<T, false, true, EPI_GRAD, ACT, 192, false>(a, st)) return rc;
+                // tiles of 128 columns by one CTA, or by two of 256 rows, whose steps are shorter by what those of the forward products are: whichever takes fewer rounds by them
+                const long long n = (H + 127) / 128, one = ((f.tokens + 127) / 128 * n + 147) / 148, two = ((f.tokens + 255) / 256 * n + 73) / 74;
+                if (const int rc = two * kFormStep[kPair] < one * kFormStep[kWide] ? ptc::run_product<T, false, true, EPI_GRAD, ACT, 384, true>(a, st)
+                                                                                 : ptc::run_product<T, false, true, EPI_GRAD, ACT, 384, false>(a, st)) return rc;
             }
         if (!tc) {
             ProductArgs g = product_args<T>(f.x, f.x_row_stride, f.w1, f.channels, f.tokens, H, f.channels);
@@ -396,21 +477,16 @@ template <typename T, int ACT> int backward(const ss2d_gated_mlp_bwd_params& p, 
     if (p.dx) {
         if constexpr (sizeof(T) == 2)
             if (tc) {
-                ptc::Product a = {};
-                a.a = {dz, H2}; a.b = {f.w1, f.channels};
-                a.M = f.tokens; a.N = f.channels; a.K = H2; a.b_rows = f.channels; a.out = p.dx; a.out_pitch = f.channels;
-                if (const int rc = run_form<T, false, true, EPI_OUT, ACT_NONE>(best_form(a.M, a.N, false, a.K), a, st)) return rc;
+                if (const int rc = tc_product<T, false, true>({dz, H2}, {f.w1, f.channels}, f.tokens, f.channels, H2, nullptr, p.dx, part, st)) return rc;
             }
         if (!tc) {
-            ProductArgs a = product_args<T>(dz, H2, f.w1, f.channels, f.tokens, f.channels, H2);
-            a.e.out = p.dx; a.e.ld = f.channels; a.e.pairs = f.channels % 2 == 0;
-            if (const int rc = launch_product<T, false, true, EPI_OUT, ACT_NONE>(a, 1, st)) return rc;
+            if (const int rc = product<T, false, true>(dz, H2, f.w1, f.channels, f.tokens, f.channels, H2, nullptr, p.dx, part, st)) return rc;
         }
     }
     auto weight = [&](const void* a, long long lda, const void* b, long long ldb, long long M, long long N, void* out) {
         if constexpr (sizeof(T) == 2)
-            if (tc) return tc_weight_gradient<T>(a, lda, b, ldb, M, N, f.tokens, out, part, st);
-        return weight_gradient<T>(a, lda, b, ldb, M, N, f.tokens, out, part, st);
+            if (tc) return tc_product<T, true, true>({a, lda}, {b, ldb}, M, N, f.tokens, nullptr, out, part, st);
+        return product<T, true, true>(a, lda, b, ldb, M, N, f.tokens, nullptr, out, part, st);
     };
     if (p.dw1)
         if (const int rc = weight(dz, H2, f.x, f.x_row_stride, H2, f.channels, p.dw1)) return rc;
@@ -448,6 +524,8 @@ int gated_mlp_fwd(const ss2d_gated_mlp_params* p, cudaStream_t st) {
     if (const int rc = check_common(*p)) return rc;
     if (!p->h || !p->y) return SS2D_EINVAL_NULL;
     if (!aligned_to(p->h, 16) || !aligned_to(p->y, 2 * dtype_size(p->dtype))) return SS2D_EINVAL_ALIGN;
+    const long long need = fwd_workspace(*p);
+    if (need && (!p->workspace || p->workspace_bytes < need || !aligned_to(p->workspace, 16))) return SS2D_EWORKSPACE;
     return for_type_act(p->dtype, p->act, [&](auto z, auto act) {
         using T = decltype(z);
         constexpr int A = decltype(act)::value;
@@ -455,6 +533,11 @@ int gated_mlp_fwd(const ss2d_gated_mlp_params* p, cudaStream_t st) {
             if (tc_fits(*p) && aligned_to(p->y, 16)) return tc_forward<T, A>(*p, st);
         return plain_forward<T, A>(*p, st);
     });
+}
+
+long long gated_mlp_workspace_bytes(const ss2d_gated_mlp_params* p) {
+    if (!p || check_common(*p) != SS2D_OK) return -1;
+    return fwd_workspace(*p);
 }
 
 long long gated_mlp_bwd_workspace_bytes(const ss2d_gated_mlp_bwd_params* p) {

@@ -25,6 +25,9 @@ static Fed mlp_fwd(const Tensor& x, const Tensor& w1, const Tensor& w2, const Te
     r.y = at::empty({p.tokens, p.outputs}, x.options());
     r.h = at::empty({p.tokens, p.hidden}, x.options());
     p.b1 = ptr(b1); p.b2 = ptr(b2); p.h = r.h.data_ptr(); p.y = r.y.data_ptr();
+    const int64_t need = ss2d_gated_mlp_workspace_bytes(&p);
+    Tensor ws;
+    if (need > 0) { ws = bytes(need, x); p.workspace = ws.data_ptr(); p.workspace_bytes = need; }
     check(ss2d_gated_mlp_fwd(&p, stream_of(x)), "ss2d_gated_mlp_fwd");
     return r;
 }

@@ -11,8 +11,8 @@
 // contractions for a tile, x . w1 for value and gate and dy . w2 for the gradient of the hidden map, and forms the gradients of value and gate from the
 // three: they are computed again instead of kept, 4 more operations per weight and token in place of 16 bytes written and read per hidden element.
 //
-// What bounds the large ones is the way of the operands from L2 to the SMs, about 40 bytes a cycle and SM with all of them reading: a tile of 128 x 128 spends
-// 32 KB on a step that takes the tensor core 128 cycles.  Pairs of CTAs (kPair) share a tile of 256 rows, each with its own half of A's rows and of
+// What bounds them is the way of the operands into an SM, some 50 bytes a cycle however few of them read: a tile of 128 x 128 needs 32 KB for a step (64 of the
+// contraction) that takes the tensor core 256 cycles, and gets them in 650.  Pairs of CTAs (kPair) share a tile of 256 rows, each with its own half of A's rows and of
 // B's: 32 KB for 128 x 256 results, in place of 48.
 //
 // Every wait is bounded; one that runs out raises the device's error flag (tc05.cuh), all roles leave and the TMEM is freed.
@@ -43,7 +43,8 @@ template <int EPI, int kCols, bool kPair> struct Shape {
     static constexpr int kB = EPI == EPI_GRAD ? 2 * kOut : kCols;                                        // rows of B of the (first) contraction
     static constexpr int kShare = kPair ? 2 : 1;                                                         // CTAs among which they are divided
     static constexpr int kABytes = kRows * kDepth * 2, kStage = kABytes + kB / kShare * kDepth * 2;
-    static constexpr int kBufs = kCols <= 256 ? 2 : 1;                                                   // tiles in TMEM
+    // tiles in TMEM; of EPI_GRAD one tile's value and gate, and two tiles' hidden gradient, which the MMAs fill while the epilogue still reads the other two
+    static constexpr int kBufs = kCols <= 256 ? 2 : 1;
     static constexpr int kOuts = EPI == EPI_GRAD ? 2 : 1;                                                // blocks of 32 rows that a warp stores at once
     static constexpr int kHalves = kOuts == 1 && kOut >= 128 ? 2 : 1;                                    // one is filled while the other is read
     static constexpr int kWarpStaging = kOuts * kHalves * 4096, kStaging = kEpiWarps * kWarpStaging;
@@ -54,6 +55,7 @@ template <int EPI, int kCols, bool kPair> struct Shape {
     static constexpr int kPitch = kTmem / kBufs;
     static constexpr int kBars = kStages * kStage + kStaging, kBiasAt = kBars + 256;
     static constexpr size_t kBytes = kBiasAt + kBias + 1024;
+    static_assert((EPI == EPI_GRAD) == (kBufs == 1) && (EPI != EPI_GRAD || kCols + kOut <= kTmem));
     static_assert(kCols <= kPitch && kOut % 64 == 0 && kStages >= 3 && (kB / kShare) % 64 == 0);
     static_assert(kBufs == 2 || kOut == 128, "with one tile in TMEM the two groups of epilogue warps have 64 columns each");
 };
@@ -124,6 +126,17 @@ product_tc05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             constexpr int kHalf = S::kB / S::kShare;     // rows of B in this CTA
             for (int i = walker; ok && i < tiles; i += walkers) {
                 const Tile t = tile_at(i);
+                if constexpr (EPI == EPI_GRAD) {
+                    constexpr int kHalf2 = S::kOut / S::kShare;
+                    for (int k = 0; ok && k < a.blocks2; ++k) {
+                        unsigned char* st = slot(S::kABytes + kHalf2 * 128);
+                        if (!ok) break;
+                        load(st, &tmA2, k * kDepth, t.m0);
+#pragma unroll
+                        for (int j = 0; j < kHalf2 / 64; ++j) load(st + S::kABytes + j * 8192, &tmB2, t.n0 + rank * kHalf2 + 64 * j, k * kDepth);
+                        next();
+                    }
+                }
                 for (int k = t.k0; k < t.k1; ++k) {
                     unsigned char* st = slot(S::kStage);
                     if (!ok) break;
@@ -143,17 +156,6 @@ product_tc05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                     } else
                         load(b, &tmB, k0, t.n0 + rank * kHalf);
                     next();
-                }
-                if constexpr (EPI == EPI_GRAD) {
-                    constexpr int kHalf2 = S::kOut / S::kShare;
-                    for (int k = 0; ok && k < a.blocks2; ++k) {
-                        unsigned char* st = slot(S::kABytes + kHalf2 * 128);
-                        if (!ok) break;
-                        load(st, &tmA2, k * kDepth, t.m0);
-#pragma unroll
-                        for (int j = 0; j < kHalf2 / 64; ++j) load(st + S::kABytes + j * 8192, &tmB2, t.n0 + rank * kHalf2 + 64 * j, k * kDepth);
-                        next();
-                    }
                 }
             }
             // what is in flight has been read, and the other CTA's last arrivals are here, before this one leaves
@@ -186,9 +188,20 @@ product_tc05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             for (int i = walker; ok && i < tiles; i += walkers, ++it) {
                 const Tile t = tile_at(i);
                 const int buf = it % NB;
-                if (it >= NB && !mbar_wait_prompt(acc_empty + buf, (it / NB - 1) & 1, abort_flag)) break;
-                tc_fence_after();
                 const uint32_t acc = tmem + buf * S::kPitch;
+                if constexpr (kDual)           // (the epilogue of two tiles ago has left this half: the wait below was for it, a tile ago)
+                    for (int k = 0; ok && k < a.blocks2; ++k) {
+                        if (!mbar_wait_prompt(full + s, round & 1, abort_flag)) { ok = false; break; }
+                        tc_fence_after();
+                        const uint64_t off = (uint64_t)((uint32_t)(s * S::kStage) >> 4);
+#pragma unroll
+                        for (int j = 0; j < kDepth / 16; ++j)
+                            mma(acc + S::kB + (it & 1) * S::kOut, da0 + off + j * stepA, db2 + off + j * (2048 >> 4), idesc2, k > 0 || j > 0 ? 1u : 0u);
+                        commit(empty + s);
+                        if (++s == NS) { s = 0; ++round; }
+                    }
+                if (!ok || (it >= NB && !mbar_wait_prompt(acc_empty + buf, (it / NB - 1) & 1, abort_flag))) break;
+                tc_fence_after();
                 for (int k = t.k0; k < t.k1; ++k) {
                     if (!mbar_wait_prompt(full + s, round & 1, abort_flag)) { ok = false; break; }
                     tc_fence_after();
@@ -198,16 +211,6 @@ product_tc05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                     commit(empty + s);
                     if (++s == NS) { s = 0; ++round; }
                 }
-                if constexpr (kDual)
-                    for (int k = 0; ok && k < a.blocks2; ++k) {
-                        if (!mbar_wait_prompt(full + s, round & 1, abort_flag)) { ok = false; break; }
-                        tc_fence_after();
-                        const uint64_t off = (uint64_t)((uint32_t)(s * S::kStage) >> 4);
-#pragma unroll
-                        for (int j = 0; j < kDepth / 16; ++j) mma(acc + S::kB, da0 + off + j * stepA, db2 + off + j * (2048 >> 4), idesc2, k > 0 || j > 0 ? 1u : 0u);
-                        commit(empty + s);
-                        if (++s == NS) { s = 0; ++round; }
-                    }
                 if (ok) commit(acc_full + buf);
             }
         }
@@ -282,7 +285,7 @@ product_tc05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                     uint32_t r[2][kIn][16];
                     auto load = [&](int q) {
 #pragma unroll
-                        for (int j = 0; j < kIn; ++j) tmem_ld16(lane_base + j * S::kOut + c + 16 * q, r[q & 1][j]);
+                        for (int j = 0; j < kIn; ++j) tmem_ld16(lane_base + (j == 2 ? 2 + (it & 1) : j) * S::kOut + c + 16 * q, r[q & 1][j]);
                     };
                     ready();
                     load(0);
@@ -385,20 +388,21 @@ template <typename T, bool kAMN, bool kBMN, int EPI, int ACT, int kCols, bool kP
     using S = Shape<EPI, kCols, kPair>;
     constexpr bool kDual = EPI == EPI_GATE || EPI == EPI_GRAD;
     constexpr auto sw = CU_TENSOR_MAP_SWIZZLE_128B;
+    constexpr auto l2 = CU_TENSOR_MAP_L2_PROMOTION_L2_256B;       // 5 % faster than 128 bytes: a row's next 64 elements are the next stage's
     // (in front of the maps: a thread that has made no runtime call yet, one of autograd's for instance, has no context for the driver to encode in)
     int* host_flag = error_flag_for_current_device();
     if (!host_flag || *host_flag) return SS2D_ECUDA;                            // no flag, or an earlier launch on this device gave up on a wait
     int* dev_flag = nullptr;
     if (cudaHostGetDevicePointer((void**)&dev_flag, host_flag, 0) != cudaSuccess) return SS2D_ECUDA;
     CUtensorMap ta, tb, ta2, tb2, to, to2;
-    bool ok = kAMN ? make_map_pitched(&ta, Fmt<T>::tm, p.a.p, p.K, p.M, p.a.pitch, kDepth, 64, sw)
-                   : make_map_pitched(&ta, Fmt<T>::tm, p.a.p, p.M, p.K, p.a.pitch, kRows, kDepth, sw);
-    ok = ok && (kBMN && !kDual ? make_map_pitched(&tb, Fmt<T>::tm, p.b.p, p.K, p.N, p.b.pitch, kDepth, 64, sw)
-                               : make_map_pitched(&tb, Fmt<T>::tm, p.b.p, p.b_rows, p.K, p.b.pitch, kDual ? S::kOut : S::kB / S::kShare, kDepth, sw));
+    bool ok = kAMN ? make_map_pitched(&ta, Fmt<T>::tm, p.a.p, p.K, p.M, p.a.pitch, kDepth, 64, sw, l2)
+                   : make_map_pitched(&ta, Fmt<T>::tm, p.a.p, p.M, p.K, p.a.pitch, kRows, kDepth, sw, l2);
+    ok = ok && (kBMN && !kDual ? make_map_pitched(&tb, Fmt<T>::tm, p.b.p, p.K, p.N, p.b.pitch, kDepth, 64, sw, l2)
+                               : make_map_pitched(&tb, Fmt<T>::tm, p.b.p, p.b_rows, p.K, p.b.pitch, kDual ? S::kOut : S::kB / S::kShare, kDepth, sw, l2));
     ta2 = ta; tb2 = tb;
     if constexpr (EPI == EPI_GRAD)
-        ok = ok && make_map_pitched(&ta2, Fmt<T>::tm, p.a2.p, p.M, p.K2, p.a2.pitch, kRows, kDepth, sw) &&
-             make_map_pitched(&tb2, Fmt<T>::tm, p.b2.p, p.K2, p.N, p.b2.pitch, kDepth, 64, sw);
+        ok = ok && make_map_pitched(&ta2, Fmt<T>::tm, p.a2.p, p.M, p.K2, p.a2.pitch, kRows, kDepth, sw, l2) &&
+             make_map_pitched(&tb2, Fmt<T>::tm, p.b2.p, p.K2, p.N, p.b2.pitch, kDepth, 64, sw, l2);
     if constexpr (EPI == EPI_PART) ok = ok && make_out_map<float>(&to, p.out, p.splits, p.M, p.N, p.out_pitch);
     else ok = ok && make_out_map<T>(&to, p.out, 1, p.M, p.N, p.out_pitch);
     to2 = to;

@@ -208,7 +208,7 @@ inline bool make_map(CUtensorMap* m, CUtensorMapDataType dt, const void* base, l
 
 // The same for rows `pitch` elements apart (pitch >= cols, a multiple of 8 elements)
 inline bool make_map_pitched(CUtensorMap* m, CUtensorMapDataType dt, const void* base, long long rows, long long cols, long long pitch,
-                             int box_rows, int box_cols, CUtensorMapSwizzle sw) {
+                             int box_rows, int box_cols, CUtensorMapSwizzle sw, CUtensorMapL2promotion l2 = CU_TENSOR_MAP_L2_PROMOTION_L2_128B) {
     EncodeFn enc = encode_fn();
     if (!enc) return false;
     const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
@@ -216,7 +216,7 @@ inline bool make_map_pitched(CUtensorMap* m, CUtensorMapDataType dt, const void*
     const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
     const cuuint32_t estr[2] = {1, 1};
     return enc(m, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
-               CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+               l2, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 inline int* error_flag_for_current_device() {
