@@ -506,7 +506,8 @@ int ss2d_planes_to_pixels(const ss2d_relayout_params *p, void *cuda_stream);
  * to be <= 0.  out: (batch, seqlen, heads, dv) of `dtype`, dense; initial_state, final_state: (batch, heads, dk, dv) fp32, dense, NULL where
  * there is none.  chunk_states: NULL, or ss2d_linear_attention_states_bytes() bytes, 16-byte aligned: the state in front of every 64th token, in the
  * layout that the backward call reads.  dk and dv up to 128 (else SS2D_ENOTSUP).  A value that is not finite may reach every output of its 64 tokens, also those in front
- * of it.  workspace: ss2d_linear_attention_workspace_bytes() bytes, 16-byte aligned (0: none).  dense tensors are aligned to two elements (fp32 ones to 8 bytes).
+ * of it.  workspace:
+ * ss2d_linear_attention_workspace_bytes() bytes, 16-byte aligned (0: none), a size of the shape and of whether chunk_states are asked for.  dense tensors are aligned to two elements (fp32 ones to 8 bytes).
  * No atomics: repeated calls give bit-identical results.
  * -------------------------------------------------------------------------------- */
 typedef struct ss2d_linear_attention_params {

@@ -749,6 +749,16 @@ __global__ void __launch_bounds__(kStepThreads) la_step_kernel(const StepArgs a)
     }
 }
 
+}  // namespace
+
+}  // namespace ss2d
+
+#include "linear_attention_tc.cuh"
+
+namespace ss2d {
+
+namespace {
+
 // ---- host --------------------------------------------------------------------------------------------------------------
 constexpr int kMostWidth = 128;
 
@@ -851,6 +861,67 @@ WalkArgs walk_args(const ss2d_linear_attention_params& p) {
     return a;
 }
 
+// ---- long bf16 sequences on the tensor cores of linear_attention_tc.cuh ---------------------------------------------------
+// by the shape: the workspace follows it
+constexpr int kLongChunks = 4;
+bool tc_shape(const ss2d_linear_attention_params& p) {
+    return p.dtype == SS2D_BF16 && p.dk % 8 == 0 && p.dv % 8 == 0 && chunks_of(p) >= kLongChunks && p.batch * p.heads <= 0x7fffffffLL / chunks_of(p);
+}
+// by strides and alignment: rows that TMA can read
+bool tc_rows(const Rows& r, long long B, long long L, long long H) {
+    return r.vec && (B == 1 || r.b > 0) && (L == 1 || r.l > 0) && (H == 1 || r.h > 0) && r.b < 1LL << 38 && r.l < 1LL << 38 && r.h < 1LL << 38;
+}
+struct TcPlan { long long chunks, decay, added, states, total; };
+TcPlan tc_plan(const ss2d_linear_attention_params& p, bool train) {
+    TcPlan t = {};
+    if (!tc_shape(p)) return t;
+    auto up = [](long long n) { return (n + 255) / 256 * 256; };
+    const long long bh = p.batch * p.heads, size = p.dk * state_row((int)p.dv);
+    t.chunks = train ? chunks_of(p) : (p.seqlen + lat::kTile - 1) / lat::kTile;
+    t.decay = up(4 * bh * t.chunks);
+    t.added = up(4 * bh * t.chunks * size);
+    t.states = train ? 0 : up(2 * bh * t.chunks * size);
+    t.total = t.decay + t.added + t.states;
+    return t;
+}
+template <typename F> int for_tc(const ss2d_linear_attention_params& p, F&& f) {
+    auto with = [&](auto dk) {
+        return p.dv <= 64 ? f(dk, std::integral_constant<int, 64>()) : f(dk, std::integral_constant<int, 128>());
+    };
+    return p.dk <= 64 ? with(std::integral_constant<int, 64>()) : with(std::integral_constant<int, 128>());
+}
+// the states in front of all chunks (backwards: the gradients behind them), `k` and `v` as in WalkArgs
+template <bool kBack> int tc_states(const ss2d_linear_attention_params& p, const WalkArgs& w, const TcPlan& plan, bool train, const float* first, float* last, void* states,
+                                    char* ws, cudaStream_t st) {
+    float* const added = (float*)(ws + plan.decay);
+    lat::GatherArgs g = {w.g, w.g_b, w.g_l, w.g_h, (float*)ws, w.H, w.rep, w.L, w.dk, w.dv, (int)plan.chunks, w.scale, nullptr};
+    const int rc = for_tc(p, [&](auto dk, auto dv) {
+        constexpr int DK = decltype(dk)::value, DV = decltype(dv)::value;
+        if constexpr (!kBack)
+            if (!train) return lat::gather<DK, DV, lat::kTile, false>(w.k, w.v, added, p.batch, p.n_groups, g, st);
+        return lat::gather<DK, DV, kChunk, kBack>(w.k, w.v, added, p.batch, p.n_groups, g, st);
+    });
+    if (rc != SS2D_OK) return rc;
+    return lat::spread({added, g.decay, first, last, (__nv_bfloat16*)states, g.chunks, w.dk, w.dv, state_row(w.dv), train ? 2 : 1, kBack}, p.batch * p.heads, st);
+}
+int tc_forward(const ss2d_linear_attention_params& p, const WalkArgs& w, cudaStream_t st) {
+    const bool train = p.chunk_states != nullptr;
+    const TcPlan plan = tc_plan(p, train);
+    char* const ws = (char*)p.workspace;
+    void* const states = train ? p.chunk_states : ws + plan.decay + plan.added;
+    if (const int rc = tc_states<false>(p, w, plan, train, (const float*)p.initial_state, (float*)p.final_state, states, ws, st)) return rc;
+    lat::OutArgs o = {w.g, w.g_b, w.g_l, w.g_h, w.H, w.rep, w.L, w.dk, w.dv, (int)((p.seqlen + lat::kTile - 1) / lat::kTile), (int)plan.chunks,
+                      train ? lat::kTile / kChunk : 1, w.scale, nullptr};
+    const Rows out = rows_of(p.out, p.seqlen * p.heads * p.dv, p.heads * p.dv, p.dv, p.dtype);
+    return for_tc(p, [&](auto dk, auto dv) {
+        return lat::outputs<decltype(dk)::value, decltype(dv)::value>(w.q, w.k, w.v, out, states, (train ? 4LL : 2LL) * w.dk * state_row(w.dv), p.batch, p.n_groups, o, st);
+    });
+}
+long long fwd_workspace(const ss2d_linear_attention_params& p) {
+    const long long walk = segment_bytes(p), tc = tc_plan(p, p.chunk_states != nullptr).total;
+    return walk > tc ? walk : tc;
+}
+
 }  // namespace
 
 long long linear_attention_states_bytes(const ss2d_linear_attention_params* p) {
@@ -860,7 +931,7 @@ long long linear_attention_states_bytes(const ss2d_linear_attention_params* p) {
 
 long long linear_attention_workspace_bytes(const ss2d_linear_attention_params* p) {
     if (!p || check_common(*p) != SS2D_OK) return -1;
-    return segment_bytes(*p);
+    return fwd_workspace(*p);
 }
 
 int linear_attention_fwd(const ss2d_linear_attention_params* p, cudaStream_t st) {
@@ -869,7 +940,7 @@ int linear_attention_fwd(const ss2d_linear_attention_params* p, cudaStream_t st)
     if (!p->out) return SS2D_EINVAL_NULL;
     if (!aligned_to(p->out, 2 * dtype_size(p->dtype)) || !aligned_to(p->initial_state, 4) || !aligned_to(p->final_state, 8) || !aligned_to(p->chunk_states, 16))
         return SS2D_EINVAL_ALIGN;
-    const long long need = segment_bytes(*p), bh = p->batch * p->heads;
+    const long long need = fwd_workspace(*p), bh = p->batch * p->heads;
     if (need && (!p->workspace || p->workspace_bytes < need || !aligned_to(p->workspace, 16))) return SS2D_EWORKSPACE;
     WalkArgs a = walk_args(*p);
     a.q = rows_of(p->q, p->q_batch_stride, p->q_token_stride, p->q_head_stride, p->dtype);
@@ -877,6 +948,9 @@ int linear_attention_fwd(const ss2d_linear_attention_params* p, cudaStream_t st)
     a.v = rows_of(p->v, p->v_batch_stride, p->v_token_stride, p->v_head_stride, p->dtype);
     a.o = p->out;
     a.states = p->chunk_states;
+    if (tc_shape(*p) && aligned_to(p->out, 16) && tc_rows(a.q, p->batch, p->seqlen, p->n_groups) && tc_rows(a.k, p->batch, p->seqlen, p->n_groups) &&
+        tc_rows(a.v, p->batch, p->seqlen, p->heads))
+        return tc_forward(*p, a, st);
     return for_type(p->dtype, [&](auto z) {
         return for_dk(p->dk, [&](auto n) {
             using T = decltype(z);
@@ -894,7 +968,8 @@ namespace {
 struct BwdPlan { long long segments, dstates, total; };
 BwdPlan bwd_plan(const ss2d_linear_attention_params& p) {
     BwdPlan b = {};
-    b.segments = (segment_bytes(p) + 255) / 256 * 256;
+    const long long walk = (segment_bytes(p) + 255) / 256 * 256, tc = tc_plan(p, true).total;
+    b.segments = walk > tc ? walk : tc;
     b.dstates = states_bytes(p);
     b.total = b.segments + b.dstates;
     return b;
@@ -942,19 +1017,22 @@ int linear_attention_bwd(const ss2d_linear_attention_bwd_params* p, cudaStream_t
     a.dq = p->dq; a.dk_ = p->dk; a.dv_ = p->dv; a.dg = (float*)p->dlog_decay;
     a.G = (int)f.n_groups; a.rep = w.rep; a.L = w.L; a.dk = w.dk; a.dv = w.dv; a.chunks = w.chunks; a.scale = f.scale;
     a.pairs_k = a.dk % 2 == 0; a.pairs_v = a.dv % 2 == 0;
+    const float* first = (const float*)p->dfinal_state;
+    float* last = (float*)p->dinitial_state;
+    const bool tc = tc_shape(f) && tc_rows(w.k, f.batch, f.seqlen, f.n_groups) && tc_rows(w.v, f.batch, f.seqlen, f.heads);
+    if (tc)
+        if (const int rc = tc_states<true>(f, w, tc_plan(f, true), true, first, last, dstates, ws, st)) return rc;
     return for_type(f.dtype, [&](auto z) {
         using T = decltype(z);
         return for_dk(f.dk, [&](auto n) {
             constexpr int DK = decltype(n)::value;
-            const float* first = (const float*)p->dfinal_state;
-            float* last = (float*)p->dinitial_state;
             int rc = SS2D_OK;
             bool wide = false;
             if constexpr (sizeof(T) == 2 || DK <= 64) {
                 wide = slice_of(f) == 64;
-                if (wide) rc = walk<T, DK, 64, false, true>(w, first, last, ws, bh, st);
+                if (wide && !tc) rc = walk<T, DK, 64, false, true>(w, first, last, ws, bh, st);
             }
-            if (!wide) rc = walk<T, DK, 32, false, true>(w, first, last, ws, bh, st);
+            if (!wide && !tc) rc = walk<T, DK, 32, false, true>(w, first, last, ws, bh, st);
             if (rc != SS2D_OK) return rc;
             const long long groups = f.batch * f.n_groups;
             return f.dv <= 32 ? launch_grad<T, DK, 32>(a, groups, st) : f.dv <= 64 ? launch_grad<T, DK, 64>(a, groups, st) : launch_grad<T, DK, 128>(a, groups, st);
