@@ -276,18 +276,20 @@ struct OutArgs {
     float scale;
     int* error_flag;
 };
+// The pairs take the place of the keys, v that of the queries, once these have been read; with both sides of 64 v has its own place, the products with the state wait
+// for the pairs to have left TMEM and take half their columns: 96 to 128 KB and 256 columns become 96 KB and 256, or 72 KB and 128, and two or three CTAs share an SM.
 template <int DK, int DV> struct OutSmem {
+    static constexpr bool kSmall = DK == 64 && DV == 64;
     static constexpr int kBlock = kTile * 128;
-    static constexpr int kQ = 0, kK = kQ + DK / 64 * kBlock, kV = kK + DK / 64 * kBlock, kS = kV + DV / 64 * kBlock, kP = kS + DV / 64 * DK * 128;
-    static constexpr int kEnd = kP + 2 * kBlock;
-    static constexpr int kTx1 = 2 * DK / 64 * kBlock, kTx2 = DV / 64 * (kBlock + DK * 128);
+    static constexpr int kQ = 0, kV = kSmall ? kBlock : 0, kP = kV + (DV > DK ? DV : DK) / 64 * kBlock, kK = kP, kS = kP + 2 * kBlock;
+    static constexpr int kEnd = kS + DV / 64 * DK * 128;
     static constexpr int kFloats = 4 * kTile + 4 * kTile;               // n, f, e, near; far of four blocks of 32 tokens
     static constexpr size_t kBytes = kEnd + kFloats * 4 + 64 + 1024;
-    static constexpr int kTmem = 256;                                   // pairs, and in their place their products with v; products with the state
+    static constexpr int kTmem = kSmall ? 128 : 256, kAcross = kSmall ? 64 : 128;   // pairs, and in their place their products with v; products with the state
 };
 
 template <int DK, int DV>
-__global__ void __launch_bounds__(kThreads) la_outputs_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+__global__ void __launch_bounds__(kThreads, DK == 64 && DV == 64 ? 3 : 2) la_outputs_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                                                               const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmS,
                                                               const __grid_constant__ CUtensorMap tmO, const OutArgs a) {
     follow_previous();
@@ -295,26 +297,27 @@ __global__ void __launch_bounds__(kThreads) la_outputs_kernel(const __grid_const
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* const sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     float *const dn = reinterpret_cast<float*>(sm + M::kEnd), *const df = dn + kTile, *const de = df + kTile, *const near = de + kTile, *const far = near + kTile;
-    uint64_t* const bars = reinterpret_cast<uint64_t*>(far + 4 * kTile);            // q and k, v and states, first products, last ones
-    uint32_t* const slot = reinterpret_cast<uint32_t*>(bars + 4);
+    uint64_t* const bars = reinterpret_cast<uint64_t*>(far + 4 * kTile);            // q and k, states, first products, last ones, v
+    uint32_t* const slot = reinterpret_cast<uint32_t*>(bars + 5);
     volatile int* const abort_flag = reinterpret_cast<volatile int*>(slot + 1);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int c = blockIdx.x % a.tiles, bh = blockIdx.x / a.tiles, b = bh / a.H, h = bh % a.H, first = c * kTile;
     if (tid == 0) {
-        for (int i = 0; i < 4; ++i) mbar_init(bars + i, 1);
+        for (int i = 0; i < 5; ++i) mbar_init(bars + i, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        mbar_expect_tx(bars, M::kTx1);
+        mbar_expect_tx(bars, 2 * DK / 64 * M::kBlock);
 #pragma unroll
         for (int i = 0; i < DK / 64; ++i) {
             tma_load_4d(sm + M::kQ + i * M::kBlock, &tmQ, 64 * i, first, h / a.rep, b, bars);
             tma_load_4d(sm + M::kK + i * M::kBlock, &tmK, 64 * i, first, h / a.rep, b, bars);
         }
-        mbar_expect_tx(bars + 1, M::kTx2);
+        mbar_expect_tx(bars + 1, DV / 64 * (DK * 128));
 #pragma unroll
-        for (int i = 0; i < DV / 64; ++i) {
-            tma_load_4d(sm + M::kV + i * M::kBlock, &tmV, 64 * i, first, h, b, bars + 1);
-            tma_load_3d(sm + M::kS + i * DK * 128, &tmS, 64 * i, 0, bh * a.states + c * a.step, bars + 1);
+        for (int i = 0; i < DV / 64; ++i) tma_load_3d(sm + M::kS + i * DK * 128, &tmS, 64 * i, 0, bh * a.states + c * a.step, bars + 1);
+        if constexpr (M::kSmall) {
+            mbar_expect_tx(bars + 4, M::kBlock);
+            tma_load_4d(sm + M::kV, &tmV, 0, first, h, b, bars + 4);
         }
     }
     if (warp == 1) { tmem_alloc(slot, M::kTmem); tmem_relinquish(); }
@@ -326,26 +329,29 @@ __global__ void __launch_bounds__(kThreads) la_outputs_kernel(const __grid_const
     const uint32_t tmem = *slot;
     const uint32_t base = smem_u32(sm);
     bool ok = true;
+    auto with_states = [&] {                                                        // queries times the state in front
+        constexpr uint32_t idesc = instr_desc(1, false, 128, DV) | (1u << 16);
+        const uint64_t q = smem_desc(base + M::kQ, 16, 1024, kSw128), s = smem_desc(base + M::kS, DK * 128, 1024, kSw128);
+        if (!mbar_wait_prompt(bars + 1, 0, abort_flag)) return false;
+        tc_fence_after();
+#pragma unroll
+        for (int i = 0; i < DK / 16; ++i)
+            tc_mma(tmem + M::kAcross, q + ((uint64_t)(i / 4 * M::kBlock + i % 4 * 32) >> 4), s + i * 128, idesc, i > 0);
+        return true;
+    };
     if (tid == 0) {
-        constexpr uint32_t pairs = instr_desc(1, false, 128, 128), states = instr_desc(1, false, 128, DV) | (1u << 16);
+        constexpr uint32_t idesc = instr_desc(1, false, 128, 128);
         const uint64_t q = smem_desc(base + M::kQ, 16, 1024, kSw128), k = smem_desc(base + M::kK, 16, 1024, kSw128);
-        const uint64_t s = smem_desc(base + M::kS, DK * 128, 1024, kSw128);
         ok = mbar_wait_prompt(bars, 0, abort_flag);
         if (ok) {
             tc_fence_after();
 #pragma unroll
             for (int i = 0; i < DK / 16; ++i) {
                 const uint64_t off = (uint64_t)(i / 4 * M::kBlock + i % 4 * 32) >> 4;
-                tc_mma(tmem, q + off, k + off, pairs, i > 0);
+                tc_mma(tmem, q + off, k + off, idesc, i > 0);
             }
-            ok = mbar_wait_prompt(bars + 1, 0, abort_flag);
-        }
-        if (ok) {
-            tc_fence_after();
-#pragma unroll
-            for (int i = 0; i < DK / 16; ++i)
-                tc_mma(tmem + 128, q + ((uint64_t)(i / 4 * M::kBlock + i % 4 * 32) >> 4), s + i * 128, states, i > 0);
-            tc_commit(bars + 2);
+            if constexpr (!M::kSmall) ok = with_states();
+            if (ok) tc_commit(bars + 2);
         }
     }
     // pairs of different blocks of 32 tokens: one exponential a token (as in the walk)
@@ -357,6 +363,12 @@ __global__ void __launch_bounds__(kThreads) la_outputs_kernel(const __grid_const
     }
     __syncthreads();
     ok = ok && mbar_wait_prompt(bars + 2, 0, abort_flag);
+    if constexpr (!M::kSmall)
+        if (tid == 0 && ok) {                                                       // the queries have been read
+            mbar_expect_tx(bars + 4, DV / 64 * M::kBlock);
+#pragma unroll
+            for (int i = 0; i < DV / 64; ++i) tma_load_4d(sm + M::kV + i * M::kBlock, &tmV, 64 * i, first, h, b, bars + 4);
+        }
     __syncwarp();
     tc_fence_after();
     const int quarter = warp & 3, row = 32 * quarter + lane;
@@ -399,9 +411,14 @@ __global__ void __launch_bounds__(kThreads) la_outputs_kernel(const __grid_const
         tc_fence_after();
         constexpr uint32_t idesc = instr_desc(1, false, 128, DV) | (1u << 16);
         const uint64_t p = smem_desc(base + M::kP, 16, 1024, kSw128), v = smem_desc(base + M::kV, M::kBlock, 1024, kSw128);
+        if constexpr (M::kSmall) ok = with_states();
+        ok = ok && mbar_wait_prompt(bars + 4, 0, abort_flag);
+        if (ok) {
+            tc_fence_after();
 #pragma unroll
-        for (int i = 0; i < kTile / 16; ++i) tc_mma(tmem, p + ((uint64_t)(i / 4 * M::kBlock + i % 4 * 32) >> 4), v + i * 128, idesc, i > 0);
-        tc_commit(bars + 3);
+            for (int i = 0; i < kTile / 16; ++i) tc_mma(tmem, p + ((uint64_t)(i / 4 * M::kBlock + i % 4 * 32) >> 4), v + i * 128, idesc, i > 0);
+            tc_commit(bars + 3);
+        }
     }
     ok = ok && mbar_wait_prompt(bars + 3, 0, abort_flag);
     __syncwarp();
@@ -416,7 +433,7 @@ __global__ void __launch_bounds__(kThreads) la_outputs_kernel(const __grid_const
             const int col = half * (DV / 2) + q;
             uint32_t x[16], y[16], w[8];
             tmem_ld16(lane_base + col, x);
-            tmem_ld16(lane_base + 128 + col, y);
+            tmem_ld16(lane_base + M::kAcross + col, y);
             tmem_ld_wait();
 #pragma unroll
             for (int j = 0; j < 8; ++j)
