@@ -234,6 +234,39 @@ def test_same_bits_streams_graphs_autocast(vb, M):
         assert all(torch.equal(now[n], got[n]) for n in now)
 
 
+def test_first_call_in_a_capture():
+    """A process whose first call on the device is captured, for inference and for training (the backward pass runs on a thread of autograd's)."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch, vmamba_b200 as vb
+mk = lambda *s: (torch.randn(s, device="cuda") / s[-1] ** 0.5).bfloat16()
+x, w1, w2, q = mk(300, 64), mk(256, 64), mk(64, 128), mk(1, 600, 2, 128)
+g = torch.zeros(1, 600, 2, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.no_grad(), torch.cuda.graph(graph):
+    y, o = vb.gated_mlp_fn(x, w1, w2), vb.linear_attention_fn(q, q, q, g)
+graph.replay()
+leaves = [t.clone().requires_grad_() for t in (x, w1, w2, q)]
+torch.cuda.synchronize()
+train = torch.cuda.CUDAGraph()
+with torch.cuda.graph(train):
+    got = torch.autograd.grad(vb.gated_mlp_fn(*leaves[:3]).sum() + vb.linear_attention_fn(leaves[3], leaves[3], leaves[3], g).sum(), leaves)
+train.replay()
+torch.cuda.synchronize()
+want = torch.autograd.grad(vb.gated_mlp_fn(*leaves[:3]).sum() + vb.linear_attention_fn(leaves[3], leaves[3], leaves[3], g).sum(), leaves)
+with torch.no_grad():
+    assert torch.equal(y, vb.gated_mlp_fn(x, w1, w2)) and torch.equal(o, vb.linear_attention_fn(q, q, q, g))
+assert all(torch.equal(a, b) for a, b in zip(got, want))
+print("same")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
+
+
 def test_refusals(vb):
     t, _ = make(4, 16, 32, 8, torch.bfloat16)
     f = vb.gated_mlp_fn

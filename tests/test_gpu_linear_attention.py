@@ -112,6 +112,39 @@ def test_against_the_recurrence(vb, shape, dtype):
     compare(run(vb, t, up), reference(t, up, scale), reference(t, up, scale, True), dtype, t, scale)
 
 
+LONG = [  # B, L, G, H, dk, dv: long bf16 sequences, the kernels of the 5th-generation tensor cores
+    (1, 193, 1, 1, 128, 128), (2, 257, 1, 3, 72, 128), (1, 320, 2, 2, 128, 40), (1, 519, 1, 2, 64, 64), (2, 640, 2, 4, 40, 56), (1, 831, 1, 1, 8, 72), (3, 385, 1, 2, 96, 96),
+]
+
+
+@pytest.mark.parametrize("shape", LONG, ids=str)
+def test_long_sequences(vb, shape):
+    t, up = make(*shape, torch.bfloat16, decay=0.05)
+    scale = shape[4] ** -0.5
+    compare(run(vb, t, up), reference(t, up, scale), reference(t, up, scale, True), torch.bfloat16, t, scale)
+    with torch.no_grad():                       # without the states that training keeps: chunks of twice as many tokens
+        o, S = vb.linear_attention_fn(*(t[n] for n in NAMES[:4]), None, t["initial_state"], True)
+    ref, mag = reference(t, up, scale), reference(t, up, scale, True)
+    assert ((o - ref[0]).abs() <= HALF[torch.bfloat16] * ref[0].abs() + (2 * FORM[torch.bfloat16] + SUMS) * mag[0]).all()
+    assert ((S - ref[1]).abs() <= (3 * PIECES[torch.bfloat16] + SUMS) * mag[1]).all()
+
+
+def test_long_sequences_whose_rows_no_tile_reads(vb):
+    """Strides of 0 and rows on any element take the walk, with the workspace of the shape."""
+    B, L, H, d = 2, 300, 2, 128
+    t, up = make(B, L, H, H, d, d, torch.bfloat16, decay=0.05)
+    scale = d ** -0.5
+    want = reference(t, up, scale), reference(t, up, scale, True)
+    wide = torch.zeros(B, L, H, d + 3, dtype=torch.bfloat16, device="cuda")
+    wide[..., 1:1 + d] = t["v"]
+    compare(run(vb, {**t, "v": wide[..., 1:1 + d]}, up), *want, torch.bfloat16, t, scale)
+    same = {**t, "k": t["k"][:1].expand(B, L, H, d)}
+    compare(run(vb, same, up), reference(same, up, scale), reference(same, up, scale, True), torch.bfloat16, same, scale)
+    packed = torch.cat([t[n] for n in "qkv"], -1)
+    three = {**t, "q": packed[..., :d], "k": packed[..., d:2 * d], "v": packed[..., 2 * d:]}
+    compare(run(vb, three, up), *want, torch.bfloat16, t, scale)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_resets(vb, dtype):
     """-inf, the type's lowest and merely large negative decays clear the state; a chunk whose decays run to thousands keeps the small ones exact."""
@@ -388,6 +421,17 @@ def test_refusals(vb):
         step(*one, two[:s.numel()].view(s.shape), state_out=two[4:4 + s.numel()].view(s.shape))
     with pytest.raises(RuntimeError, match="no backward"):
         step(*one, s.clone().requires_grad_())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_resets_in_long_sequences(vb, dtype):
+    t, up = make(1, 400, 1, 2, 128, 72, dtype, decay=0.01)
+    g = t["log_decay"]
+    g[0, 31:34], g[0, 127], g[0, 128], g[0, 200:231, 0] = -float("inf"), -3e38, -1e4, -float("inf")
+    ref = reference(t, up, 0.2)
+    got = run(vb, t, up, 0.2)
+    compare(got, ref, reference(t, up, 0.2, True), dtype, t, 0.2)
+    assert (got[5][0, 31:34] == 0).all() and (got[5][0, 127] == 0).all()
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])

@@ -791,9 +791,11 @@ int slice_of(const ss2d_linear_attention_params& p) { return p.dv <= 32 || (p.dt
 // long as all others.  us with 1 / 2 / 3 / 4 / 8 / 12 segments: 16 385 tokens of 16 heads of 128 x 128, forward 1134 / 873 / 587 / 448 / 288 / 349 (9 of them: 257);
 // 2 x 4 096 tokens, training 845 / 713 / 666 / 573 / 586 / 611 (4); 16 x 3 136 tokens of 12 heads of 64 x 32, training 550 / 543 / 488 / 513 / 502 / 505 (3);
 // 16 x 784 tokens of 24 heads, forward 73 / 115 / 113 / 111 (1).
+long long room_of(const ss2d_linear_attention_params& p) {
+    return 148 * (p.dk > 64 ? 2 : 4) / (p.batch * p.heads * ((p.dv + slice_of(p) - 1) / slice_of(p)));
+}
 int segments_of(const ss2d_linear_attention_params& p) {
-    const long long ctas = p.batch * p.heads * ((p.dv + slice_of(p) - 1) / slice_of(p)), chunks = chunks_of(p);
-    const long long room = 148 * (p.dk > 64 ? 2 : 4) / ctas;
+    const long long chunks = chunks_of(p), room = room_of(p);
     if (room < 2 || chunks < 8) return 1;
     const long long seg = room < chunks / 2 ? room : chunks / 2, per = (chunks + seg - 1) / seg;
     return (int)((chunks + per - 1) / per);
@@ -862,10 +864,17 @@ WalkArgs walk_args(const ss2d_linear_attention_params& p) {
 }
 
 // ---- long bf16 sequences on the tensor cores of linear_attention_tc.cuh ---------------------------------------------------
-// by the shape: the workspace follows it
+// By the shape; the workspace follows it.  The walk moves less and is one launch where it need not be cut; these kernels win where a walk would be cut (room for
+// twice its CTAs), and with wide heads from 8 chunks on.  us of the walk / these, forward, then a training step: 4 096 tokens of 16 heads of 128 x 128 79 / 41, 306 / 227,
+// of 64 x 64 36 / 26, 117 / 98, of 64 x 32 25 / 25, 96 / 97; 16 x 3 136 of 12 heads of 128 x 128 482 / 322, 2 329 / 1 948, of 128 x 64 271 / 237, 1 439 / 1 315, of 64 x 64
+// 201 / 160, 760 / 694, of 64 x 32 120 / 141; 16 x 784 of 24 heads of 128 x 64 133 / 135, 766 / 696, of 64 x 64 67 / 95, 345 / 374; 64 x 200 of 8 heads of 128 x 128
+// 92 / 86, 448 / 427, of 128 x 64 49 / 60, 284 / 281.
 constexpr int kLongChunks = 4;
 bool tc_shape(const ss2d_linear_attention_params& p) {
-    return p.dtype == SS2D_BF16 && p.dk % 8 == 0 && p.dv % 8 == 0 && chunks_of(p) >= kLongChunks && p.batch * p.heads <= 0x7fffffffLL / chunks_of(p);
+    const long long chunks = chunks_of(p);
+    if (p.dtype != SS2D_BF16 || p.dk % 8 || p.dv % 8 || chunks < kLongChunks || p.batch * p.heads > 0x7fffffffLL / chunks) return false;
+    if (p.dk > 64 || p.dv > 64) return room_of(p) >= 2 || chunks >= 8 || (p.dk > 64 && p.dv > 64);
+    return p.dk > 32 && p.dv > 32 && room_of(p) >= 2;
 }
 // by strides and alignment: rows that TMA can read
 bool tc_rows(const Rows& r, long long B, long long L, long long H) {

@@ -226,9 +226,14 @@ inline int* error_flag_for_current_device() {
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
     std::lock_guard<std::mutex> lock(mu);
     if (!flags[dev]) {
-        // mapped, pinned host memory: the kernel can raise the flag and the host can read it without a copy
+        // mapped, pinned host memory: the kernel can raise the flag and the host can read it without a copy.  The first call on a device may stand in a
+        // stream capture, which forbids allocations unless the thread says that they are none of the graph's.
         int* h = nullptr;
-        if (cudaHostAlloc((void**)&h, sizeof(int), cudaHostAllocMapped) != cudaSuccess) return nullptr;
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return nullptr;
+        const cudaError_t rc = cudaHostAlloc((void**)&h, sizeof(int), cudaHostAllocMapped);
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (rc != cudaSuccess) return nullptr;
         *h = 0;
         flags[dev] = h;
     }
