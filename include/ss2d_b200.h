@@ -497,7 +497,7 @@ int ss2d_pixels_norm_to_planes(const ss2d_relayout_params *p, void *cuda_stream)
 int ss2d_planes_to_pixels(const ss2d_relayout_params *p, void *cuda_stream);
 
 /* ------------------------------------------------------------------------------------
- * Linear attention with a decay for each head (the scan of the m0 family of SS2D, classification/models/vmamba.py:717-911, in attention's terms:
+ * Linear attention with a decay for each head (the scan of the m0 family of SS2D, classification/models/vmamba.py:915-1104, in attention's terms:
  * C, B and x dt are q, k and v, dt A is log_decay).  For every sequence b and head h, with group h / (heads / n_groups) of q and k:
  *   S_t = exp(log_decay_t) S_{t-1} + k_t v_t^T          S (dk, dv) fp32, S_0 = initial_state or zero
  *   out_t = scale S_t^T q_t
@@ -557,7 +557,7 @@ typedef struct ss2d_linear_attention_step_params {
 int ss2d_linear_attention_step(const ss2d_linear_attention_step_params *p, void *cuda_stream);
 
 /* ------------------------------------------------------------------------------------
- * Gated feed-forward block (gMlp.forward, classification/models/vmamba.py:131-149):
+ * Gated feed-forward block (gMlp.forward, classification/models/vmamba.py:42-149):
  *   [v g] = x w1^T + b1;  h = v * act(g);  y = h w2^T + b2
  * x: (tokens, channels), rows x_row_stride elements apart; w1: (2 hidden, channels), the rows of the values first; w2: (outputs, hidden); b1 (2 hidden) and
  * b2 (outputs) or NULL; y: (tokens, outputs).  All of `dtype`; dense but for x's rows.  act: 1 GELU (erf), 2 SiLU.  h: (tokens, hidden) of `dtype`,

@@ -182,7 +182,7 @@ def linear_attention_fn(q, k, v, log_decay, scale=None, initial_state=None, retu
 
         S_t = exp(log_decay_t) S_{t-1} + k_t v_t^T,    o_t = scale S_t^T q_t
 
-    the scan of the reference's m0 family (classification/models/vmamba.py:717-911: C, B and x dt are q, k and v, dt A is log_decay) and what
+    the scan of the reference's m0 family (classification/models/vmamba.py:915-1104: C, B and x dt are q, k and v, dt A is log_decay) and what
     `selective_scan_fn` computes where all channels of a head share one decay.
 
     q, k: (batch, tokens, groups, dk), v: (batch, tokens, heads, dv), one dtype (float32, float16, bfloat16); heads is a multiple of groups, and heads
@@ -504,7 +504,7 @@ def mlp_fused(x: torch.Tensor, w1: torch.Tensor, b1: torch.Tensor, w2: torch.Ten
 
 
 def gated_mlp_fn(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, b1=None, b2=None, act="gelu") -> torch.Tensor:
-    """Gated feed-forward block, gMlp.forward (classification/models/vmamba.py:131-149) on tokens:
+    """Gated feed-forward block, gMlp.forward (classification/models/vmamba.py:42-149) on tokens:
 
         v, g = (x w1^T + b1).chunk(2, -1);    y = (v * act(g)) w2^T + b2
 
