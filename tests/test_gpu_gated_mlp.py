@@ -325,3 +325,51 @@ def test_block_of_attention_and_feed_forward(vb):
             z = z + o.flatten(-2)
             z = z + vb.gated_mlp_fn(z, w1, w2)
             assert (z - want[:, t]).norm() <= 2.0 ** -13 * want[:, t].norm()
+
+
+# ---- gates one by one -------------------------------------------------------------------------------------------------
+# Half a step for a rounded result.  Activations: 2^-16 of the value beside 16-bit types (the fit of Phi 2^-18, exponents of up to 127 rounded in fp32 2^-17), for fp32
+# CUDA's normcdff (5 steps of 2^-23), one more product and the two tf32 pieces that carry a gradient (2^-22).  What is below 2^-126 may come as zero.
+RELATIVE = {torch.bfloat16: 2.0 ** -16, torch.float16: 2.0 ** -16, torch.float32: 2.0 ** -19}
+
+
+def gates(act, dtype):
+    far = -13.0 if act == "gelu" else -80.0
+    g = torch.cat((torch.linspace(far, 13.0, 2417), torch.linspace(-10.0, -3.0, 700), torch.tensor([s * 2.0 ** -k for s in (1, -1) for k in range(14)]), torch.zeros(3)))
+    return (g.to(dtype) if dtype != torch.float32 else g.bfloat16().float()).cuda()       # few bits: nothing is lost in front of the activation
+
+
+def single_gates(vb, g, act, offset=0):
+    """(act(g), gradient of the value, gradient of the gate) of a block that does nothing else: value 1, unit weights, an upstream gradient for one hidden channel"""
+    M, dtype = g.numel(), g.dtype
+    wide = torch.zeros(M, 16, dtype=dtype, device="cuda")
+    x = wide[:, offset:offset + 8]
+    x[:, 0], x[:, 1] = g, 1
+    x.requires_grad_()
+    w1, dy = torch.zeros(16, 8, dtype=dtype, device="cuda"), torch.zeros(M, 8, dtype=dtype, device="cuda")
+    w1[:8, 1], w1[8:, 0], dy[:, 3] = 1, 1, 1
+    y = vb.gated_mlp_fn(x, w1, torch.eye(8, dtype=dtype, device="cuda"), act=act)
+    dx, = torch.autograd.grad(y, x, dy)
+    assert all(torch.equal(y[:, 0], y[:, j]) for j in range(8))
+    return y[:, 3].detach(), dx[:, 1], dx[:, 0]
+
+
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("kernels", ["many_tokens", "few_tokens", "unaligned"])
+def test_activations_elementwise(vb, kernels, dtype, act):
+    g = gates(act, dtype)
+    per = 13 if kernels == "few_tokens" else g.numel()
+    parts = [single_gates(vb, c, act, offset=1 if kernels == "unaligned" else 0) for c in g.split(per)]
+    got = [torch.cat(p).double() for p in zip(*parts)]
+    z = g.double()
+    a, da = bent(z, act)
+    if act == "gelu":
+        size = 0.5 * torch.erfc(-z / math.sqrt(2)) + z.abs() * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    else:
+        size = torch.sigmoid(z) * (1 + z.abs() * torch.sigmoid(-z))
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 2.0 ** -119
+    for name, x, want, mag in (("value", got[0], a, a.abs()), ("gradient of the value", got[1], a, a.abs()), ("gradient of the gate", got[2], da, size)):
+        worst = ((x - want).abs() / (HALF[dtype] * want.abs() + RELATIVE[dtype] * mag + tiny)).max().item()
+        print(f"{name}: {worst:.3f} of the tolerance")
+        assert worst <= 1, (name, worst)

@@ -50,21 +50,4 @@ __device__ __forceinline__ float2 gelu_pair_poly(float2 v) {
     return __fmul2_rn(v, phi);
 }
 
-// Phi on a pair of values, the same way with two more terms: for activations whose result meets another rounding to fp16, and for derivatives.
-// |v Phi(v) error| <= 3.5e-5 for every v in fp32 arithmetic (fit on |z| <= 3.05, checked on 2 million points up to 12 and, where it saturates, to 1e18).
-__device__ __forceinline__ float2 normal_cdf_pair(float2 v) {
-    const float2 z = __fmul2_rn(v, splat2(0.70710678118654752f));
-    const float2 t = __fmul2_rn(z, z);
-    float2 p = splat2(1.487421731e-08f);
-    p = __ffma2_rn(p, t, splat2(-7.567000110e-07f));
-    p = __ffma2_rn(p, t, splat2(1.701804670e-05f));
-    p = __ffma2_rn(p, t, splat2(-2.248523860e-04f));
-    p = __ffma2_rn(p, t, splat2(1.962875246e-03f));
-    p = __ffma2_rn(p, t, splat2(-1.209753586e-02f));
-    p = __ffma2_rn(p, t, splat2(5.480693100e-02f));
-    p = __ffma2_rn(p, t, splat2(-1.870886549e-01f));
-    p = __ffma2_rn(p, t, splat2(5.639843889e-01f));
-    return make_float2(fma_sat(p.x, z.x, 0.5f), fma_sat(p.y, z.y, 0.5f));
-}
-
 }  // namespace ss2d

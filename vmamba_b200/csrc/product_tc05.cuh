@@ -308,12 +308,12 @@ product_tc05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                                 const float2 g = __fadd2_rn(make_float2(__uint_as_float(x[1][e]), __uint_as_float(x[1][e + 1])),
                                                             *reinterpret_cast<const float2*>(b + kBiasCols + e));
                                 if constexpr (EPI == EPI_GATE) {
-                                    const float2 o = __fmul2_rn(v, act_pair<T, ACT>(g));
+                                    const float2 o = __fmul2_rn(v, act_pair<ACT>(g));
                                     w[j] = Half2Of<T>::pack(o.x, o.y);
                                 } else {
                                     const float2 dh = make_float2(__uint_as_float(x[kIn - 1][e]), __uint_as_float(x[kIn - 1][e + 1]));
                                     float2 act, slope;
-                                    act_grad_pair<T, ACT>(g, act, slope);
+                                    act_grad_pair<ACT>(g, act, slope);
                                     const float2 dv = __fmul2_rn(dh, act), dg = __fmul2_rn(__fmul2_rn(dh, v), slope);
                                     w[j] = Half2Of<T>::pack(dv.x, dv.y);
                                     w2[j] = Half2Of<T>::pack(dg.x, dg.y);
