@@ -447,3 +447,31 @@ def test_long_memory(vb, dtype):
     assert ((S - want).abs() / want).max() <= 2.0 ** -16 + 1024 * 2.0 ** -24 / 3
     # the roundings of the additions are of random sign, those of the products fall off: a chunk's error is at most 24 steps of 2^-24 cut off
     assert (S - want).norm() <= 2.0 ** -18 * want.norm()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_states_side_by_side(vb, dtype):
+    """Two states of a sequence next to one another in one cache, read and written in turn: memory that interleaves without overlapping."""
+    B, G, H, dk, dv = 5, 2, 4, 32, 16
+    t, _ = make(B, 1, G, H, dk, dv, dtype)
+    a = [t[n][:, 0] for n in ("q", "k", "v", "log_decay")]
+    cache = torch.full((B, 3, H, dk, dv), 7.0, device="cuda")
+    cache[:, 1] = t["initial_state"]
+    y, new = vb.linear_attention_step(*a, t["initial_state"])
+    for src, dst in ((1, 0), (1, 2)):
+        y2, s2 = vb.linear_attention_step(*a, cache[:, src], state_out=cache[:, dst])
+        assert torch.equal(y2, y) and torch.equal(cache[:, dst], new) and torch.equal(cache[:, 1], t["initial_state"]) and s2.data_ptr() == cache[:, dst].data_ptr()
+    y3, _ = vb.linear_attention_step(*(x[:1] for x in a), cache[:1, 1], state_out=cache[:1, 0])
+    assert torch.equal(y3, y[:1])
+    size = H * dk * dv
+    flat = cache.view(-1)
+    view = lambda first, stride, n=B: flat.as_strided((n, H, dk, dv), (stride, dk * dv, dv, 1), first)      # noqa: E731
+    for first in (size - 4, size + 4, 3 * size + 4, 5 * size - 4):     # into the state of the same sequence, or of the one behind ([4, 5) size)
+        with pytest.raises(RuntimeError, match="overlap"):
+            vb.linear_attention_step(*(x[:3] for x in a), view(size, 3 * size, 3), state_out=view(first, 3 * size, 3))
+    two = [x[:2] for x in a]
+    with pytest.raises(RuntimeError, match="overlap"):                  # strides that differ: the second state into the third's place
+        vb.linear_attention_step(*two, view(0, 2 * size, 2), state_out=view(size, size, 2))
+    flat[:size], flat[3 * size:4 * size] = t["initial_state"][0].flatten(), t["initial_state"][1].flatten()
+    y4, s4 = vb.linear_attention_step(*two, view(0, 3 * size, 2), state_out=view(size, size, 2))
+    assert torch.equal(y4, y[:2]) and torch.equal(s4, new[:2])

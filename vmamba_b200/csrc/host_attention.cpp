@@ -121,6 +121,17 @@ static std::pair<Tensor, OptT> attention_fn(const Tensor& q_, const Tensor& k_, 
     return {r[0], final_state ? OptT(r[1]) : OptT()};
 }
 
+// Two sets of states of `size` elements, each set evenly spaced: whether any of one touches any of the other.  Both are walked in the order of their addresses.
+static bool states_overlap(const Tensor& x, const Tensor& y, int64_t size) {
+    const int64_t n = x.size(0), sx = x.stride(0), sy = y.stride(0), ahead = y.data_ptr<float>() - x.data_ptr<float>();
+    for (int64_t i = 0, j = 0; i < n && j < n;) {
+        const int64_t d = j * sy + ahead - i * sx;              // from the one to the other
+        if (d > -size && d < size) return true;
+        d > 0 ? ++i : ++j;
+    }
+    return false;
+}
+
 static std::pair<Tensor, Tensor> attention_step(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& decay, const Tensor& state,
                                                 std::optional<double> scale_, const OptT& out_) {
     Tensor to = opt(out_);
@@ -144,9 +155,7 @@ static std::pair<Tensor, Tensor> attention_step(const Tensor& q_, const Tensor& 
     check_state(state, "state");
     if (to.defined()) {
         check_state(to, "state_out");
-        const char *a = (const char*)state.data_ptr(), *b = (const char*)to.data_ptr();
-        auto end = [&](const Tensor& s, const char* p) { return B ? p + 4 * ((B - 1) * (B == 1 ? 0 : s.stride(0)) + size) : p; };
-        TORCH_CHECK((a == b && (B < 2 || state.stride(0) == to.stride(0))) || end(state, a) <= b || end(to, b) <= a,
+        TORCH_CHECK(B == 0 || (state.data_ptr() == to.data_ptr() && (B == 1 || state.stride(0) == to.stride(0))) || !states_overlap(state, to, size),
                     "state_out must be state itself or memory that does not overlap it");
     } else
         to = at::empty({B, H, dk, dv}, state.options());

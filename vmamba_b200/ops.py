@@ -202,7 +202,8 @@ def linear_attention_step(q, k, v, log_decay, state, scale=None, state_out=None)
     """One token of every sequence through `linear_attention_fn`: (o, new state).
 
     q, k: (batch, groups, dk), v: (batch, heads, dv), log_decay: (batch, heads) or (heads,), state: float32 (batch, heads, dk, dv), dense but for its
-    batch stride (a slice of a larger cache will do).  The new state goes to `state_out` (default: a new tensor), which may be `state` itself.  Inference only."""
+    batch stride (a slice of a larger cache will do).  The new state goes to `state_out` (default: a new tensor), which may be `state` itself or any memory that
+    does not overlap it, also between the states of other sequences.  Inference only."""
     return _host.linear_attention_step(q, k, v, log_decay, state, scale, state_out)
 
 
