@@ -475,3 +475,27 @@ def test_states_side_by_side(vb, dtype):
     flat[:size], flat[3 * size:4 * size] = t["initial_state"][0].flatten(), t["initial_state"][1].flatten()
     y4, s4 = vb.linear_attention_step(*two, view(0, 3 * size, 2), state_out=view(size, size, 2))
     assert torch.equal(y4, y[:2]) and torch.equal(s4, new[:2])
+
+
+def test_a_state_written_in_place_is_seen_by_autograd(vb):
+    """A tensor that a backward pass still needs and that a step has overwritten: refused, as for any operation in place."""
+    t, _ = make(2, 1, 1, 2, 16, 16, torch.float32)
+    a = [t[n][:, 0] for n in ("q", "k", "v", "log_decay")]
+    leaf = torch.ones_like(t["initial_state"], requires_grad=True)
+    state = t["initial_state"].clone()
+    loss = (leaf * state).sum()
+    before = state._version
+    with torch.no_grad():
+        vb.linear_attention_step(*a, state, state_out=state)
+    assert state._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.no_grad():
+        before = state._version
+        vb.linear_attention_step(*a, state)
+    assert state._version == before
+    with torch.inference_mode():                                        # tensors without versions
+        own = state.clone()
+        y, _ = vb.linear_attention_step(*a, own, state_out=own)
+        z, _ = vb.linear_attention_step(*a, state)
+    assert torch.equal(y, z)

@@ -173,6 +173,7 @@ static std::pair<Tensor, Tensor> attention_step(const Tensor& q_, const Tensor& 
     p.dtype = dtype_code(v);
     p.scale = (float)scale_.value_or(1.0 / std::sqrt((double)dk));
     check(ss2d_linear_attention_step(&p, stream_of(v)), "ss2d_linear_attention_step");
+    if (!to.is_inference()) to.unsafeGetTensorImpl()->bump_version();       // a graph that has kept what was there is told
     return {o, to};
 }
 
