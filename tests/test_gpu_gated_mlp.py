@@ -373,3 +373,16 @@ def test_activations_elementwise(vb, kernels, dtype, act):
         worst = ((x - want).abs() / (HALF[dtype] * want.abs() + RELATIVE[dtype] * mag + tiny)).max().item()
         print(f"{name}: {worst:.3f} of the tolerance")
         assert worst <= 1, (name, worst)
+
+
+def test_forward_mode_is_refused(vb):
+    """There is no forward-mode derivative: a dual tensor raises instead of losing its tangent."""
+    import torch.autograd.forward_ad as fwad
+    for M in (5, 0):
+        t, _ = make(5, 16, 32, 8, torch.float32)
+        t["x"] = t["x"][:M]
+        for name in t:
+            with fwad.dual_level(), pytest.raises((RuntimeError, NotImplementedError), match="forward"):
+                vb.gated_mlp_fn(**{**t, name: fwad.make_dual(t[name], torch.ones_like(t[name]))})
+    with fwad.dual_level():
+        vb.gated_mlp_fn(**t)                                            # plain tensors inside a level: as ever

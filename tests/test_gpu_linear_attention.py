@@ -499,3 +499,18 @@ def test_a_state_written_in_place_is_seen_by_autograd(vb):
         y, _ = vb.linear_attention_step(*a, own, state_out=own)
         z, _ = vb.linear_attention_step(*a, state)
     assert torch.equal(y, z)
+
+
+def test_forward_mode_is_refused(vb):
+    """There is no forward-mode derivative: a dual tensor raises instead of losing its tangent."""
+    import torch.autograd.forward_ad as fwad
+    t, _ = make(1, 5, 1, 2, 16, 16, torch.float32)
+    for name in NAMES:
+        with fwad.dual_level():
+            x = {**t, name: fwad.make_dual(t[name], torch.ones_like(t[name]))}
+            with pytest.raises((RuntimeError, NotImplementedError), match="forward"):
+                vb.linear_attention_fn(x["q"], x["k"], x["v"], x["log_decay"], None, x["initial_state"])
+            with torch.no_grad(), pytest.raises((RuntimeError, NotImplementedError), match="forward"):
+                vb.linear_attention_step(*(x[n][:, 0] for n in NAMES[:4]), x["initial_state"])
+    with fwad.dual_level():
+        vb.linear_attention_fn(*(t[n] for n in NAMES[:4]))              # plain tensors inside a level: as ever

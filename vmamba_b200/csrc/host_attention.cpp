@@ -94,6 +94,7 @@ static std::pair<Tensor, OptT> attention_fn(const Tensor& q_, const Tensor& k_, 
                                             const OptT& state_, bool final_state) {
     const Tensor state = opt(state_);
     check_types(q_, k_, v_, decay, state);
+    no_tangents("linear_attention_fn", {&q_, &k_, &v_, &decay, &state});
     TORCH_CHECK(q_.dim() == 4 && v_.dim() == 4 && k_.sizes() == q_.sizes() && q_.size(0) == v_.size(0) && q_.size(1) == v_.size(1),
                 "q and k must be (batch, tokens, groups, dk) and v (batch, tokens, heads, dv), got ", q_.sizes(), " ", k_.sizes(), " ", v_.sizes());
     const int64_t B = v_.size(0), L = v_.size(1), G = q_.size(2), H = v_.size(2), dk = q_.size(3), dv = v_.size(3);
@@ -137,6 +138,7 @@ static std::pair<Tensor, Tensor> attention_step(const Tensor& q_, const Tensor& 
     Tensor to = opt(out_);
     check_types(q_, k_, v_, decay, state);
     require_on(v_, {&to});
+    no_tangents("linear_attention_step", {&q_, &k_, &v_, &decay, &state, &to});
     TORCH_CHECK(!wants_grad({&q_, &k_, &v_, &decay, &state, &to}),
                 "linear_attention_step has no backward pass: call it under torch.no_grad(), or linear_attention_fn for training");
     TORCH_CHECK(q_.dim() == 3 && v_.dim() == 3 && k_.sizes() == q_.sizes() && q_.size(0) == v_.size(0),

@@ -47,6 +47,10 @@ inline void require_on(const Tensor& x, std::initializer_list<const Tensor*> ts)
     for (const Tensor* t : ts)
         TORCH_CHECK(!t->defined() || t->device() == x.device(), "expected all tensors on ", x.device(), ", got one on ", t->device());
 }
+// kernels on raw pointers carry no tangents: a dual tensor would lose its own without a word, also where no gradient is recorded
+inline void no_tangents(const char* name, std::initializer_list<const Tensor*> ts) {
+    for (const Tensor* t : ts) TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), name, " has no forward-mode derivative: it was given a dual tensor");
+}
 inline void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 inline Tensor opt(const OptT& t) { return t.has_value() ? *t : Tensor(); }
 inline void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }

@@ -74,6 +74,7 @@ struct GatedMlpNode : public torch::autograd::Function<GatedMlpNode> {
 static Tensor gated_mlp_fn(const Tensor& x, const Tensor& w1, const Tensor& w2, const OptT& b1_, const OptT& b2_, int64_t act) {
     const Tensor b1 = opt(b1_), b2 = opt(b2_);
     require_on(x, {&w1, &w2, &b1, &b2});
+    no_tangents("gated_mlp_fn", {&x, &w1, &w2, &b1, &b2});
     dtype_code(x);
     for (const Tensor* t : {&w1, &w2, &b1, &b2})
         TORCH_CHECK_TYPE(!t->defined() || t->scalar_type() == x.scalar_type(), "x, weights and biases must share one dtype, got ", x.scalar_type(), " and ", t->scalar_type());
