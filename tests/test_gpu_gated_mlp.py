@@ -386,3 +386,14 @@ def test_forward_mode_is_refused(vb):
                 vb.gated_mlp_fn(**{**t, name: fwad.make_dual(t[name], torch.ones_like(t[name]))})
     with fwad.dual_level():
         vb.gated_mlp_fn(**t)                                            # plain tensors inside a level: as ever
+
+
+def test_second_derivatives_are_refused(vb):
+    """The gradients have no history of their own: asked for one, the backward pass raises instead of leaving a term out."""
+    t, _ = make(20, 16, 32, 8, torch.float32)
+    leaves = {n: v.requires_grad_() for n, v in t.items()}
+    loss = (vb.gated_mlp_fn(**leaves) ** 2).sum() + (leaves["x"] ** 3).sum()
+    with pytest.raises(RuntimeError, match="once differentiable"):
+        torch.autograd.grad(loss, leaves["x"], create_graph=True)
+    g, = torch.autograd.grad(loss, leaves["x"])
+    assert g.shape == leaves["x"].shape

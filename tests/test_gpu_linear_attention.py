@@ -514,3 +514,16 @@ def test_forward_mode_is_refused(vb):
                 vb.linear_attention_step(*(x[n][:, 0] for n in NAMES[:4]), x["initial_state"])
     with fwad.dual_level():
         vb.linear_attention_fn(*(t[n] for n in NAMES[:4]))              # plain tensors inside a level: as ever
+
+
+def test_second_derivatives_are_refused(vb):
+    """The gradients have no history of their own: asked for one, the backward pass raises instead of leaving a term out."""
+    t, _ = make(1, 70, 1, 2, 16, 16, torch.float32)
+    leaves = {n: x.requires_grad_() for n, x in t.items()}
+    for start in (None, leaves["initial_state"]):
+        o, S = vb.linear_attention_fn(*(leaves[n] for n in NAMES[:4]), None, start, True)
+        loss = (o ** 2).sum() + S.sum() + (leaves["q"] ** 3).sum()
+        with pytest.raises(RuntimeError, match="once differentiable"):
+            torch.autograd.grad(loss, leaves["q"], create_graph=True)
+        g, = torch.autograd.grad(loss, leaves["q"])
+        assert g.shape == leaves["q"].shape

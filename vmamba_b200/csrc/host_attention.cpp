@@ -58,6 +58,7 @@ struct AttentionNode : public torch::autograd::Function<AttentionNode> {
         return {r.out, r.state};
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        once_differentiable("linear_attention_fn");
         const auto s = ctx->get_saved_variables();
         const Tensor &q = s[0], &k = s[1], &v = s[2], &g = s[3];
         const bool start = ctx->saved_data["start"].toBool();

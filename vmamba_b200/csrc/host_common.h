@@ -51,6 +51,10 @@ inline void require_on(const Tensor& x, std::initializer_list<const Tensor*> ts)
 inline void no_tangents(const char* name, std::initializer_list<const Tensor*> ts) {
     for (const Tensor* t : ts) TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), name, " has no forward-mode derivative: it was given a dual tensor");
 }
+// in a backward pass that is itself recorded: gradients out of raw pointers would be constants to it
+inline void once_differentiable(const char* name) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), name, " is once differentiable: its backward pass has no derivative (create_graph)");
+}
 inline void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 inline Tensor opt(const OptT& t) { return t.has_value() ? *t : Tensor(); }
 inline void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }

@@ -44,6 +44,7 @@ struct GatedMlpNode : public torch::autograd::Function<GatedMlpNode> {
         return r.y;
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        once_differentiable("gated_mlp_fn");
         const auto s = ctx->get_saved_variables();
         const Tensor &x = s[0], &w1 = s[1], &w2 = s[2];
         const CallGuard guard(x);
