@@ -527,3 +527,16 @@ def test_second_derivatives_are_refused(vb):
             torch.autograd.grad(loss, leaves["q"], create_graph=True)
         g, = torch.autograd.grad(loss, leaves["q"])
         assert g.shape == leaves["q"].shape
+
+
+def test_no_tokens_and_only_a_state_to_differentiate(vb):
+    q, v, g = torch.zeros(2, 0, 1, 16, device="cuda"), torch.zeros(2, 0, 2, 8, device="cuda"), torch.zeros(2, 0, 2, device="cuda")
+    for dtype in (torch.float32, torch.bfloat16):
+        s = torch.randn(2, 2, 16, 8, device="cuda", dtype=dtype, requires_grad=True)
+        o = vb.linear_attention_fn(q, q, v, g, initial_state=s)
+        assert o.dtype == torch.float32 and o.shape == v.shape
+        ds, = torch.autograd.grad(o.sum(), s)
+        assert ds.shape == s.shape and ds.dtype == dtype and (ds == 0).all()
+    infinite = torch.full((2, 2, 16, 8), float("inf"), device="cuda", requires_grad=True)
+    ds, = torch.autograd.grad(vb.linear_attention_fn(q, q, v, g, initial_state=infinite).sum(), infinite)
+    assert (ds == 0).all()

@@ -109,7 +109,8 @@ static std::pair<Tensor, OptT> attention_fn(const Tensor& q_, const Tensor& k_, 
     const double scale = scale_.value_or(1.0 / std::sqrt((double)dk));
     const Tensor s0 = state.defined() ? state.to(at::kFloat).contiguous() : Tensor();
     if (B == 0 || L == 0) {                     // no token: nothing but the state, and zeros for whoever asks for gradients
-        const Tensor none = v_ + (q_.sum() + k_.sum() + decay.sum().to(v_.scalar_type())) * 0;
+        Tensor none = v_ + (q_.sum() + k_.sum() + decay.sum().to(v_.scalar_type())) * 0;
+        if (s0.defined()) none = none + s0.sum().to(v_.scalar_type()) * 0;
         if (!final_state) return {none, OptT()};
         return {none, s0.defined() ? s0.clone() : at::zeros({B, H, dk, dv}, v_.options().dtype(at::kFloat))};
     }
