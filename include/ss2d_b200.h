@@ -575,7 +575,9 @@ int ss2d_gated_mlp_fwd(const ss2d_gated_mlp_params *p, void *cuda_stream);
 int64_t ss2d_gated_mlp_workspace_bytes(const ss2d_gated_mlp_params *p);      /* < 0: invalid arguments */
 
 /* Its backward call: `fwd` with h as the forward call left it (y, b2 and its workspace are not read); dy (tokens, outputs) of `dtype`, rows dy_row_stride
- * elements apart.  dx (tokens, channels), dw1, dw2, db1, db2 as the tensors that they belong to, dense; NULL: not asked for. */
+ * elements apart.  dx (tokens, channels), dw1, dw2, db1, db2 as the tensors that they belong to, dense; NULL: not asked for.  workspace: as ss2d_gated_mlp_bwd_workspace_bytes() says
+ * for these same arguments, their pointers and strides among them: the kernels of 16-bit rows that start on 16 bytes need 4 bytes for each token and hidden channel (and sums),
+ * the others 8 more. */
 typedef struct ss2d_gated_mlp_bwd_params {
     ss2d_gated_mlp_params fwd;
     const void *dy;

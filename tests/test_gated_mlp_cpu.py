@@ -74,3 +74,29 @@ def test_cpu_tensors_and_unknown_activations_are_refused():
         vb.gated_mlp_fn(x, w1, w2)
     with pytest.raises(ValueError, match="activation"):
         vb.gated_mlp_fn(x, w1, w2, act="relu")
+
+
+def test_backward_workspace_holds_what_its_kernels_use():
+    """Aligned 16-bit calls: the gradients of value and gate and sums.  Others keep value and gate in fp32 beside them; a workspace of the one is refused by the other."""
+    L = _lib.lib()
+    before = _lib.launch_count()
+    M, C, H = 12544, 512, 2048
+    def call(dtype=_lib.SS2D_BF16, off=0):
+        b = _lib.GatedMlpBwdParams()
+        b.fwd, a = params()
+        b.fwd.tokens, b.fwd.channels, b.fwd.hidden, b.fwd.outputs, b.fwd.x_row_stride, b.fwd.dtype = M, C, H, C, C, dtype
+        for f in ("dx", "dw1", "dw2", "db1", "db2"):
+            setattr(b, f, a)
+        b.dy, b.dy_row_stride = a + off, C
+        return b, a
+    sums = 4 * 2 ** 20 * 16                                       # splits of the weight gradients, of 2 H C elements at most
+    need = L.ss2d_gated_mlp_bwd_workspace_bytes(call()[0])
+    assert 4 * M * H <= need <= 4 * M * H + sums
+    for other, size in ((call(off=2)[0], 4), (call(_lib.SS2D_F32)[0], 8)):
+        assert L.ss2d_gated_mlp_bwd_workspace_bytes(other) >= (size + 8) * M * H
+        other.workspace, other.workspace_bytes = call()[1], need
+        assert L.ss2d_gated_mlp_bwd(other, None) == -8
+    early, _ = call()
+    early.dy = None                                               # a size asked for before the upstream gradient is known: enough for any
+    assert L.ss2d_gated_mlp_bwd_workspace_bytes(early) >= 12 * M * H
+    assert _lib.launch_count() == before

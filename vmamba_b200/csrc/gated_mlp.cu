@@ -425,35 +425,39 @@ long long fwd_workspace(const ss2d_gated_mlp_params& p) {
     return 4 * (plain > tc ? plain : tc);
 }
 
-struct BwdPlan { long long dz, part, pre, total; };
-BwdPlan bwd_plan(const ss2d_gated_mlp_params& p) {
+// The same for the backward call's own tensors: what its workspace holds follows from it.
+bool tc_fits(const ss2d_gated_mlp_bwd_params& p) {
+    if (!tc_fits(p.fwd) || !p.dy || p.dy_row_stride % 8) return false;
+    for (const void* q : {p.dy, (const void*)p.dx, (const void*)p.dw1, (const void*)p.dw2})
+        if (!aligned_to(q, 16)) return false;
+    return true;
+}
+struct BwdPlan { bool tc; long long dz, part, pre, total; };
+BwdPlan bwd_plan(const ss2d_gated_mlp_bwd_params& b) {
+    const ss2d_gated_mlp_params& p = b.fwd;
     auto up = [](long long n) { return (n + 255) / 256 * 256; };
-    BwdPlan b;
-    b.dz = up(2 * p.tokens * p.hidden * (long long)dtype_size(p.dtype));
+    BwdPlan w;
+    w.tc = tc_fits(b);
+    w.dz = up(2 * p.tokens * p.hidden * (long long)dtype_size(p.dtype));
     const long long spans = (p.tokens + kSpan - 1) / kSpan;
     long long most = spans * (2 * p.hidden + p.outputs);
     const long long M1 = 2 * p.hidden, N1 = p.channels, M2 = p.outputs, N2 = p.hidden;
-    for (long long n : {splits_of(M1, N1, p.tokens) * M1 * N1, splits_of(M2, N2, p.tokens) * M2 * N2, (long long)(splits_of(p.tokens, p.channels, M1) * p.tokens * p.channels), part_elements(M1, N1, p.tokens),
-                        part_elements(M2, N2, p.tokens), part_elements(p.tokens, p.channels, M1)})
+    auto parts = [&](long long M, long long N, long long K) { return w.tc ? part_elements(M, N, K) : splits_of(M, N, K) * M * N; };
+    for (long long n : {parts(M1, N1, p.tokens), parts(M2, N2, p.tokens), parts(p.tokens, p.channels, M1)})
         if (n > most) most = n;
-    b.part = up(4 * most);
-    b.pre = up(8 * p.tokens * p.hidden);                      // of calls that the tensor-core kernels do not take, wherever their tensors start
-    b.total = b.dz + b.part + b.pre;
-    return b;
+    w.part = up(4 * most);
+    w.pre = w.tc ? 0 : up(8 * p.tokens * p.hidden);           // the tensor-core kernels have value and gate in TMEM
+    w.total = w.dz + w.part + w.pre;
+    return w;
 }
 
-template <typename T, int ACT> int backward(const ss2d_gated_mlp_bwd_params& p, cudaStream_t st) {
+template <typename T, int ACT> int backward(const ss2d_gated_mlp_bwd_params& p, const BwdPlan& plan, cudaStream_t st) {
     const ss2d_gated_mlp_params& f = p.fwd;
-    const BwdPlan plan = bwd_plan(f);
     char* const ws = (char*)p.workspace;
     void* const dz = ws;
     float *const part = (float*)(ws + plan.dz), *const pre = (float*)(ws + plan.dz + plan.part);
     const long long H = f.hidden, H2 = 2 * H;
-    bool tc = false;
-    if constexpr (sizeof(T) == 2) {
-        tc = tc_fits(f) && p.dy_row_stride % 8 == 0;
-        for (const void* q : {p.dy, (const void*)p.dx, (const void*)p.dw1, (const void*)p.dw2}) tc = tc && aligned_to(q, 16);
-    }
+    const bool tc = plan.tc;
     if (p.dx || p.dw1 || p.db1) {
         if constexpr (sizeof(T) == 2)
             if (tc) {
@@ -544,7 +548,7 @@ long long gated_mlp_workspace_bytes(const ss2d_gated_mlp_params* p) {
 
 long long gated_mlp_bwd_workspace_bytes(const ss2d_gated_mlp_bwd_params* p) {
     if (!p || check_common(p->fwd) != SS2D_OK) return -1;
-    return bwd_plan(p->fwd).total;
+    return bwd_plan(*p).total;
 }
 
 int gated_mlp_bwd(const ss2d_gated_mlp_bwd_params* p, cudaStream_t st) {
@@ -557,8 +561,9 @@ int gated_mlp_bwd(const ss2d_gated_mlp_bwd_params* p, cudaStream_t st) {
     if (!aligned_to(p->dy, e) || !aligned_to(f.h, 16)) return SS2D_EINVAL_ALIGN;
     for (const void* q : {p->dx, p->dw1, p->dw2, p->db1, p->db2})
         if (!aligned_to(q, 2 * e)) return SS2D_EINVAL_ALIGN;
-    if (!p->workspace || p->workspace_bytes < bwd_plan(f).total || !aligned_to(p->workspace, 16)) return SS2D_EWORKSPACE;
-    return for_type_act(f.dtype, f.act, [&](auto z, auto act) { return backward<decltype(z), decltype(act)::value>(*p, st); });
+    const BwdPlan plan = bwd_plan(*p);
+    if (!p->workspace || p->workspace_bytes < plan.total || !aligned_to(p->workspace, 16)) return SS2D_EWORKSPACE;
+    return for_type_act(f.dtype, f.act, [&](auto z, auto act) { return backward<decltype(z), decltype(act)::value>(*p, plan, st); });
 }
 
 }  // namespace ss2d
