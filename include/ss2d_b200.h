@@ -588,6 +588,16 @@ typedef struct ss2d_gated_mlp_bwd_params {
 int ss2d_gated_mlp_bwd(const ss2d_gated_mlp_bwd_params *p, void *cuda_stream);
 int64_t ss2d_gated_mlp_bwd_workspace_bytes(const ss2d_gated_mlp_bwd_params *p);
 
+/* Which kernel takes a product of a call with these arguments, without a launch (tests ask it whether they reach what they mean to): product 0 value and gate, 1 the output, 2 the
+ * gradients of value and gate, 3 dx, 4 dw1, 5 dw2.  One of the below + 16 times the parts that the contraction is split into, or a status < 0.  Tiles of the tensor-core kernels
+ * in rows x columns of products: a product 0 has half as many columns of results, a product 2 128. */
+enum { SS2D_GATED_MLP_PLAIN = 0,    /* any type, size and alignment: mma.sync, tiles of 64 x 64 */
+       SS2D_GATED_MLP_FEW = 1,      /* up to 16 tokens */
+       SS2D_GATED_MLP_NARROW = 2,   /* tcgen05: 128 x 128 */
+       SS2D_GATED_MLP_WIDE = 3,     /* 128 x 256 */
+       SS2D_GATED_MLP_PAIR = 4 };   /* 256 x 256 by two CTAs */
+int ss2d_gated_mlp_kernel(const ss2d_gated_mlp_bwd_params *p, int product);
+
 int ss2d_version(void);
 const char *ss2d_strerror(int status);
 /* number of kernel launches issued by this library in this process so far (all entry points) */

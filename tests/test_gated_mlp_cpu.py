@@ -100,3 +100,45 @@ def test_backward_workspace_holds_what_its_kernels_use():
     early.dy = None                                               # a size asked for before the upstream gradient is known: enough for any
     assert L.ss2d_gated_mlp_bwd_workspace_bytes(early) >= 12 * M * H
     assert _lib.launch_count() == before
+
+
+def kernels(M, C, H, O):
+    """{(layout of the operands, kernel, split, whether a CTA walks three tiles or more and not all as many)} of a 16-bit call and its backward call"""
+    L = _lib.lib()
+    b = _lib.GatedMlpBwdParams()
+    b.fwd, a = params()
+    b.fwd.tokens, b.fwd.channels, b.fwd.hidden, b.fwd.outputs, b.fwd.x_row_stride, b.dy, b.dy_row_stride = M, C, H, O, C, a, O
+    found = set()
+    for product, (rows, cols, layout) in enumerate([(M, 2 * H, "gate"), (M, O, "NT"), (M, H, "gradients of value and gate"), (M, C, "NN"), (2 * H, C, "TN"), (O, H, "TN")]):
+        code = L.ss2d_gated_mlp_kernel(b, product)
+        assert code >= 16
+        kernel, splits = code % 16, code // 16
+        if kernel < 2:
+            continue
+        high, wide = (256 if kernel == 4 else 128), (128 if kernel == 2 or product == 2 else 256)
+        tiles, walkers = -(-rows // high) * -(-cols // wide) * splits, 74 if kernel == 4 else 148
+        found.add((layout, kernel, splits > 1, tiles > 2 * walkers and tiles % walkers != 0))
+    return found
+
+
+def test_shapes_of_the_gpu_tests_reach_every_kernel():
+    from tests.test_gpu_gated_mlp import LARGE, SHAPES
+    L = _lib.lib()
+    small = set().union(*(kernels(*s) for s in SHAPES))
+    found = small.union(*(kernels(*s) for s in LARGE))
+    kinds = {("gate", k, False) for k in (2, 3, 4)} | {("gradients of value and gate", k, False) for k in (3, 4)} | \
+            {(layout, k, split) for layout in ("NT", "NN", "TN") for k in (2, 3, 4) for split in (False, True)}
+    assert {f[:3] for f in found} == kinds
+    # what is never chosen for many tiles, wider ones being faster there: narrow tiles in front of the activation; unsplit narrow ones and split wide ones of most products
+    many = {f[:3] for f in found if f[3]}
+    assert many >= {k for k in kinds if k[1] == 4} | {("gate", 3, False), ("gradients of value and gate", 3, False), ("NT", 3, False), ("TN", 3, False), ("TN", 3, True),
+                                                      ("NT", 2, True), ("NN", 2, True), ("TN", 2, False), ("TN", 2, True)}
+    b = _lib.GatedMlpBwdParams()
+    assert L.ss2d_gated_mlp_kernel(None, 0) == -1 and L.ss2d_gated_mlp_kernel(b, 0) == -1
+    b.fwd, a = params()
+    assert L.ss2d_gated_mlp_kernel(b, 6) == -2 and L.ss2d_gated_mlp_kernel(b, -1) == -2
+    assert [L.ss2d_gated_mlp_kernel(b, i) % 16 for i in range(6)] == [1, 1, 0, 0, 0, 0]       # no upstream gradient yet
+    b.dy, b.dy_row_stride = a, 16
+    assert [L.ss2d_gated_mlp_kernel(b, i) % 16 for i in range(6)] == [1, 1, 4, 2, 2, 2]
+    b.fwd.x = a + 2
+    assert [L.ss2d_gated_mlp_kernel(b, i) % 16 for i in range(6)] == [0] * 6

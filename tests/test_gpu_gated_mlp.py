@@ -397,3 +397,22 @@ def test_second_derivatives_are_refused(vb):
         torch.autograd.grad(loss, leaves["x"], create_graph=True)
     g, = torch.autograd.grad(loss, leaves["x"])
     assert g.shape == leaves["x"].shape
+
+
+# ---- large calls -------------------------------------------------------------------------------------------------------
+# Every form of the tensor-core kernels, with several tiles for each CTA where its form is ever chosen for that, ragged edges, and last rounds that leave some without
+# a tile (test_gated_mlp_cpu.py holds the planner to it).
+LARGE = [(2928, 16, 12720, 8), (320, 24, 18976, 8), (13232, 536, 8, 544), (17, 512, 12232, 1080), (6931, 48, 24, 2008), (5557, 264, 6344, 96), (2485, 40, 4904, 1920), (6225, 672, 16, 96)]
+
+
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", LARGE, ids=str)
+def test_large_calls(vb, shape, dtype, act):
+    t, dy = make(*shape, dtype)
+    ref = reference(t, dy, act, dtype)
+    got = run(vb, t, dy, act)
+    compare(got, ref, dtype)
+    del ref
+    again = run(vb, t, dy, act)
+    assert all(torch.equal(got[n], again[n]) for n in got)

@@ -198,6 +198,7 @@ EXPORTS = {
     "ss2d_gated_mlp_workspace_bytes": (_i64, [ctypes.POINTER(GatedMlpParams)]),
     "ss2d_gated_mlp_bwd": (ctypes.c_int, [ctypes.POINTER(GatedMlpBwdParams), _vp]),
     "ss2d_gated_mlp_bwd_workspace_bytes": (_i64, [ctypes.POINTER(GatedMlpBwdParams)]),
+    "ss2d_gated_mlp_kernel": (ctypes.c_int, [ctypes.POINTER(GatedMlpBwdParams), ctypes.c_int]),
     "ss2d_set_debug_checks": (ctypes.c_int, [ctypes.c_int]),
     "ss2d_version": (ctypes.c_int, []),
     "ss2d_strerror": (ctypes.c_char_p, [ctypes.c_int]),

@@ -53,6 +53,7 @@ int linear_attention_step(const ss2d_linear_attention_step_params* p, cudaStream
 int gated_mlp_fwd(const ss2d_gated_mlp_params* p, cudaStream_t st);
 int gated_mlp_bwd(const ss2d_gated_mlp_bwd_params* p, cudaStream_t st);
 long long gated_mlp_bwd_workspace_bytes(const ss2d_gated_mlp_bwd_params* p);
+int gated_mlp_kernel(const ss2d_gated_mlp_bwd_params* p, int product);
 long long gated_mlp_workspace_bytes(const ss2d_gated_mlp_params* p);
 
 static std::atomic<long long> g_launches{0};
@@ -247,6 +248,7 @@ int ss2d_gated_mlp_bwd(const ss2d_gated_mlp_bwd_params* p, void* stream) {
     return ss2d::gated_mlp_bwd(p, (cudaStream_t)stream);
 }
 int64_t ss2d_gated_mlp_bwd_workspace_bytes(const ss2d_gated_mlp_bwd_params* p) { return ss2d::gated_mlp_bwd_workspace_bytes(p); }
+int ss2d_gated_mlp_kernel(const ss2d_gated_mlp_bwd_params* p, int product) { return ss2d::gated_mlp_kernel(p, product); }
 int ss2d_version(void) { return SS2D_ABI_VERSION; }
 int64_t ss2d_launch_count(void) { return ss2d::g_launches.load(std::memory_order_relaxed); }
 

@@ -341,6 +341,8 @@ bool tc_fits(const ss2d_gated_mlp_params& p) {
     return true;
 }
 
+bool tc_forward_fits(const ss2d_gated_mlp_params& p) { return tc_fits(p) && aligned_to(p.y, 16); }
+
 // Tiles of the tensor-core kernels: 128 x 128, 128 x 256 (in TMEM; EPI_GATE gives half as many columns) by one CTA, 256 x 256 by two.
 enum Form { kNarrow, kWide, kPair, kForms };
 constexpr int kFormRows[kForms] = {128, 128, 256}, kFormCols[kForms] = {128, 256, 256}, kFormCtas[kForms] = {1, 1, 2};
@@ -365,6 +367,12 @@ Plan plan_of(long long M, long long N, long long K, bool gate, bool may_split) {
         }
     }
     return best;
+}
+// Gradients of value and gate: tiles of 128 columns by one CTA, or by two of 256 rows, whose steps are shorter by what those of the forward products are: whichever takes
+// fewer rounds by them
+bool grad_by_pairs(long long tokens, long long hidden) {
+    const long long n = (hidden + 127) / 128, one = ((tokens + 127) / 128 * n + 147) / 148, two = ((tokens + 255) / 256 * n + 73) / 74;
+    return two * kFormStep[kPair] < one * kFormStep[kWide];
 }
 long long part_elements(long long M, long long N, long long K) {
     const Plan w = plan_of(M, N, K, false, true);
@@ -465,10 +473,8 @@ template <typename T, int ACT> int backward(const ss2d_gated_mlp_bwd_params& p, 
                 a.a = {f.x, f.x_row_stride}; a.b = {f.w1, f.channels}; a.a2 = {p.dy, p.dy_row_stride}; a.b2 = {f.w2, H};
                 a.M = f.tokens; a.N = H; a.K = f.channels; a.K2 = f.outputs; a.b_rows = H2; a.bias = f.b1;
                 a.out = dz; a.out2 = (T*)dz + H; a.out_pitch = H2;
-                // tiles of 128 columns by one CTA, or by two of 256 rows, whose steps are shorter by what those of the forward products are: whichever takes fewer rounds by them
-                const long long n = (H + 127) / 128, one = ((f.tokens + 127) / 128 * n + 147) / 148, two = ((f.tokens + 255) / 256 * n + 73) / 74;
-                if (const int rc = two * kFormStep[kPair] < one * kFormStep[kWide] ? ptc::run_product<T, false, true, EPI_GRAD, ACT, 384, true>(a, st)
-                                                                                 : ptc::run_product<T, false, true, EPI_GRAD, ACT, 384, false>(a, st)) return rc;
+                if (const int rc = grad_by_pairs(f.tokens, H) ? ptc::run_product<T, false, true, EPI_GRAD, ACT, 384, true>(a, st)
+                                                              : ptc::run_product<T, false, true, EPI_GRAD, ACT, 384, false>(a, st)) return rc;
             }
         if (!tc) {
             ProductArgs g = product_args<T>(f.x, f.x_row_stride, f.w1, f.channels, f.tokens, H, f.channels);
@@ -536,7 +542,7 @@ int gated_mlp_fwd(const ss2d_gated_mlp_params* p, cudaStream_t st) {
         using T = decltype(z);
         constexpr int A = decltype(act)::value;
         if constexpr (sizeof(T) == 2)
-            if (tc_fits(*p) && aligned_to(p->y, 16)) return tc_forward<T, A>(*p, st);
+            if (tc_forward_fits(*p)) return tc_forward<T, A>(*p, st);
         return plain_forward<T, A>(*p, st);
     });
 }
@@ -549,6 +555,25 @@ long long gated_mlp_workspace_bytes(const ss2d_gated_mlp_params* p) {
 long long gated_mlp_bwd_workspace_bytes(const ss2d_gated_mlp_bwd_params* p) {
     if (!p || check_common(p->fwd) != SS2D_OK) return -1;
     return bwd_plan(*p).total;
+}
+
+int gated_mlp_kernel(const ss2d_gated_mlp_bwd_params* p, int product) {
+    if (!p) return SS2D_EINVAL_NULL;
+    const ss2d_gated_mlp_params& f = p->fwd;
+    if (const int rc = check_common(f)) return rc;
+    const long long sizes[6][3] = {{f.tokens, f.hidden, f.channels}, {f.tokens, f.outputs, f.hidden}, {f.tokens, f.hidden, f.outputs}, {f.tokens, f.channels, 2 * f.hidden},
+                                   {2 * f.hidden, f.channels, f.tokens}, {f.outputs, f.hidden, f.tokens}};
+    if (product < 0 || product > 5) return SS2D_EINVAL_SHAPE;
+    const auto& [M, N, K] = sizes[product];
+    const bool one = product == 0 || product == 2;                                // nothing is split in front of an activation
+    if (!(product < 2 ? tc_forward_fits(f) : tc_fits(*p))) {
+        const long long want = one ? 1 : splits_of(M, N, K), per = ((K + want - 1) / want + kStep - 1) / kStep * kStep;
+        return SS2D_GATED_MLP_PLAIN + 16 * (int)((K + per - 1) / per);
+    }
+    if (product < 2 && f.tokens <= kFew) return SS2D_GATED_MLP_FEW + 16;
+    if (product == 2) return (grad_by_pairs(M, N) ? SS2D_GATED_MLP_PAIR : SS2D_GATED_MLP_WIDE) + 16;
+    const Plan w = plan_of(M, N, K, product == 0, !one);
+    return SS2D_GATED_MLP_NARROW + w.form + 16 * w.splits;
 }
 
 int gated_mlp_bwd(const ss2d_gated_mlp_bwd_params* p, cudaStream_t st) {
