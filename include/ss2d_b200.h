@@ -498,7 +498,7 @@ int ss2d_planes_to_pixels(const ss2d_relayout_params *p, void *cuda_stream);
 
 /* ------------------------------------------------------------------------------------
  * Linear attention with a decay for each head (the scan of the m0 family of SS2D, classification/models/vmamba.py:915-1104, in attention's terms:
- * C, B and x dt are q, k and v, dt A is log_decay).  For every sequence b and head h, with group h / (heads / n_groups) of q and k:
+ * C, B and x dt are q, k and v, dt A is log_decay, scale is 1).  For every sequence b and head h, with group h / (heads / n_groups) of q and k:
  *   S_t = exp(log_decay_t) S_{t-1} + k_t v_t^T          S (dk, dv) fp32, S_0 = initial_state or zero
  *   out_t = scale S_t^T q_t
  * q, k: (batch, seqlen, n_groups, dk), v: (batch, seqlen, heads, dv), of `dtype`, last dimension contiguous, the others strided (elements,

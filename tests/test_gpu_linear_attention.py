@@ -540,3 +540,24 @@ def test_no_tokens_and_only_a_state_to_differentiate(vb):
     infinite = torch.full((2, 2, 16, 8), float("inf"), device="cuda", requires_grad=True)
     ds, = torch.autograd.grad(vb.linear_attention_fn(q, q, v, g, initial_state=infinite).sum(), infinite)
     assert (ds == 0).all()
+
+
+@pytest.mark.parametrize("groups", [1, 2])
+def test_is_the_selective_scan_of_heads_that_share_a_decay(vb, groups):
+    """`selective_scan_fn` with B, C, u dt and A dt as keys, queries, values and log decays: the same numbers with scale 1, which is not the default."""
+    B, L, H, N, P = 2, 150, 4, 16, 8
+    gen = torch.Generator().manual_seed(1)
+    rnd = lambda *s: torch.randn(s, generator=gen).cuda()      # noqa: E731
+    u, k, q = rnd(B, H, P, L), rnd(B, groups, N, L), rnd(B, groups, N, L)
+    dt, rate = 0.1 * torch.rand((B, H, 1, L), generator=gen).cuda(), -1.0 - torch.rand(H, generator=gen).cuda()
+    y = vb.selective_scan_fn(u.flatten(1, 2), dt.expand(B, H, P, L).flatten(1, 2).contiguous(), rate[:, None, None].expand(H, P, N).flatten(0, 1).contiguous(),
+                             k, q, delta_softplus=False).view(B, H, P, L).permute(0, 3, 1, 2)
+    tokens = lambda x: x.permute(0, 3, 1, 2)      # noqa: E731
+    v, g = tokens(u * dt), (dt[:, :, 0] * rate[:, None]).transpose(1, 2)
+    o = vb.linear_attention_fn(tokens(q), tokens(k), v, g, scale=1.0)
+    t = {"q": tokens(q), "k": tokens(k), "v": v, "log_decay": g, "initial_state": torch.zeros(B, H, N, P, device="cuda")}
+    mag = recurrence(*(t[n].double().abs() if n != "log_decay" else t[n].double() for n in NAMES), 1.0)[0]
+    # SUMS of the magnitudes for the one and the other, products of pieces
+    assert ((o - y).abs() <= (2 * SUMS + 2 * FORM[torch.float32]) * mag).all()
+    default = vb.linear_attention_fn(tokens(q), tokens(k), v, g)
+    assert ((default * N ** 0.5 - y).abs() <= (2 * SUMS + 2 * FORM[torch.float32]) * mag).all()

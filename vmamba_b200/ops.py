@@ -182,8 +182,8 @@ def linear_attention_fn(q, k, v, log_decay, scale=None, initial_state=None, retu
 
         S_t = exp(log_decay_t) S_{t-1} + k_t v_t^T,    o_t = scale S_t^T q_t
 
-    the scan of the reference's m0 family (classification/models/vmamba.py:915-1104: C, B and x dt are q, k and v, dt A is log_decay) and what
-    `selective_scan_fn` computes where all channels of a head share one decay.
+    with `scale=1` the scan of the reference's m0 family (classification/models/vmamba.py:915-1104: C, B and x dt are q, k and v, dt A is log_decay) and what
+    `selective_scan_fn` computes where all channels of a head share one decay; the default scale is attention's, dk ** -0.5.
 
     q, k: (batch, tokens, groups, dk), v: (batch, tokens, heads, dv), one dtype (float32, float16, bfloat16); heads is a multiple of groups, and heads
     h * groups // heads share their queries and keys.  Any strides (rows whose last dimension is not contiguous are copied); dk and dv up to 128.
