@@ -505,8 +505,8 @@ int ss2d_planes_to_pixels(const ss2d_relayout_params *p, void *cuda_stream);
  * >= 0: heads that share rows have a stride of 0); log_decay: (batch, seqlen, heads) fp32, strided.  -inf resets the state; values are meant
  * to be <= 0.  out: (batch, seqlen, heads, dv) of `dtype`, dense; initial_state, final_state: (batch, heads, dk, dv) fp32, dense, NULL where
  * there is none.  chunk_states: NULL, or ss2d_linear_attention_states_bytes() bytes, 16-byte aligned: the state in front of every 64th token, in the
- * layout that the backward call reads.  dk and dv up to 128 (else SS2D_ENOTSUP).  A value that is not finite may reach every output of its 64 tokens, also those in front
- * of it.  workspace:
+ * layout that the backward call reads.  dk and dv up to 128 (else SS2D_ENOTSUP).  A value of v that is not finite reaches its column's outputs from the first token of its block
+ * of 128 tokens on, also those in front of it, and may reach any gradient of its block.  workspace:
  * ss2d_linear_attention_workspace_bytes() bytes, 16-byte aligned (0: none), a size of the shape and of whether chunk_states are asked for.  dense tensors are aligned to two elements (fp32 ones to 8 bytes).
  * No atomics: repeated calls give bit-identical results.
  * -------------------------------------------------------------------------------- */

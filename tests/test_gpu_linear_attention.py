@@ -561,3 +561,33 @@ def test_is_the_selective_scan_of_heads_that_share_a_decay(vb, groups):
     assert ((o - y).abs() <= (2 * SUMS + 2 * FORM[torch.float32]) * mag).all()
     default = vb.linear_attention_fn(tokens(q), tokens(k), v, g)
     assert ((default * N ** 0.5 - y).abs() <= (2 * SUMS + 2 * FORM[torch.float32]) * mag).all()
+
+
+FORMS = [(1, 400, 1, 2, 128, 128, torch.bfloat16), (1, 400, 1, 2, 32, 32, torch.bfloat16), (1, 150, 1, 2, 64, 64, torch.float16), (1, 150, 1, 2, 32, 64, torch.float32)]
+
+
+@pytest.mark.parametrize("shape", FORMS, ids=str)
+def test_values_that_are_not_finite(vb, shape):
+    """A query's: its own token.  A key's or decay's: its heads from its token on.  A value's: its own column, from the first token of its 128 on."""
+    *shape, dtype = shape
+    t, _ = make(*shape, dtype)
+    at, tokens = 141, torch.arange(shape[1], device="cuda")
+    for bad in (float("nan"), float("inf")):
+        for name in NAMES[:4]:
+            if name == "log_decay" and bad == float("inf"):
+                continue
+            x = {n: y.clone() for n, y in t.items()}
+            x[name][(0, at, 0) + ((5,) if name != "log_decay" else ())] = bad
+            with torch.no_grad():
+                o, S = vb.linear_attention_fn(*(x[n] for n in NAMES[:4]), None, x["initial_state"], True)
+            fine = torch.isfinite(o[0])                                 # (tokens, heads, columns)
+            if name == "q":
+                assert fine[tokens != at].all() and not fine[at].any() and torch.isfinite(S).all()
+            elif name == "k":
+                assert fine[tokens < at].all() and not fine[tokens >= at].any()
+            elif name == "log_decay":
+                assert fine[:, 1].all() and fine[tokens < at].all() and not fine[tokens >= at, 0].any() and torch.isfinite(S[0, 1]).all()
+            else:
+                assert fine[:, 1].all() and fine[tokens < 128].all() and not fine[tokens >= at, 0, 5].any()
+                others = torch.arange(shape[5], device="cuda") != 5
+                assert fine[:, 0][:, others].all() and torch.isfinite(S[0, 0][:, others]).all() and torch.isfinite(S[0, 1]).all()

@@ -192,8 +192,9 @@ def linear_attention_fn(q, k, v, log_decay, scale=None, initial_state=None, retu
     Returns o (batch, tokens, heads, dv) of v's dtype; with `return_final_state` also the state behind the last token, float32.  Differentiable in
     all tensors; the backward pass keeps the inputs and the state in front of every 64th token.  Repeated calls give bit-identical results.
 
-    Sequences of other lengths in one batch: k = 0 and log_decay = 0 on the padding leave the state as it is.  A value that is not finite may reach all
-    outputs of its 64 tokens, also those in front of it."""
+    Sequences of other lengths in one batch: k = 0 and log_decay = 0 on the padding leave the state as it is.  A value (of v) that is not finite reaches its column's outputs
+    from the first token of its block of 128 tokens on, which is up to 127 tokens in front of it, and may reach any gradient of its block; queries, keys and decays that are not finite
+    reach what the formulas let them reach."""
     o, state = _host.linear_attention_fn(q, k, v, log_decay, scale, initial_state, bool(return_final_state))
     return (o, state) if return_final_state else o
 
