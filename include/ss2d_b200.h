@@ -503,7 +503,7 @@ int ss2d_planes_to_pixels(const ss2d_relayout_params *p, void *cuda_stream);
  *   out_t = scale S_t^T q_t
  * q, k: (batch, seqlen, n_groups, dk), v: (batch, seqlen, heads, dv), of `dtype`, last dimension contiguous, the others strided (elements,
  * >= 0: heads that share rows have a stride of 0); log_decay: (batch, seqlen, heads) fp32, strided.  -inf resets the state; values are meant
- * to be <= 0.  out: (batch, seqlen, heads, dv) of `dtype`, dense; initial_state, final_state: (batch, heads, dk, dv) fp32, dense, NULL where
+ * to be <= 0 (positive ones are as exact while the weights from any token to any later one of its 128 are numbers of fp32; behind the first that is not, results are inf or NaN).  out: (batch, seqlen, heads, dv) of `dtype`, dense; initial_state, final_state: (batch, heads, dk, dv) fp32, dense, NULL where
  * there is none.  chunk_states: NULL, or ss2d_linear_attention_states_bytes() bytes, 16-byte aligned: the state in front of every 64th token, in the
  * layout that the backward call reads.  dk and dv up to 128 (else SS2D_ENOTSUP).  A value of v that is not finite reaches its column's outputs from the first token of its block
  * of 128 tokens on, also those in front of it, and may reach any gradient of its block.  workspace:

@@ -591,3 +591,21 @@ def test_values_that_are_not_finite(vb, shape):
                 assert fine[:, 1].all() and fine[tokens < 128].all() and not fine[tokens >= at, 0, 5].any()
                 others = torch.arange(shape[5], device="cuda") != 5
                 assert fine[:, 0][:, others].all() and torch.isfinite(S[0, 0][:, others]).all() and torch.isfinite(S[0, 1]).all()
+
+
+@pytest.mark.parametrize("shape", FORMS, ids=str)
+def test_states_that_grow(vb, shape):
+    """Positive log decays: exact as long as the weights between two tokens are numbers of fp32.  Growth by 2^30 over some tokens, decay by as much behind them."""
+    *shape, dtype = shape
+    t, _ = make(*shape, dtype, decay=0.02)
+    g = t["log_decay"]
+    for first in (3, 40, 70, 140):
+        g[:, first:first + 10] += 3 * 0.6931
+        g[:, first + 20:first + 30] -= 3 * 0.6931
+    scale = 2.0 ** -24
+    with torch.no_grad():
+        o, S = vb.linear_attention_fn(*(t[n] for n in NAMES[:4]), scale, t["initial_state"], True)
+    ref, mag = (recurrence(*(f(n) for n in NAMES), scale) for f in (lambda n: t[n].double(), lambda n: t[n].double() if n == "log_decay" else t[n].double().abs()))
+    # beside the roundings of the head of this file: log decays of up to 3 in base 2, each off by 2^-23, in weights of up to 20 of them
+    assert ((S - ref[1]).abs() <= (3 * PIECES[dtype] + SUMS + 2.0 ** -17) * mag[1]).all()
+    assert ((o - ref[0]).abs() <= HALF[dtype] * ref[0].abs() + (2 * FORM[dtype] + SUMS + 2.0 ** -17) * mag[0] + (2.0 ** -25 if dtype == torch.float16 else 0)).all()

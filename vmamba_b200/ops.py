@@ -188,7 +188,8 @@ def linear_attention_fn(q, k, v, log_decay, scale=None, initial_state=None, retu
     q, k: (batch, tokens, groups, dk), v: (batch, tokens, heads, dv), one dtype (float32, float16, bfloat16); heads is a multiple of groups, and heads
     h * groups // heads share their queries and keys.  Any strides (rows whose last dimension is not contiguous are copied); dk and dv up to 128.
     log_decay: (batch, tokens, heads), or (heads,) for rates that the tokens share; computed in float32.  It is meant to be <= 0; -inf resets the state
-    (what lies below -138 does).  scale: default dk ** -0.5.  initial_state: (batch, heads, dk, dv), default zeros.
+    (what lies below -138 does).  Positive ones let it grow: results are as exact while the weights exp(sum of log decays) from any token to any later one of its block of 128 are
+    numbers of float32, and inf or NaN behind the first that is not.  scale: default dk ** -0.5.  initial_state: (batch, heads, dk, dv), default zeros.
     Returns o (batch, tokens, heads, dv) of v's dtype; with `return_final_state` also the state behind the last token, float32.  Differentiable in
     all tensors; the backward pass keeps the inputs and the state in front of every 64th token.  Repeated calls give bit-identical results.
 
