@@ -609,3 +609,18 @@ def test_states_that_grow(vb, shape):
     # beside the roundings of the head of this file: log decays of up to 3 in base 2, each off by 2^-23, in weights of up to 20 of them
     assert ((S - ref[1]).abs() <= (3 * PIECES[dtype] + SUMS + 2.0 ** -17) * mag[1]).all()
     assert ((o - ref[0]).abs() <= HALF[dtype] * ref[0].abs() + (2 * FORM[dtype] + SUMS + 2.0 ** -17) * mag[0] + (2.0 ** -25 if dtype == torch.float16 else 0)).all()
+
+
+def test_long_memory_of_wide_heads(vb):
+    """The sum of `test_long_memory` in the kernels of long bf16 sequences: chunks of 128 tokens, each summed apart (2 x 128 products of two pieces, cut off, 2^-16 as there),
+    256 of them added in fp32."""
+    B, L, H, d = 1, 32768, 2, 128
+    t, _ = make(B, L, H, H, d, d, torch.bfloat16)
+    k, v = t["k"].abs(), t["v"].abs()
+    want = torch.einsum("blhk,blhv->bhkv", k.double(), v.double())
+    for train in (False, True):                                         # chunks of 128 and of 64 tokens
+        with torch.set_grad_enabled(train):
+            leaf = v.clone().requires_grad_(train)
+            _, S = vb.linear_attention_fn(t["q"], k, leaf, torch.zeros(H, device="cuda"), return_final_state=True)
+        assert ((S.detach() - want).abs() / want).max() <= 2.0 ** -16 + 1024 * 2.0 ** -24 / 3
+        assert (S.detach() - want).norm() <= 2.0 ** -17 * want.norm()
