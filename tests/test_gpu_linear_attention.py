@@ -624,3 +624,16 @@ def test_long_memory_of_wide_heads(vb):
             _, S = vb.linear_attention_fn(t["q"], k, leaf, torch.zeros(H, device="cuda"), return_final_state=True)
         assert ((S.detach() - want).abs() / want).max() <= 2.0 ** -16 + 1024 * 2.0 ** -24 / 3
         assert (S.detach() - want).norm() <= 2.0 ** -17 * want.norm()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_resets_behind_decays_of_almost_one(vb, dtype):
+    """Log decays between -2^-25 and 0 (saturated gates), whose whole numbers and fractions are at their border, and resets among them: nothing crosses these."""
+    t, up = make(1, 192, 1, 2, 32, 32, dtype)
+    resets = [2, 7, 33, 64, 100, 127, 128, 190]
+    for small in (-1e-9, -2.0 ** -26, -2.0 ** -24, 0.0):
+        t["log_decay"].fill_(small)
+        t["log_decay"][:, resets] = -float("inf")
+        got = run(vb, t, up)
+        compare(got, reference(t, up, 32 ** -0.5), reference(t, up, 32 ** -0.5, True), dtype, t, 32 ** -0.5)
+        assert (got[5][:, resets] == 0).all(), small

@@ -50,8 +50,8 @@ struct Cum { float n, f; };         // n + f, n whole, 0 <= f < 1: exact in n, 2
 __device__ __forceinline__ Cum cum_of(float log_decay) {
     float x = log_decay * kLog2e;
     x = x < kFloor ? kFloor : x;    // (NaN stays)
-    const float n = floorf(x);
-    return {n, x - n};
+    const float n = floorf(x), f = x - n;
+    return f >= 1.f ? Cum{n + 1.f, 0.f} : Cum{n, f};        // (x between -2^-25 and 0: its fraction rounds up)
 }
 __device__ __forceinline__ Cum cum_add(Cum a, Cum b) {
     const float f = a.f + b.f, c = f >= 1.f ? 1.f : 0.f;
@@ -670,7 +670,8 @@ __global__ void __launch_bounds__(GradShape<T, DK, DV>::kThreads, GradShape<T, D
             for (int s = 0; s < 2; ++s) {
                 const int i = 2 * lane + s;
                 // nothing crosses a reset; the pairs in front of it and behind it have cancelled to rounding only
-                const bool reset = d.n[i] - (i ? d.n[i - 1] : 0.f) <= kFloor;
+                // (neighbouring sums may have been added up in other orders, one of them with a carry more)
+                const bool reset = d.n[i] - (i ? d.n[i - 1] : 0.f) <= kFloor + 1.f;
                 if (i < rows) a.dg[((long long)b * a.L + first + i) * H + h] = reset ? 0.f : y[s];
             }
         }
