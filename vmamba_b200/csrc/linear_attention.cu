@@ -855,7 +855,6 @@ int walk(WalkArgs a, const float* first, float* last, void* workspace, long long
     launch(la_join_kernel, (unsigned)(bh * ((j.size + 255) / 256)), 256, 0, st, j);
     count_launch();
     if (const int rc = check_launch()) return rc;
-    if (!kOut && !a.states) return SS2D_OK;
     a.start = part; a.end = nullptr;
     return launch_walk<T, DK, DVT, kOut, kBack>(a, bh, st);
 }

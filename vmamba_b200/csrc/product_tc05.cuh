@@ -366,7 +366,7 @@ template <typename E> bool make_out_map(CUtensorMap* m, const void* base, long l
                CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// An operand of (rows of M or N, contraction) elements: `mn_major`: stored (contraction, rows)
+// An operand in memory: rows `pitch` elements apart, of the contraction where the kernel's kAMN / kBMN says so ("MN-major"), else of M / N
 struct Operand {
     const void* p;
     long long pitch;
