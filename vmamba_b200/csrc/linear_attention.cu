@@ -790,8 +790,11 @@ Rows rows_of(const void* p, int64_t b, int64_t l, int64_t h, int dtype) {
 }
 long long chunks_of(const ss2d_linear_attention_params& p) { return (p.seqlen + kChunk - 1) / kChunk; }
 
-// columns of v of a walking CTA: fp32 operands in pieces beside 128 rows of 64 columns of state would not stay in registers
-int slice_of(const ss2d_linear_attention_params& p) { return p.dv <= 32 || (p.dtype == SS2D_F32 && p.dk > 64) ? 32 : 64; }
+// Columns of v of a walking CTA: 64, but 32 where derived operands in fp32 (all types but bf16) beside 128 rows of 64 columns of state would not stay in registers.  fp16, us with 64 / 32,
+// forward, then a training step: 4 096 tokens of 16 heads of 128 x 128 175 / 163, 551 / 551; 16 x 784 of 24 heads of 128 x 64 283 / 254, 1 090 / 1 049, of 128 x 128 544 / 478, 2 030 / 2 028;
+// 64 x 200 of 8 heads of 128 x 64 123 / 113, 453 / 446; 4 x 1 000 of 16 heads of 96 x 80 174 / 106, 478 / 371.
+template <typename T, int DK> constexpr bool kWideSlices = std::is_same<T, __nv_bfloat16>::value || DK <= 64;
+int slice_of(const ss2d_linear_attention_params& p) { return p.dv <= 32 || (p.dtype != SS2D_BF16 && p.dk > 64) ? 32 : 64; }
 
 // Segments of a sequence: where sequences, heads and slices leave room on the chip, sequences are cut, and each segment's own state is gathered by a
 // walk of its own first.  As many as are resident at once (two CTAs an SM with 128 rows of state, four with fewer): one more round of few CTAs would take as
@@ -972,7 +975,7 @@ int linear_attention_fwd(const ss2d_linear_attention_params* p, cudaStream_t st)
             constexpr int DK = decltype(n)::value;
             const float* first = (const float*)p->initial_state;
             float* last = (float*)p->final_state;
-            if constexpr (sizeof(T) == 2 || DK <= 64)
+            if constexpr (kWideSlices<T, DK>)
                 if (slice_of(*p) == 64) return walk<T, DK, 64, true, false>(a, first, last, p->workspace, bh, st);
             return walk<T, DK, 32, true, false>(a, first, last, p->workspace, bh, st);
         });
@@ -1043,7 +1046,7 @@ int linear_attention_bwd(const ss2d_linear_attention_bwd_params* p, cudaStream_t
             constexpr int DK = decltype(n)::value;
             int rc = SS2D_OK;
             bool wide = false;
-            if constexpr (sizeof(T) == 2 || DK <= 64) {
+            if constexpr (kWideSlices<T, DK>) {
                 wide = slice_of(f) == 64;
                 if (wide && !tc) rc = walk<T, DK, 64, false, true>(w, first, last, ws, bh, st);
             }
