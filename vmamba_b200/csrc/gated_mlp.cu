@@ -361,6 +361,7 @@ Plan plan_of(long long M, long long N, long long K, bool gate, bool may_split) {
         const long long out = gate ? kFormCols[f] / 2 : kFormCols[f], at_once = 148 / kFormCtas[f];
         const long long tiles = ((M + kFormRows[f] - 1) / kFormRows[f]) * ((N + out - 1) / out);
         for (long long s = 1; s <= (may_split ? 64 : 1) && s <= steps; ++s) {
+            if (s > 1 && 4500.0 + 8.0 * s * M * N / 3300.0 >= least) break;          // (what the parts alone cost: more of them are no better)
             const long long per = (steps + s - 1) / s, splits = (steps + per - 1) / per;
             const double t = (double)((tiles * splits + at_once - 1) / at_once) * per * kFormStep[f] + (splits > 1 ? 4500.0 + 8.0 * splits * M * N / 3300.0 : 0.0);
             if (t < least) { least = t; best = {f, (int)splits, (int)per}; }
