@@ -637,3 +637,31 @@ def test_resets_behind_decays_of_almost_one(vb, dtype):
         got = run(vb, t, up)
         compare(got, reference(t, up, 32 ** -0.5), reference(t, up, 32 ** -0.5, True), dtype, t, 32 ** -0.5)
         assert (got[5][:, resets] == 0).all(), small
+
+
+# ---- fp32 results ------------------------------------------------------------------------------------------------------
+PRECISE = [(4, 1001, 8, 8, 32, 64), (2, 359, 4, 4, 16, 24), (3, 300, 1, 6, 64, 80), (1, 640, 2, 2, 128, 128), (2, 200, 2, 4, 96, 128)]
+
+
+def plain_decays(B, L, H):
+    """Step sizes of [1e-3, 1e-1] through a softplus, rates of [1, 16]: what a scan's decays look like."""
+    gen = torch.Generator().manual_seed(2)
+    dt = torch.exp(torch.rand(H, generator=gen) * 4.6 - 6.9)
+    raw = torch.randn((B, L, H), generator=gen) + torch.log(torch.expm1(dt))
+    return (-torch.nn.functional.softplus(raw) * (1 + 15 * torch.rand(H, generator=gen))).cuda()
+
+
+def relative_errors(vb, shape, dtype):
+    t, up = make(*shape, dtype)
+    t["log_decay"] = plain_decays(shape[0], shape[1], shape[3])
+    got, ref = run(vb, t, up), reference(t, up, shape[4] ** -0.5)
+    found = {n: ((x.double() - y).norm() / y.norm()).item() for n, x, y in zip(("out", "final_state", *NAMES), got, ref) if x.dtype == torch.float32}
+    print(shape, dtype, {n: f"{e:.1e}" for n, e in found.items()})
+    return found
+
+
+@pytest.mark.parametrize("shape", PRECISE, ids=str)
+def test_fp32_calls_are_as_exact_as_fp32(vb, shape):
+    """Norm against norm, at most 2^-20: sums of some hundred terms of random sign, each product 2^-22 off (two tf32 pieces), each addition 2^-24 of what it adds to."""
+    for name, e in relative_errors(vb, shape, torch.float32).items():
+        assert e <= 2.0 ** -20, (name, e)

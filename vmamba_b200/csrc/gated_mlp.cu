@@ -87,8 +87,8 @@ __global__ void __launch_bounds__(128) product_kernel(const ProductArgs p) {
                     load_b2<kBK>(b0, b1, s + S::kA + j * S::kB, S::kLdB, wn + 8 * n, k0, lane);
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        mma_exact(to[j][u][n], a[u], b0);
-                        mma_exact(to[j][u][n + 1], a[u], b1);
+                        mma_exact<false>(to[j][u][n], a[u], b0);
+                        mma_exact<false>(to[j][u][n + 1], a[u], b1);
                     }
                 }
         }
