@@ -665,3 +665,11 @@ def test_fp32_calls_are_as_exact_as_fp32(vb, shape):
     """Norm against norm, at most 2^-20: sums of some hundred terms of random sign, each product 2^-22 off (two tf32 pieces), each addition 2^-24 of what it adds to."""
     for name, e in relative_errors(vb, shape, torch.float32).items():
         assert e <= 2.0 ** -20, (name, e)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", PRECISE + [(30, 25, 1, 2, 32, 64)], ids=str)
+def test_states_of_16_bit_calls_are_as_exact_as_fp32(vb, shape, dtype):
+    """The same for the states and their gradients, fp32 results of 16-bit inputs: three pieces of bf16 (2^-25 off), two of tf32 beside fp16 (2^-23)."""
+    e = relative_errors(vb, shape, dtype)
+    assert e["final_state"] <= 2.0 ** -20 and e["initial_state"] <= 2.0 ** -20

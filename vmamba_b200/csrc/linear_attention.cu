@@ -320,13 +320,15 @@ __global__ void __launch_bounds__(128) la_walk_kernel(const WalkArgs a) {
                     values(load_a<true>(sk, M::kLdK, m_first + 64 * m, k0, lane), x);
 #pragma unroll
                     for (int s = 0; s < 8; ++s) x[s] *= ws[(s & 1) + 2 * (s >> 2)];
-                    const Derived<T, 2> kd = derive<T, 2>(x);       // two pieces: the state is an fp32 result
+                    // the state is an fp32 result: three pieces of bf16, two of tf32
+                    constexpr int kPieces = std::is_same<T, __nv_bfloat16>::value ? 3 : 2;
+                    const Derived<T, kPieces> kd = derive<T, kPieces>(x);
 #pragma unroll
                     for (int j = 0; j < NT; j += 2) {
                         OpB<T> b0, b1;
                         load_b2<true>(b0, b1, sv, M::kLdV, 8 * j, k0, lane);
-                        mma_derived<T, 2>(add[j], kd, b0);
-                        mma_derived<T, 2>(add[j + 1], kd, b1);
+                        mma_derived<T, kPieces>(add[j], kd, b0);
+                        mma_derived<T, kPieces>(add[j + 1], kd, b1);
                     }
                 }
 #pragma unroll
