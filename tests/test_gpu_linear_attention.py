@@ -673,3 +673,10 @@ def test_states_of_16_bit_calls_are_as_exact_as_fp32(vb, shape, dtype):
     """The same for the states and their gradients, fp32 results of 16-bit inputs: three pieces of bf16 (2^-25 off), two of tf32 beside fp16 (2^-23)."""
     e = relative_errors(vb, shape, dtype)
     assert e["final_state"] <= 2.0 ** -20 and e["initial_state"] <= 2.0 ** -20
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", PRECISE + [(30, 25, 1, 2, 32, 64), (1, 1500, 4, 12, 64, 32)], ids=str)
+def test_decay_gradients_of_16_bit_calls_are_as_exact_as_fp32(vb, shape, dtype):
+    """The same for the gradients of the decays: sums of products with both states, which keep their 32 bits between the passes."""
+    assert relative_errors(vb, shape, dtype)["log_decay"] <= 2.0 ** -20

@@ -102,7 +102,7 @@ __device__ __forceinline__ void load_decays(float& g0, float& g1, const float* g
     g1 = t + 1 < L ? g[(t + 1) * stride] : 0.f;
 }
 
-// A state that the gradient kernel reads: rows of `state_row(dv)` elements, 4 bytes each: beside bf16 two planes of pieces, else fp32.  What is behind dv is zero.
+// A state that the gradient kernel reads: rows of `state_row(dv)` elements, fp32.  What is behind dv is zero.
 __host__ __device__ constexpr int state_row(int dv) { return (dv + 7) / 8 * 8; }
 
 // ---- walking a sequence ------------------------------------------------------------------------------------------------
@@ -113,7 +113,7 @@ struct WalkArgs {
     const float* start;             // (B, H, segments, dk, dv) or NULL: zeros
     float* end;                     // the same, or NULL
     float* end_decay;               // (B, H, segments): log2 of the decay over the segment, or NULL
-    void* states;                   // (B, H, chunks) states (below): in front of every chunk (walking backwards: behind it), or NULL
+    float* states;                  // (B, H, chunks) states (above): in front of every chunk (walking backwards: behind it), or NULL
     void* o;                        // (B, L, H, dv)
     int H, rep, L, dk, dv, chunks, per_segment, segments, pairs;
     float scale;
@@ -184,12 +184,12 @@ __global__ void __launch_bounds__(128) la_walk_kernel(const WalkArgs a) {
                 }
             });
     };
-    auto write_planes = [&](long long which) {
+    auto keep_state = [&](long long which) {
         const int ld = state_row(a.dv);
-        P* const to = (P*)((char*)a.states + which * a.dk * ld * 4) + v0;
+        float* const to = a.states + which * a.dk * ld + v0;
         if (holds)
             for_state([&](int row, int col, float* s) {
-                if (row < a.dk && v0 + col < ld) put2<T, 2>(to + row * ld + col, a.dk * ld, s[0], s[1]);
+                if (row < a.dk && v0 + col < ld) *reinterpret_cast<float2*>(to + row * ld + col) = make_float2(s[0], s[1]);
             });
     };
     auto fetch = [&](int c, int buf) {
@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(128) la_walk_kernel(const WalkArgs a) {
         __syncthreads();
         if (i + 1 < n) fetch(chunk_at(i + 1), buf ^ 1);
         next_decays(i + 1);
-        if (a.states) write_planes((long long)bh * a.chunks + c);
+        if (a.states) keep_state((long long)bh * a.chunks + c);
         const T* sk = stage0 + buf * ((kOut ? 2 : 1) * M::kQ + M::kV);
         const T* sv = sk + M::kQ;
         if constexpr (kOut) {
@@ -385,7 +385,7 @@ struct GradArgs {
     Rows q, k, v, dy;
     const float* g;
     long long g_b, g_l, g_h;
-    const void *states, *dstates;   // (B, H, chunks) states: in front of the chunk; gradient of the state behind it
+    const float *states, *dstates;  // (B, H, chunks) states: in front of the chunk; gradient of the state behind it
     void *dq, *dk_, *dv_;           // dense
     float* dg;                      // (B, L, H)
     int G, rep, L, dk, dv, chunks, pairs_k, pairs_v;
@@ -394,22 +394,26 @@ struct GradArgs {
 
 template <typename T, int DK, int DV> struct GradShape {
     using P = typename Plane<T>::type;
-    static constexpr int kPlanes = Plane<T>::kSplit ? 2 : 1;
+    static constexpr bool kSplit = Plane<T>::kSplit;
+    static constexpr int kPlanes = kSplit ? 3 : 1;
     static constexpr int kGroups = DK == 128 || DV == 128 ? 3 : 2;      // groups of four warps: dq; dk and dv, apart where both would not stay in registers
     static constexpr int kThreads = 128 * kGroups, kSlabs = DK / kSlab;
     static constexpr int kLdK = DK + 8, kLdV = DV + 8, kLdP = kChunk + 8;
     static constexpr int kK = kChunk * kLdK, kV = kChunk * kLdV, kPair = kChunk * kLdP, kPlane = kSlab * kLdV;
     static constexpr size_t kRowBytes = (2 * kK + 2 * kV) * sizeof(T), kPairBytes = 2 * kPair * sizeof(P), kSlabBytes = 2 * kPlanes * kPlane * sizeof(P);
     static constexpr size_t kSums = (3 + 4 + 2) * kChunk * sizeof(float) + 64;
-    static constexpr size_t kFixed = kRowBytes + kPairBytes + sizeof(Decays) + kSums;
-    static constexpr int kStages = kSlabs == 1 || kFixed + 2 * kSlabBytes > 232448 ? 1 : 2;
+    static constexpr size_t kWaitBytes = kSplit ? 2 * kSlab * DV * sizeof(float) : 0;       // beside bf16: a slab in fp32, on its way into pieces
+    static constexpr size_t kFixed = kRowBytes + kPairBytes + kWaitBytes + sizeof(Decays) + kSums;
+    static constexpr int kStages = kSplit || kSlabs == 1 || kFixed + 2 * kSlabBytes > 232448 ? 1 : 2;
     static constexpr size_t kBytes = kFixed + kStages * kSlabBytes;
     static constexpr int kResident = 2 * (kBytes + 1024) <= 233472 && kGroups == 2 ? 2 : 1;
     static_assert(kBytes <= 232448);
 };
 
 // Pairs first: the 16 x 16 blocks of the lower triangle go round the warps, each gives decayed q . k and do . v, their sums by row and column, and both as operands in
-// shared memory.  Then a group of warps has dq, 16 queries a warp, another dk and dv, 16 keys a warp; the states pass in slabs of 32 rows.  Heads that share
+// shared memory.  Then a group of warps has dq, 16 queries a warp, another dk and dv, 16 keys a warp; the states pass in slabs of 32 rows, beside bf16 in three pieces: the gradients of
+// the decays are fp32 results, sums over products with both states whose terms cancel (of two pieces 2e-6 to 4e-6 from 64 bits, of three 3e-7 to 5e-7, as of elementary fp32 operations; training of 2 x 4 096
+// tokens of 16 heads of 128 x 128 459 -> 502 us, of 16 x 3 136 of 12 heads of 64 x 32 522 -> 518).  Heads that share
 // their keys follow one another with dq and dk in accumulators.
 template <typename T, int DK, int DV>
 __global__ void __launch_bounds__(GradShape<T, DK, DV>::kThreads, GradShape<T, DK, DV>::kResident) la_grad_kernel(const GradArgs a) {
@@ -420,7 +424,8 @@ __global__ void __launch_bounds__(GradShape<T, DK, DV>::kThreads, GradShape<T, D
     extern __shared__ __align__(16) unsigned char smem[];
     T *const sq = reinterpret_cast<T*>(smem), *const sk = sq + M::kK, *const sv = sk + M::kK, *const sy = sv + M::kV;
     P *const s_w = reinterpret_cast<P*>(smem + M::kRowBytes), *const s_a = s_w + M::kPair, *const slabs = s_a + M::kPair;
-    Decays& d = *reinterpret_cast<Decays*>(smem + M::kRowBytes + M::kPairBytes + M::kStages * M::kSlabBytes);
+    float* const waiting = reinterpret_cast<float*>(smem + M::kRowBytes + M::kPairBytes + M::kStages * M::kSlabBytes);
+    Decays& d = *reinterpret_cast<Decays*>(smem + M::kRowBytes + M::kPairBytes + M::kStages * M::kSlabBytes + M::kWaitBytes);
     float *const row_sum = reinterpret_cast<float*>(&d + 1), *const col_sum = row_sum + 3 * kChunk, *const into = col_sum + 4 * kChunk, *const from = into + kChunk,
                 *const cross = from + kChunk;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, t = lane & 3;
@@ -441,17 +446,27 @@ __global__ void __launch_bounds__(GradShape<T, DK, DV>::kThreads, GradShape<T, D
         if (hh) __syncthreads();
         fetch_rows<T, kChunk, DV>(sv, kLdV, src(a.v, h), a.v.l, rows, a.dv, a.v.vec, tid, kThreads);
         fetch_rows<T, kChunk, DV>(sy, kLdV, src(a.dy, h), a.dy.l, rows, a.dv, a.dy.vec, tid, kThreads);
-        const long long at = ((long long)(b * H + h) * a.chunks + c) * a.dk * ld * 4;
+        const long long at = ((long long)(b * H + h) * a.chunks + c) * a.dk * ld;
         auto fetch_slab = [&](int s) {
             if (s < n_slabs) {
-                P* to = slabs + (s % M::kStages) * (2 * M::kPlanes * M::kPlane);
 #pragma unroll
-                for (int p = 0; p < 2 * M::kPlanes; ++p) {
-                    const P* g = (const P*)((const char*)(p < M::kPlanes ? a.states : a.dstates) + at) + (p % M::kPlanes) * a.dk * ld + s * kSlab * ld;
-                    fetch_rows<P, kSlab, DV>(to + p * M::kPlane, kLdV, g, ld, a.dk - s * kSlab, ld, true, tid, kThreads);
+                for (int p = 0; p < 2; ++p) {
+                    const float* g = (p ? a.dstates : a.states) + at + s * kSlab * ld;
+                    if constexpr (M::kSplit) fetch_rows<float, kSlab, DV>(waiting + p * kSlab * DV, DV, g, ld, a.dk - s * kSlab, ld, true, tid, kThreads);
+                    else fetch_rows<float, kSlab, DV>(slabs + ((s % M::kStages) * 2 + p) * M::kPlane, kLdV, g, ld, a.dk - s * kSlab, ld, true, tid, kThreads);
                 }
             }
             commit_copies();
+        };
+        float both = 0.f;                                  // <S, dS>, this thread's share
+        auto take_slab = [&]() {                           // beside bf16: what has waited, into pieces
+            for (int i = tid; i < kSlab * DV / 2; i += kThreads) {
+                const int row = i / (DV / 2), col = i % (DV / 2) * 2;
+                const float2 x = *reinterpret_cast<const float2*>(waiting + row * DV + col), y = *reinterpret_cast<const float2*>(waiting + (kSlab + row) * DV + col);
+                both = fmaf(x.x, y.x, fmaf(x.y, y.y, both));
+                put2<T, 3>(slabs + row * kLdV + col, M::kPlane, x.x, x.y);
+                put2<T, 3>(slabs + M::kPlanes * M::kPlane + row * kLdV + col, M::kPlane, y.x, y.y);
+            }
         };
         fetch_slab(0);
         if constexpr (M::kStages == 2) fetch_slab(1);
@@ -462,6 +477,7 @@ __global__ void __launch_bounds__(GradShape<T, DK, DV>::kThreads, GradShape<T, D
         }
         wait_copies<M::kStages - 1>();
         __syncthreads();
+        if constexpr (M::kSplit) take_slab();
         {
             float sum[2] = {0.f, 0.f};
             const Cum own[2] = {d.at(r0 + gq), d.at(r0 + gq + 8)};
@@ -530,7 +546,7 @@ __global__ void __launch_bounds__(GradShape<T, DK, DV>::kThreads, GradShape<T, D
 #pragma unroll
                 for (int s = 0; s < 4; ++s) dv[j][s] = 0.f;
         }
-        float through[2] = {0.f, 0.f}, both = 0.f;
+        float through[2] = {0.f, 0.f};
         const T *const X = has_dq ? sy : sv, *const Own = has_dq ? sq : sk, *const Other = has_dq ? sk : sq;
 #pragma unroll
         for (int s = 0; s < M::kSlabs; ++s) {
@@ -539,20 +555,18 @@ __global__ void __launch_bounds__(GradShape<T, DK, DV>::kThreads, GradShape<T, D
                 if (s) {
                     wait_copies<M::kStages - 1>();
                     __syncthreads();
+                    if constexpr (M::kSplit) {
+                        take_slab();
+                        __syncthreads();
+                    }
                 }
+                if constexpr (M::kSplit) fetch_slab(s + 1);
                 const P *const s_in = slabs + (s % M::kStages) * (2 * M::kPlanes * M::kPlane), *const s_out = s_in + M::kPlanes * M::kPlane;
-                for (int i = tid; i < kSlab * DV / 2; i += kThreads) {
-                    const int at = i / (DV / 2) * kLdV + i % (DV / 2) * 2;
-                    if constexpr (Plane<T>::kSplit) {
-                        auto two = [&](const P* p) {
-                            const float2 u = Half2Of<P>::unpack(*reinterpret_cast<const uint32_t*>(p)), v = Half2Of<P>::unpack(*reinterpret_cast<const uint32_t*>(p + M::kPlane));
-                            return make_float2(u.x + v.x, u.y + v.y);
-                        };
-                        const float2 x = two(s_in + at), y = two(s_out + at);
-                        both = fmaf(x.x, y.x, fmaf(x.y, y.y, both));
-                    } else
+                if constexpr (!M::kSplit)
+                    for (int i = tid; i < kSlab * DV / 2; i += kThreads) {
+                        const int at = i / (DV / 2) * kLdV + i % (DV / 2) * 2;
                         both = fmaf(s_in[at], s_out[at], fmaf(s_in[at + 1], s_out[at + 1], both));
-                }
+                    }
                 if (has_dq || has_dk) {
                     const P* const S = has_dq ? s_in : s_out;
                     float acc[4][4] = {};
@@ -560,7 +574,7 @@ __global__ void __launch_bounds__(GradShape<T, DK, DV>::kThreads, GradShape<T, D
                     for (int k0 = 0; k0 < DV; k0 += 16) {
                         const OpA<T> x = load_a<false>(X, kLdV, r0, k0, lane);
 #pragma unroll
-                        for (int j = 0; j < 4; j += 2) mma_plane2<T, 2, false>(acc[j], acc[j + 1], x, S, M::kPlane, kLdV, 8 * j, k0, lane);
+                        for (int j = 0; j < 4; j += 2) mma_plane2<T, M::kSplit ? 3 : 2, false>(acc[j], acc[j + 1], x, S, M::kPlane, kLdV, 8 * j, k0, lane);
                     }
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
@@ -590,11 +604,13 @@ __global__ void __launch_bounds__(GradShape<T, DK, DV>::kThreads, GradShape<T, D
                         for (int j = 0; j < DV / 8; j += 2) mma_plane2<T, 1, true>(dv[j], dv[j + 1], x, s_out, M::kPlane, kLdV, 8 * j, k0, lane);
                     }
                 }
-                if (s + M::kStages < M::kSlabs) {
-                    __syncthreads();
-                    fetch_slab(s + M::kStages);
-                } else if constexpr (M::kStages == 2)
-                    commit_copies();                       // keeps the count of groups behind a slab
+                if constexpr (!M::kSplit) {
+                    if (s + M::kStages < M::kSlabs) {
+                        __syncthreads();
+                        fetch_slab(s + M::kStages);
+                    } else if constexpr (M::kStages == 2)
+                        commit_copies();                   // keeps the count of groups behind a slab
+                }
             }
         }
         if (has_dv) {
@@ -892,7 +908,7 @@ bool tc_rows(const Rows& r, long long B, long long L, long long H) {
     return r.vec && (B == 1 || r.b > 0) && (L == 1 || r.l > 0) && (H == 1 || r.h > 0) && r.b < 1LL << 38 && r.l < 1LL << 38 && r.h < 1LL << 38;
 }
 struct TcPlan { long long chunks, decay, added, states, total; };
-TcPlan tc_plan(const ss2d_linear_attention_params& p, bool train) {
+TcPlan tc_plan(const ss2d_linear_attention_params& p, bool train, bool back) {
     TcPlan t = {};
     if (!tc_shape(p)) return t;
     auto up = [](long long n) { return (n + 255) / 256 * 256; };
@@ -900,7 +916,7 @@ TcPlan tc_plan(const ss2d_linear_attention_params& p, bool train) {
     t.chunks = train ? chunks_of(p) : (p.seqlen + lat::kTile - 1) / lat::kTile;
     t.decay = up(4 * bh * t.chunks);
     t.added = up(4 * bh * t.chunks * size);
-    t.states = train ? 0 : up(2 * bh * t.chunks * size);
+    t.states = back ? 0 : up(2 * bh * t.chunks * size);         // in bf16, for the outputs; the gradients read those in fp32
     t.total = t.decay + t.added + t.states;
     return t;
 }
@@ -911,8 +927,8 @@ template <typename F> int for_tc(const ss2d_linear_attention_params& p, F&& f) {
     return p.dk <= 64 ? with(std::integral_constant<int, 64>()) : with(std::integral_constant<int, 128>());
 }
 // the states in front of all chunks (backwards: the gradients behind them), `k` and `v` as in WalkArgs
-template <bool kBack> int tc_states(const ss2d_linear_attention_params& p, const WalkArgs& w, const TcPlan& plan, bool train, const float* first, float* last, void* states,
-                                    char* ws, cudaStream_t st) {
+template <bool kBack> int tc_states(const ss2d_linear_attention_params& p, const WalkArgs& w, const TcPlan& plan, bool train, const float* first, float* last, float* states,
+                                    __nv_bfloat16* plane, char* ws, cudaStream_t st) {
     float* const added = (float*)(ws + plan.decay);
     lat::GatherArgs g = {w.g, w.g_b, w.g_l, w.g_h, (float*)ws, w.H, w.rep, w.L, w.dk, w.dv, (int)plan.chunks, w.scale, nullptr};
     const int rc = for_tc(p, [&](auto dk, auto dv) {
@@ -922,23 +938,23 @@ template <bool kBack> int tc_states(const ss2d_linear_attention_params& p, const
         return lat::gather<DK, DV, kChunk, kBack>(w.k, w.v, added, p.batch, p.n_groups, g, st);
     });
     if (rc != SS2D_OK) return rc;
-    return lat::spread({added, g.decay, first, last, (__nv_bfloat16*)states, g.chunks, w.dk, w.dv, state_row(w.dv), train ? 2 : 1, kBack}, p.batch * p.heads, st);
+    return lat::spread({added, g.decay, first, last, states, plane, g.chunks, w.dk, w.dv, state_row(w.dv), kBack}, p.batch * p.heads, st);
 }
 int tc_forward(const ss2d_linear_attention_params& p, const WalkArgs& w, cudaStream_t st) {
     const bool train = p.chunk_states != nullptr;
-    const TcPlan plan = tc_plan(p, train);
+    const TcPlan plan = tc_plan(p, train, false);
     char* const ws = (char*)p.workspace;
-    void* const states = train ? p.chunk_states : ws + plan.decay + plan.added;
-    if (const int rc = tc_states<false>(p, w, plan, train, (const float*)p.initial_state, (float*)p.final_state, states, ws, st)) return rc;
+    __nv_bfloat16* const plane = (__nv_bfloat16*)(ws + plan.decay + plan.added);
+    if (const int rc = tc_states<false>(p, w, plan, train, (const float*)p.initial_state, (float*)p.final_state, (float*)p.chunk_states, plane, ws, st)) return rc;
     lat::OutArgs o = {w.g, w.g_b, w.g_l, w.g_h, w.H, w.rep, w.L, w.dk, w.dv, (int)((p.seqlen + lat::kTile - 1) / lat::kTile), (int)plan.chunks,
                       train ? lat::kTile / kChunk : 1, w.scale, nullptr};
     const Rows out = rows_of(p.out, p.seqlen * p.heads * p.dv, p.heads * p.dv, p.dv, p.dtype);
     return for_tc(p, [&](auto dk, auto dv) {
-        return lat::outputs<decltype(dk)::value, decltype(dv)::value>(w.q, w.k, w.v, out, states, (train ? 4LL : 2LL) * w.dk * state_row(w.dv), p.batch, p.n_groups, o, st);
+        return lat::outputs<decltype(dk)::value, decltype(dv)::value>(w.q, w.k, w.v, out, plane, 2LL * w.dk * state_row(w.dv), p.batch, p.n_groups, o, st);
     });
 }
 long long fwd_workspace(const ss2d_linear_attention_params& p) {
-    const long long walk = segment_bytes(p), tc = tc_plan(p, p.chunk_states != nullptr).total;
+    const long long walk = segment_bytes(p), tc = tc_plan(p, p.chunk_states != nullptr, false).total;
     return walk > tc ? walk : tc;
 }
 
@@ -967,7 +983,7 @@ int linear_attention_fwd(const ss2d_linear_attention_params* p, cudaStream_t st)
     a.k = rows_of(p->k, p->k_batch_stride, p->k_token_stride, p->k_head_stride, p->dtype);
     a.v = rows_of(p->v, p->v_batch_stride, p->v_token_stride, p->v_head_stride, p->dtype);
     a.o = p->out;
-    a.states = p->chunk_states;
+    a.states = (float*)p->chunk_states;
     if (tc_shape(*p) && aligned_to(p->out, 16) && tc_rows(a.q, p->batch, p->seqlen, p->n_groups) && tc_rows(a.k, p->batch, p->seqlen, p->n_groups) &&
         tc_rows(a.v, p->batch, p->seqlen, p->heads))
         return tc_forward(*p, a, st);
@@ -988,7 +1004,7 @@ namespace {
 struct BwdPlan { long long segments, dstates, total; };
 BwdPlan bwd_plan(const ss2d_linear_attention_params& p) {
     BwdPlan b = {};
-    const long long walk = (segment_bytes(p) + 255) / 256 * 256, tc = tc_plan(p, true).total;
+    const long long walk = (segment_bytes(p) + 255) / 256 * 256, tc = tc_plan(p, true, true).total;
     b.segments = walk > tc ? walk : tc;
     b.dstates = states_bytes(p);
     b.total = b.segments + b.dstates;
@@ -1023,7 +1039,7 @@ int linear_attention_bwd(const ss2d_linear_attention_bwd_params* p, cudaStream_t
     if (!p->workspace || p->workspace_bytes < plan.total || !aligned_to(p->workspace, 16)) return SS2D_EWORKSPACE;
     const long long bh = f.batch * f.heads;
     char* ws = (char*)p->workspace;
-    void* dstates = ws + plan.segments;
+    float* dstates = (float*)(ws + plan.segments);
     WalkArgs w = walk_args(f);
     w.k = rows_of(f.q, f.q_batch_stride, f.q_token_stride, f.q_head_stride, f.dtype);
     w.v = rows_of(p->dout, p->dout_batch_stride, p->dout_token_stride, p->dout_head_stride, f.dtype);
@@ -1033,7 +1049,7 @@ int linear_attention_bwd(const ss2d_linear_attention_bwd_params* p, cudaStream_t
     a.k = rows_of(f.k, f.k_batch_stride, f.k_token_stride, f.k_head_stride, f.dtype);
     a.v = rows_of(f.v, f.v_batch_stride, f.v_token_stride, f.v_head_stride, f.dtype);
     a.g = w.g; a.g_b = w.g_b; a.g_l = w.g_l; a.g_h = w.g_h;
-    a.states = f.chunk_states; a.dstates = dstates;
+    a.states = (const float*)f.chunk_states; a.dstates = dstates;
     a.dq = p->dq; a.dk_ = p->dk; a.dv_ = p->dv; a.dg = (float*)p->dlog_decay;
     a.G = (int)f.n_groups; a.rep = w.rep; a.L = w.L; a.dk = w.dk; a.dv = w.dv; a.chunks = w.chunks; a.scale = f.scale;
     a.pairs_k = a.dk % 2 == 0; a.pairs_v = a.dv % 2 == 0;
@@ -1041,7 +1057,7 @@ int linear_attention_bwd(const ss2d_linear_attention_bwd_params* p, cudaStream_t
     float* last = (float*)p->dinitial_state;
     const bool tc = tc_shape(f) && tc_rows(w.k, f.batch, f.seqlen, f.n_groups) && tc_rows(w.v, f.batch, f.seqlen, f.heads);
     if (tc)
-        if (const int rc = tc_states<true>(f, w, tc_plan(f, true), true, first, last, dstates, ws, st)) return rc;
+        if (const int rc = tc_states<true>(f, w, tc_plan(f, true, true), true, first, last, dstates, nullptr, ws, st)) return rc;
     return for_type(f.dtype, [&](auto z) {
         using T = decltype(z);
         return for_dk(f.dk, [&](auto n) {

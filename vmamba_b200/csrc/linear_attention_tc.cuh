@@ -242,8 +242,9 @@ struct SpreadArgs {
     const float *added, *decay; // (B, H, chunks, dk, ld), (B, H, chunks)
     const float* first;         // (B, H, dk, dv) or NULL
     float* last;                // the same, or NULL
-    __nv_bfloat16* states;      // (B, H, chunks) of one or two planes (dk, ld)
-    int chunks, dk, dv, ld, planes;
+    float* states;              // (B, H, chunks, dk, ld) or NULL: for the gradients
+    __nv_bfloat16* plane;       // the same rounded, or NULL: for the outputs
+    int chunks, dk, dv, ld;
     bool back;
 };
 // Four neighbouring elements a thread, eight chunks read ahead (sixteen: 47 us in place of 39 at 129 chunks of 16 heads of 128 x 128; two groups of four in turn: 65)
@@ -271,14 +272,9 @@ __global__ void __launch_bounds__(128) la_spread_kernel(const SpreadArgs a) {
 #pragma unroll
         for (int i = 0; i < kAhead; ++i)
             if (i0 + i < a.chunks) {
-                __nv_bfloat16* const to = a.states + at(i0 + i) * a.planes * size + e;
-                const uint32_t h0 = Half2Of<__nv_bfloat16>::pack(s[0], s[1]), h1 = Half2Of<__nv_bfloat16>::pack(s[2], s[3]);
-                *reinterpret_cast<uint2*>(to) = make_uint2(h0, h1);
-                if (a.planes == 2) {
-                    const float2 u = Half2Of<__nv_bfloat16>::unpack(h0), v = Half2Of<__nv_bfloat16>::unpack(h1);
-                    *reinterpret_cast<uint2*>(to + size) =
-                        make_uint2(Half2Of<__nv_bfloat16>::pack(s[0] - u.x, s[1] - u.y), Half2Of<__nv_bfloat16>::pack(s[2] - v.x, s[3] - v.y));
-                }
+                if (a.states) *reinterpret_cast<float4*>(a.states + at(i0 + i) * size + e) = make_float4(s[0], s[1], s[2], s[3]);
+                if (a.plane)
+                    *reinterpret_cast<uint2*>(a.plane + at(i0 + i) * size + e) = make_uint2(Half2Of<__nv_bfloat16>::pack(s[0], s[1]), Half2Of<__nv_bfloat16>::pack(s[2], s[3]));
                 const float k = ex2_approx(d[i]);
                 s[0] = fmaf(k, s[0], x[i].x); s[1] = fmaf(k, s[1], x[i].y); s[2] = fmaf(k, s[2], x[i].z); s[3] = fmaf(k, s[3], x[i].w);
             }
