@@ -561,7 +561,7 @@ int ss2d_linear_attention_step(const ss2d_linear_attention_step_params *p, void 
  *   [v g] = x w1^T + b1;  h = v * act(g);  y = h w2^T + b2
  * x: (tokens, channels), rows x_row_stride elements apart; w1: (2 hidden, channels), the rows of the values first; w2: (outputs, hidden); b1 (2 hidden) and
  * b2 (outputs) or NULL; y: (tokens, outputs).  All of `dtype`; dense but for x's rows.  act: 1 GELU (erf), 2 SiLU.  h: (tokens, hidden) of `dtype`,
- * written by the forward call, 16-byte aligned.  workspace: ss2d_gated_mlp_workspace_bytes() bytes, 16-byte aligned (0: none), a size of the shape alone.  Sums are fp32; no atomics: repeated calls give bit-identical results.
+ * written by the forward call, 16-byte aligned.  Up to 4 194 240 tokens, channels and outputs and 2 097 088 hidden (else SS2D_ENOTSUP).  workspace: ss2d_gated_mlp_workspace_bytes() bytes, 16-byte aligned (0: none), a size of the shape alone.  Sums are fp32; no atomics: repeated calls give bit-identical results.
  * -------------------------------------------------------------------------------- */
 typedef struct ss2d_gated_mlp_params {
     const void *x, *w1, *b1, *w2, *b2;

@@ -23,7 +23,7 @@ struct ProductArgs {
     int per_split;          // contraction elements of a split (a multiple of the step)
     EpiArgs e;
 };
-// fp32 and what TMA cannot read.  1 001 tokens of 192 channels, 768 hidden, fp32: 25 us for value and gate, of which three tf32 products for each would take 10 at 512
+// fp32 and what TMA cannot read.  1 001 tokens of 192 channels, 768 hidden, fp32: 26 us for value and gate, of which three tf32 products for each would take 10 at 512
 // multiplications a cycle and SM.  Taking operands apart once for all their products and reading them in pairs changed nothing (25 us).
 constexpr int kTile = 64, kStep = 32, kRing = 3;
 
@@ -116,8 +116,9 @@ __global__ void __launch_bounds__(128) product_kernel(const ProductArgs p) {
 // ---- few tokens ---------------------------------------------------------------------------------------------------------
 // Up to 16 tokens of 16-bit types: the weights' way from memory is the whole time, and every SM has to take part in it.  A CTA has kRows rows of the weights (of value and
 // gate alike), its eight warps every eighth 32 elements of them, straight from memory into the A operand of mma.sync: a lane reads 16 bytes, 8 contraction elements in a row,
-// and the products take them in that order (the tokens' elements come the same way).  The warps' sums meet in shared memory.  us of both launches with 1 / 8 / 16 tokens, and
-// of the tensor-core kernels with 33: 768 channels and 2 048 hidden 9.3 / 9.0 / 12.4, 15.9; 384 and 1 536 5.4 / 5.9 / 8.8, 14.0; 1 024 and 4 096, from memory, 18 / 18 / 24, 19.
+// and the products take them in that order (the tokens' elements come the same way).  The warps' sums meet in shared memory.  us of both launches in a
+// graph, eight sets of weights in turn, with 1 / 8 / 16 tokens, and of the tensor-core kernels with 33: 768 channels and 2 048 hidden 9.2 / 9.1 / 11.9, 16.1; 384 and 1 536 5.5 / 5.9 / 8.9, 14.1;
+// 1 024 and 4 096, more than L2 holds, 18 / 19 / 24, 19.
 constexpr int kFew = 16;
 struct FewArgs {
     const void *x, *w, *bias;
@@ -346,8 +347,8 @@ bool tc_forward_fits(const ss2d_gated_mlp_params& p) { return tc_fits(p) && alig
 // Tiles of the tensor-core kernels: 128 x 128, 128 x 256 (in TMEM; EPI_GATE gives half as many columns) by one CTA, 256 x 256 by two.
 enum Form { kNarrow, kWide, kPair, kForms };
 constexpr int kFormRows[kForms] = {128, 128, 256}, kFormCols[kForms] = {128, 256, 256}, kFormCtas[kForms] = {1, 1, 2};
-// Cycles that a step of 64 of the contraction takes them, measured with all SMs at it (us of h / y / dx of 16 384 tokens, 1 024 channels and 2 728 hidden: 194 / 121 / 189,
-// 132 / 114 / 164, 119 / 87 / 134; of 6 272, 384 and 1 536: 22.0 / 11.5 / 18.1, 16.9 / 15.1 / 21.7, 21.0 / 14.6 / 20.9: rounds of tiles over the SMs decide there).
+// Cycles that a step of 64 of the contraction takes them, measured with all SMs at it (kernel times in us of h / y / dx of 16 384 tokens, 1 024 channels and 2 728 hidden: 201 / 122 / 195,
+// 138 / 112 / 167, 126 / 85 / 137; of 6 272, 384 and 1 536: 24.0 / 12.4 / 19.6, 19.3 / 15.3 / 22.8, 23.7 / 15.1 / 22.2: rounds of tiles over the SMs decide there).
 constexpr double kFormStep[kForms] = {660, 950, 800};
 
 struct Plan { int form, splits, per_split; };

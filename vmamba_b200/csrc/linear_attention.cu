@@ -24,9 +24,9 @@
 // linear_attention_tc.cuh in place of the walk.
 //
 // What bounds them (B200): the walk issues some 10 instructions for each matrix instruction and its warps wait for one another at two barriers a chunk (issue 55 %, tensor
-// pipe 33 %, DRAM 5 % of their rates at 16 x 784 tokens of 24 heads of 64 x 32, fp16: 76 us, 8 of them for its bytes); la_grad waits at barriers for loads of a chunk that nothing
-// overlaps but the other CTA of the SM (issue 39 %, tensor pipe 18 %, DRAM 16 % at 16 x 3 136 tokens of 12 heads of 64 x 32: 264 us, of which 114 are loads, decays, barriers and
-// stores, 55 the pairs, 65 the products with the states); la_step is a copy of the state (128 sequences of 16 heads of 128 x 128: 52 us, 5.2 TB/s, 0.79 of the copy rate).
+// pipe 33 %, DRAM 5 % of their rates at 16 x 784 tokens of 24 heads of 64 x 32, fp16: 75 us, 8 of them for its bytes); la_grad waits at barriers for loads of a chunk that nothing
+// overlaps but the other CTA of the SM (issue 38 %, tensor pipe 20 %, DRAM 16 % at 16 x 3 136 tokens of 12 heads of 64 x 32: 268 us; when states came in two pieces, 264, of which
+// 114 were loads, decays, barriers and stores, 55 the pairs, 65 the products with the states); la_step is a copy of the state (128 sequences of 16 heads of 128 x 128: 52 us, 5.2 TB/s, 0.79 of the copy rate).
 #include "mma_tiles.cuh"
 
 namespace ss2d {
@@ -816,9 +816,9 @@ int slice_of(const ss2d_linear_attention_params& p) { return p.dv <= 32 || (p.dt
 
 // Segments of a sequence: where sequences, heads and slices leave room on the chip, sequences are cut, and each segment's own state is gathered by a
 // walk of its own first.  As many as are resident at once (two CTAs an SM with 128 rows of state, four with fewer): one more round of few CTAs would take as
-// long as all others.  us with 1 / 2 / 3 / 4 / 8 / 12 segments: 16 385 tokens of 16 heads of 128 x 128, forward 1134 / 873 / 587 / 448 / 288 / 349 (9 of them: 257);
-// 2 x 4 096 tokens, training 845 / 713 / 666 / 573 / 586 / 611 (4); 16 x 3 136 tokens of 12 heads of 64 x 32, training 550 / 543 / 488 / 513 / 502 / 505 (3);
-// 16 x 784 tokens of 24 heads, forward 73 / 115 / 113 / 111 (1).
+// long as all others.  us with 1 / 2 / 3 / 4 / 8 / 9 / 12 segments (the one that the rule takes in brackets), bf16: 16 385 tokens of 16 heads of 128 x 128, forward 1 311 / 1 000 / 675 / 515 /
+// 343 / 306 / 433 (9); 2 x 4 096 tokens, training 859 / 755 / 703 / 607 / 622 / 622 / 648 (4); 16 x 3 136 tokens of 12 heads of 64 x 32, training 566 / 570 / 517 / 540 / 531 / 529 / 531 (3);
+// 16 x 784 tokens of 24 heads, fp16, forward 80 / 122 / 120 / 116 / 118 / 118 / 118 (1).
 long long room_of(const ss2d_linear_attention_params& p) {
     return 148 * (p.dk > 64 ? 2 : 4) / (p.batch * p.heads * ((p.dv + slice_of(p) - 1) / slice_of(p)));
 }
@@ -892,10 +892,10 @@ WalkArgs walk_args(const ss2d_linear_attention_params& p) {
 
 // ---- long bf16 sequences on the tensor cores of linear_attention_tc.cuh ---------------------------------------------------
 // By the shape; the workspace follows it.  The walk moves less and is one launch where it need not be cut; these kernels win where a walk would be cut (room for
-// twice its CTAs), and with wide heads from 8 chunks on.  us of the walk / these, forward, then a training step: 4 096 tokens of 16 heads of 128 x 128 79 / 41, 306 / 227,
-// of 64 x 64 36 / 26, 117 / 98, of 64 x 32 25 / 25, 96 / 97; 16 x 3 136 of 12 heads of 128 x 128 482 / 322, 2 329 / 1 948, of 128 x 64 271 / 237, 1 439 / 1 315, of 64 x 64
-// 201 / 160, 760 / 694, of 64 x 32 120 / 141; 16 x 784 of 24 heads of 128 x 64 133 / 135, 766 / 696, of 64 x 64 67 / 95, 345 / 374; 64 x 200 of 8 heads of 128 x 128
-// 92 / 86, 448 / 427, of 128 x 64 49 / 60, 284 / 281.
+// twice its CTAs), and with wide heads from 8 chunks on.  us of the walk / these, forward, then a training step: 4 096 tokens of 16 heads of 128 x 128 97 / 48, 323 / 254,
+// of 64 x 64 43 / 33, 124 / 111, of 64 x 32 32 / 32, 93 / 95; 16 x 3 136 of 12 heads of 128 x 128 624 / 341, 2 345 / 2 095, of 128 x 64 322 / 257, 1 480 / 1 401, of 64 x 64
+// 224 / 177, 785 / 754, of 64 x 32 142 / 159, 572 / 596; 16 x 784 of 24 heads of 128 x 64 174 / 152, 779 / 752, of 64 x 64 119 / 108, 388 / 412; 64 x 200 of 8 heads of 128 x 128
+// 116 / 101, 462 / 474, of 128 x 64 60 / 71, 296 / 311.
 constexpr int kLongChunks = 4;
 bool tc_shape(const ss2d_linear_attention_params& p) {
     const long long chunks = chunks_of(p);

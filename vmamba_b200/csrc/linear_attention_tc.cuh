@@ -1,8 +1,8 @@
 // Long bf16 sequences of the linear attention on the 5th-generation tensor cores, no chunk waiting for the one in front of it: what each chunk adds to the state
 // (la_gather), the states in front of the chunks by one pass over them (la_spread), and the outputs (la_outputs).  The walk of linear_attention.cu moves fewer bytes (q, k, v
 // once, no state), but its chunks follow one another through barriers and some 10 instructions for each matrix instruction; here the CUDA cores do no more than
-// weight the keys, decay the pairs and add up.  16 385 tokens of 16 heads of 128 x 128: la_gather 53 us (DRAM 49 % of its rate), la_spread 38 (55 %), la_outputs 66 (59 %), the walk
-// 257 in all; 41 for the bytes of q, k, v and outputs alone.  What is left is the latency of each CTA's own chain, loads, weights, products, stores, with two CTAs an SM.
+// weight the keys, decay the pairs and add up.  16 385 tokens of 16 heads of 128 x 128: la_gather 61 us (DRAM 43 % of its rate), la_spread 38 (57 %), la_outputs 65 (58 %), the walk
+// 306 in all; 41 for the bytes of q, k, v and outputs alone.  What is left is the latency of each CTA's own chain, loads, weights, products, stores, with two CTAs an SM.
 //
 // A tile of tokens comes by TMA as rows of 64 elements with the 128-byte swizzle.  Contractions over tokens read it as an MN-major operand, those over dk as a
 // K-major one, so that nothing is transposed.  dk fills 64 or 128 rows, dv 64 or 128 columns; what is missing is read as zeros.
@@ -295,6 +295,8 @@ struct OutArgs {
     float scale;
     int* error_flag;
 };
+// Two roundings to bf16 in front of the outputs' own: the pairs' weights and the state that the queries meet, one piece each.  Outputs are 1.4 times as far from 64 bits as one
+// rounding (2.4e-3 for 1.7e-3, 2-norm); a second piece of both would double the products and bring 40 KB more into a CTA for what the outputs' own rounding hides.
 // The pairs take the place of the keys, v that of the queries, once these have been read; with both sides of 64 v has its own place, the products with the state wait
 // for the pairs to have left TMEM and take half their columns: 96 to 128 KB and 256 columns become 96 KB and 256, or 72 KB and 128, and two or three CTAs share an SM.
 template <int DK, int DV> struct OutSmem {

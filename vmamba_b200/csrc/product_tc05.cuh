@@ -15,8 +15,9 @@
 // contraction) that takes the tensor core 256 cycles, and gets them in 650.  Pairs of CTAs (kPair) share a tile of 256 rows, each with its own half of A's rows and of
 // B's: 32 KB for 128 x 256 results, in place of 48.
 //
-// Rates (bf16): 8 192 tokens, 1 024 channels, 4 096 hidden, both launches of the forward call 148 us, 1 394 TFLOP/s, 0.84 of the measured peak (library products without the
-// activation 150); 12 544, 512, 2 048 72 us, 1 098 (73); tensor pipe 60 % active there, DRAM 4 to 20 %.
+// Rates (bf16, both launches of the forward call, GELU and biases; library products of these sizes, which leave both out, in brackets): 8 192 tokens, 1 024 channels, 4 096 hidden, a
+// call at a time 155 us (148), 200 in a row 163 (171), 1 270 TFLOP/s, 0.91 of the measured sustained rate; 12 544, 512, 2 048 in a row 81 (82), 970 TFLOP/s; kernels alone 51 and 29, tensor
+// pipe 54 and 58 % active, DRAM 4 and 20 %, the second one 98 tiles on 74 pairs of CTAs, two rounds for 1.3.
 //
 // Every wait is bounded; one that runs out raises the device's error flag (tc05.cuh), all roles leave and the TMEM is freed.
 #pragma once

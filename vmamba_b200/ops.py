@@ -191,7 +191,9 @@ def linear_attention_fn(q, k, v, log_decay, scale=None, initial_state=None, retu
     (what lies below -138 does).  Positive ones let it grow: results are as exact while the weights exp(sum of log decays) from any token to any later one of its block of 128 are
     numbers of float32, and inf or NaN behind the first that is not.  scale: default dk ** -0.5.  initial_state: (batch, heads, dk, dv), default zeros.
     Returns o (batch, tokens, heads, dv) of v's dtype; with `return_final_state` also the state behind the last token, float32.  Differentiable in
-    all tensors; the backward pass keeps the inputs and the state in front of every 64th token.  Repeated calls give bit-identical results.
+    all tensors, once (no forward mode, no second derivatives); the backward pass keeps the inputs and the state in front of every 64th token, float32, and computes all gradients.  Repeated
+    calls give bit-identical results.  Inputs of 16 bits: outputs and their gradients meet one more rounding to that type on the way (weights of pairs, states); states and the decays'
+    gradients come in float32's accuracy.  No casts under autocast.
 
     Sequences of other lengths in one batch: k = 0 and log_decay = 0 on the padding leave the state as it is.  A value (of v) that is not finite reaches its column's outputs
     from the first token of its block of 128 tokens on, which is up to 127 tokens in front of it, and may reach any gradient of its block; queries, keys and decays that are not finite
@@ -513,8 +515,9 @@ def gated_mlp_fn(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, b1=None, b
 
     x: (..., channels), w1: (2 * hidden, channels), w2: (outputs, hidden), b1: (2 * hidden,) or None, b2: (outputs,) or None, all of one dtype (float32, float16,
     bfloat16); act: "gelu" (erf) or "silu".  Returns (..., outputs).  Both projections, the activation and the product are one kernel; sums are fp32, the
-    hidden map is rounded to the inputs' type.  Differentiable in all tensors; the backward pass keeps x and the hidden map and
-    computes v and g again.  Repeated calls give bit-identical results."""
+    hidden map and the gradients of v and g are rounded to the inputs' type.  Differentiable in all tensors, once (no forward mode, no second derivatives); the backward pass keeps x and
+    the hidden map and computes v and g again.  Repeated calls give bit-identical results.  No casts under autocast: float32 weights of 16-bit tokens are the caller's to cast.  Up to
+    4 194 240 tokens, channels and outputs, 2 097 088 hidden."""
     if act not in ("gelu", "silu"):
         raise ValueError(f"unknown activation {act!r}: expected 'gelu' or 'silu'")
     return _host.gated_mlp_fn(x, w1, w2, b1, b2, _ACTS[act])
