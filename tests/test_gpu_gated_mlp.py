@@ -416,3 +416,19 @@ def test_large_calls(vb, shape, dtype, act):
     del ref
     again = run(vb, t, dy, act)
     assert all(torch.equal(got[n], again[n]) for n in got)
+
+
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("kernels", ["many_tokens", "few_tokens", "unaligned"])
+def test_gates_of_any_size(vb, kernels, dtype, act):
+    """Up to the type's largest: the activation is the gate or zero, its derivative one or zero."""
+    top = 15 if dtype == torch.float16 else 126
+    g = torch.tensor([s * 2.0 ** e for e in range(7, top + 1, 1 if top == 15 else 7) for s in (1, -1)], device="cuda").to(dtype)
+    g = torch.cat((g, torch.ones(20, device="cuda", dtype=dtype)))
+    per = 13 if kernels == "few_tokens" else g.numel()
+    parts = [single_gates(vb, c, act, offset=1 if kernels == "unaligned" else 0) for c in g.split(per)]
+    y, dv, dg = (torch.cat(p)[:-20] for p in zip(*parts))
+    g = g[:-20]
+    for x, yes in ((y, g), (dv, g), (dg, torch.ones_like(g))):
+        assert torch.equal(x, torch.where(g > 0, yes, torch.zeros_like(yes)))

@@ -22,7 +22,7 @@ struct EpiArgs {
 // the negative side, where 1/2 - 1/2 tanh and 1/2 + 1/2 erf would leave no digits of them.
 template <int ACT> __device__ __forceinline__ void gate_act_grad(float g, float& a, float& da) {
     if constexpr (ACT == ACT_GELU) {
-        const float phi = normcdff(g), h = g * g, rest = fmaf(g, g, -h);        // g^2 in two pieces: an exponent's rounding is the result's
+        const float phi = normcdff(g), h = g * g, rest = h < 1e8f ? fmaf(g, g, -h) : 0.f;       // g^2 in two pieces: an exponent's rounding is the result's
         a = g * phi;
         da = fmaf(g * 0.3989422804014327f, expf(-0.5f * h) * fmaf(-0.5f, rest, 1.0f), phi);
     } else {
