@@ -2,9 +2,9 @@
 // elements a step, fp32 accumulators.
 //
 // Two kinds of operand.  What is read as the caller's type is exact: 16-bit elements go to the 16-bit form as they are, fp32 ones are taken as
-// the sum of two tf32 halves, three products for one (22 bits; the product of the low halves is below fp32's rounding).  What a kernel has
+// the sum of two tf32 halves, three products for one (22 bits; the product of the low halves, 2^-22 at most, is left out).  What a kernel has
 // computed in fp32 ("derived") is rounded for the product, into `kParts` pieces of the form's type: one where the result is a 16-bit map whose own rounding is
-// as large, two where an fp32 result follows.  A derived operand beside fp16 goes as tf32 and not as fp16: the same 11 bits, but fp32's range
+// as large, as many as fp32 has where an fp32 result follows: three of bf16, two of tf32.  A derived operand beside fp16 goes as tf32 and not as fp16: the same 11 bits, but fp32's range
 // (a state sums over the tokens and has no bound of fp16).
 //
 // The contraction order of the tf32 form is permuted in pairs (element 2t of 8 in place of t, 2t + 1 in place of t + 4, t the lane's quad
