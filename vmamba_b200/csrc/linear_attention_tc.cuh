@@ -149,6 +149,7 @@ __global__ void __launch_bounds__(kThreads) la_gather_kernel(const __grid_consta
     tc_fence_after();
     const uint32_t tmem = *slot;
     bool ok = mbar_wait_prompt(loaded, 0, abort_flag);
+    int commits = 0;                                                    // of the thread that issues them
     constexpr int kUnits = DK / 64 * M::kBlock / 16 / kThreads;         // 8 elements each, of a thread
     uint4 second[kUnits];
     if (ok) {
@@ -185,6 +186,7 @@ __global__ void __launch_bounds__(kThreads) la_gather_kernel(const __grid_consta
 #pragma unroll
         for (int k = 0; k < kTokens / 16; ++k) tc_mma(tmem, low + k * 128, v + k * 128, idesc, k > 0);
         tc_commit(done);
+        commits = 1;
     }
     ok = ok && mbar_wait_prompt(done, 0, abort_flag);
     __syncwarp();
@@ -200,6 +202,7 @@ __global__ void __launch_bounds__(kThreads) la_gather_kernel(const __grid_consta
 #pragma unroll
         for (int k = 0; k < kTokens / 16; ++k) tc_mma(tmem, high + k * 128, v + k * 128, idesc, 1);
         tc_commit(done);
+        commits = 2;
     }
     ok = ok && mbar_wait_prompt(done, 1, abort_flag);
     __syncwarp();
@@ -230,6 +233,10 @@ __global__ void __launch_bounds__(kThreads) la_gather_kernel(const __grid_consta
         }
         if (lane == 0) store_boxes_done();
         __syncwarp();
+    }
+    if (tid == 0 && !ok) {
+        mbar_drain(loaded, 0);
+        if (commits) mbar_drain(done, commits - 1);
     }
     tc_fence_before();
     __syncthreads();
@@ -350,6 +357,7 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && DV == 64 ? 3 : 2) la_out
     const uint32_t tmem = *slot;
     const uint32_t base = smem_u32(sm);
     bool ok = true;
+    bool pending[5] = {true, true, false, false, M::kSmall};                        // barriers that something is on its way to (of the thread that sends it)
     auto with_states = [&] {                                                        // queries times the state in front
         constexpr uint32_t idesc = instr_desc(1, false, 128, DV) | (1u << 16);
         const uint64_t q = smem_desc(base + M::kQ, 16, 1024, kSw128), s = smem_desc(base + M::kS, DK * 128, 1024, kSw128);
@@ -372,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && DV == 64 ? 3 : 2) la_out
                 tc_mma(tmem, q + off, k + off, idesc, i > 0);
             }
             if constexpr (!M::kSmall) ok = with_states();
-            if (ok) tc_commit(bars + 2);
+            if (ok) { tc_commit(bars + 2); pending[2] = true; }
         }
     }
     // pairs of different blocks of 32 tokens: one exponential a token (as in the walk)
@@ -389,6 +397,7 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && DV == 64 ? 3 : 2) la_out
             mbar_expect_tx(bars + 4, DV / 64 * M::kBlock);
 #pragma unroll
             for (int i = 0; i < DV / 64; ++i) tma_load_4d(sm + M::kV + i * M::kBlock, &tmV, 64 * i, first, h, b, bars + 4);
+            pending[4] = true;
         }
     __syncwarp();
     tc_fence_after();
@@ -439,6 +448,7 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && DV == 64 ? 3 : 2) la_out
 #pragma unroll
             for (int i = 0; i < kTile / 16; ++i) tc_mma(tmem, p + ((uint64_t)(i / 4 * M::kBlock + i % 4 * 32) >> 4), v + i * 128, idesc, i > 0);
             tc_commit(bars + 3);
+            pending[3] = true;
         }
     }
     ok = ok && mbar_wait_prompt(bars + 3, 0, abort_flag);
@@ -473,6 +483,11 @@ __global__ void __launch_bounds__(kThreads, DK == 64 && DV == 64 ? 3 : 2) la_out
         const int x = DV == 128 ? (warp >> 2) * 64 : 0, y = first + 32 * quarter;
         if (x < a.dv && y < a.L) tma_store_4d(&tmO, sm + M::kP + warp * 4096, x, y, h, b);
         store_boxes_done();
+    }
+    if (tid == 0 && !ok) {
+#pragma unroll
+        for (int i = 0; i < 5; ++i)
+            if (pending[i]) mbar_drain(bars + i, 0);
     }
     tc_fence_before();
     __syncthreads();

@@ -162,11 +162,18 @@ product_tc05_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                     next();
                 }
             }
+            const int last = s, rounds = round;
             // what is in flight has been read, and the other CTA's last arrivals are here, before this one leaves
             for (int j = 0; ok && j < NS; ++j) {
                 if (round > 0) ok = mbar_wait_prompt(empty + s, (round - 1) & 1, abort_flag);
                 next();
             }
+            // or, where this CTA has given up, has arrived (of a pair the first CTA's barriers count both)
+            if (!ok && rank == 0)
+                for (int j = 0; j < NS; ++j) {
+                    const int sent = rounds + (j < last);
+                    if (sent > 0) mbar_drain(full + j, (sent - 1) & 1);
+                }
         }
     } else if (warp == 1) {
         // ---------------------------------------------------------------- MMA issuer

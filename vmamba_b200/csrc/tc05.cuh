@@ -77,6 +77,14 @@ __device__ __forceinline__ bool mbar_wait_prompt(uint64_t* bar, uint32_t parity,
     return false;
 }
 
+// In front of leaving a kernel that has given up: what is in flight may still write into shared memory or TMEM, which the next CTA on the SM will have.  Waits for it,
+// two seconds at most, whatever the other roles do.
+__device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
+    const unsigned long long t0 = global_ns();
+    while (!mbar_try_wait(bar, parity))
+        if (global_ns() - t0 > 2000000000ull) return;
+}
+
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
                  ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y) : "memory");
